@@ -583,6 +583,59 @@ int lo_moe_fused_gate(const void *input, int dtype, const void *bias, int bias_d
                       double routed_scaling_factor, int apply_routed_scaling_factor_on_output,
                       float *topk_weights, void *topk_indices, int idx_dtype, lo_stream_t stream);
 
+/* ---- 8-bit operators beside the routed int8 experts --------------------------------------------------
+ * e4m3: OCP 8-bit floating point (torch.float8_e4m3fn), one fp32 scale for 128 values of a row:
+ *   top = max(max|v|, eps), scale = top / 448, code = e4m3(448 v / top), to nearest, ties to even.
+ * A NaN keeps its code and is left out of the maximum; an infinity makes its group's scale infinite. */
+enum { LO_Q_INT8_ROWS = 0, LO_Q_INT8_GROUPS = 1, LO_Q_FP8_GROUPS = 2 };
+
+/*
+ * RMS norm with the residual's addition and an 8-bit output: the producer of the quantised rows that
+ * lo_fused_experts_channel_int8_prequant (int8.py:291-293), lo_moe_gemm_block_int8 and lo_gemm_w8a8_fp8_block take.
+ *   z = x + residual, y = z * (mean(z^2) + eps)^-1/2 * weight, in fp32
+ *   x, residual [M, H] rows of `dtype` x_stride / residual_stride values apart (multiples of 16 bytes); residual may be NULL
+ *   weight [H] of `dtype` or LO_F32;  M >= 0, H <= 65536, a multiple of 128 (LO_Q_INT8_ROWS: of 8)
+ *   residual_out [M, H]: z rounded once; may be x or residual itself where that is contiguous.  Not written without residual
+ *   normed_out [M, H] or NULL: y rounded once;  q [M, H], scale: codes of the fp32 y
+ *   q_form  LO_Q_INT8_ROWS: scale [M], the rule of lo_per_token_quant_int8
+ *           LO_Q_INT8_GROUPS: scale [M, H/128], the rule of lo_per_token_group_quant_int8 (eps 1e-10)
+ *           LO_Q_FP8_GROUPS: scale [M, H/128], e4m3 codes (eps 1e-10)
+ */
+int lo_rms_norm_quant(const void *x, int dtype, int64_t x_stride, const void *residual, int64_t residual_stride,
+                      const void *weight, int weight_dtype, int64_t M, int64_t H, float eps, int q_form,
+                      void *residual_out, void *normed_out, void *q, float *scale, lo_stream_t stream);
+
+/* e4m3 codes q [rows, cols] and scales s [rows, cols/128] of x [rows, cols] (bf16, fp16 or fp32); eps from 1e-30 up. */
+int lo_per_token_group_quant_fp8(const void *x, int dtype, int64_t rows, int64_t cols, float eps, void *q, float *s,
+                                 lo_stream_t stream);
+
+/* The same of act(c1[:, :I]) * c1[:, I:], c1 [rows, 2I], computed in fp32 (eps 1e-10). */
+int lo_act_mul_group_quant_fp8(const void *c1, int dtype, int activation, int64_t rows, int64_t I, void *q, float *s,
+                               lo_stream_t stream);
+
+/*
+ * c[m, n] = sum over kb of (a[m, kb] . b[n, kb]) * a_scale[m, kb] * b_scale[n / 128, kb] over K blocks of 128.
+ *   a [M, K], b [N, K] e4m3, K a multiple of 128; a_scale [M, K/128], b_scale [ceil(N/128), K/128] fp32
+ *   c [M, N] of out_dtype: the fp32 sum rounded once.  The order of the sum is fixed.
+ */
+int lo_gemm_w8a8_fp8_block(const void *a, const float *a_scale, const void *b, const float *b_scale, void *c,
+                           int out_dtype, int64_t M, int64_t N, int64_t K, lo_stream_t stream);
+
+/*
+ * The experts of a few tokens (M <= 64, M * top_k <= 1024) with e4m3 weights, in two launches: e4m3 rows of x, first
+ * product, act(gate) * up and its e4m3 codes, second product, weighted sum over a token's slots.
+ *   w1 [E, 2I, H], w2 [E, H, I] e4m3 row-major; w1s [E, 2I/128, H/128], w2s [E, H/128, I/128] fp32
+ *   topk_w, topk_ids [M, top_k]; ids without an expert here (out of range, or no entry in expert_map) add nothing
+ *   out[t] = routed_scaling_factor * sum_j topk_w[t, j] * y (+ shared_output[t]); out may be x or shared_output
+ *   workspace: lo_fused_experts_fp8_workspace_bytes, 16-byte aligned; one call's at a time
+ */
+int64_t lo_fused_experts_fp8_workspace_bytes(int64_t M, int32_t top_k, int64_t I, int32_t E);
+int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t H, int64_t I, int32_t E, int32_t num_experts,
+                         int32_t top_k, const void *w1, const float *w1s, const void *w2, const float *w2s,
+                         const float *topk_w, const void *topk_ids, int ids_dtype, const int32_t *expert_map,
+                         int activation, float routed_scaling_factor, const void *shared_output, void *out,
+                         void *workspace, int64_t workspace_bytes, lo_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,7 @@ LO_FUSED_FORCE_DECODE_PATH = 128
 LO_FUSED_ACT_GELU = 256
 LO_ACT_SILU, LO_ACT_GELU = 0, 1
 LO_FORM_BLOCK, LO_FORM_CHANNEL, LO_FORM_W4 = 0, 1, 2
+LO_Q_INT8_ROWS, LO_Q_INT8_GROUPS, LO_Q_FP8_GROUPS = 0, 1, 2
 LO_NOALLOC_SCRATCH_BYTES = 32 << 20
 LO_KERNEL_WS, LO_KERNEL_TILE, LO_KERNEL_PC, LO_KERNEL_AS, LO_KERNEL_T128, LO_KERNEL_W4_TILE, LO_KERNEL_DEC = 0, 1, 2, 3, 4, 5, 6
 KERNEL_NAMES = {LO_KERNEL_WS: "moe_gemm_ws_kernel", LO_KERNEL_TILE: "moe_gemm_tile_kernel",
@@ -104,6 +105,16 @@ SIGNATURES = {
                                                     c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                                     c_void_p, c_int, c_void_p, c_int, c_float, c_void_p, c_void_p,
                                                     c_void_p, c_int32, c_int, c_void_p]),
+    "lo_rms_norm_quant": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64, c_int64, c_float,
+                                  c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "lo_per_token_group_quant_fp8": (c_int, [c_void_p, c_int, c_int64, c_int64, c_float, c_void_p, c_void_p, c_void_p]),
+    "lo_act_mul_group_quant_fp8": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "lo_gemm_w8a8_fp8_block": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64,
+                                       c_void_p]),
+    "lo_fused_experts_fp8_workspace_bytes": (c_int64, [c_int64, c_int32, c_int64, c_int32]),
+    "lo_fused_experts_fp8": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p,
+                                     c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_float, c_void_p,
+                                     c_void_p, c_void_p, c_int64, c_void_p]),
 }
 
 _lib = None
@@ -143,6 +154,7 @@ class _NoHost:
         return None
 
     fused_experts = topk_softmax = fused_gate = _decline
+    rms_norm_quant = group_quant_fp8 = gemm_fp8 = experts_fp8 = _decline
 
 
 def host():
@@ -167,7 +179,9 @@ def host():
             return _host
         mod.bind(*(ctypes.cast(getattr(handle, n), c_void_p).value for n in (
             "lo_fused_experts_block_int8", "lo_fused_experts_channel_int8", "lo_fused_experts_workspace_bytes",
-            "lo_topk_softmax", "lo_moe_fused_gate", "lo_last_error")))
+            "lo_topk_softmax", "lo_moe_fused_gate", "lo_last_error", "lo_rms_norm_quant", "lo_per_token_group_quant_fp8",
+            "lo_act_mul_group_quant_fp8", "lo_gemm_w8a8_fp8_block", "lo_fused_experts_fp8",
+            "lo_fused_experts_fp8_workspace_bytes")))
         _host = mod
     return _host
 

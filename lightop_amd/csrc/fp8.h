@@ -1,0 +1,112 @@
+// e4m3 (OCP) helpers of the 8-bit floating-point operators.
+#pragma once
+#include "common.h"
+
+namespace lo {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+
+constexpr float kFp8Max = 448.0f; // largest e4m3 value
+
+// The rule of every e4m3 group here: top = max(max|v|, floor), scale = top / 448, code = e4m3(448 v / top), to nearest, ties to even.
+// 16-bit values often lie halfway between two codes, and a quotient by the rounded scale falls to either side.  7/8 v and top / 512 are
+// exact, so the one division rounds once (Markstein: a multiplication by the rounded reciprocal and two fused multiply-adds, exact
+// away from the ends of the range), and the quotient of two numbers of at most 11 bits never comes within 2^-24 of a halfway point
+// that it is not.  An infinite maximum: reciprocal 0, codes 0 and, for the infinity itself, NaN; a NaN keeps its code and is left out
+// of the maximum.  |v| <= top, so a quotient exceeds 448 by rounding at the most, and still rounds to it.
+struct Fp8Group {
+  float d, y; // top / 512 and its reciprocal
+};
+__device__ __forceinline__ Fp8Group fp8_group(float top, float &scale) {
+  scale = top / kFp8Max;
+  const float d = top * 0x1p-9f;
+  return {d, 1.0f / d};
+}
+__device__ __forceinline__ float fp8_quotient(float v, const Fp8Group &g) {
+  const float t = v * 0.875f;
+  const float q = t * g.y;
+  const float rem = __builtin_fmaf(-q, g.d, t);
+  return g.y > 0.0f ? __builtin_fmaf(rem, g.y, q) : q;
+}
+__device__ __forceinline__ int fp8_pack4(const float *v, const Fp8Group &g) {
+  int p = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_quotient(v[0], g), fp8_quotient(v[1], g), 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(fp8_quotient(v[2], g), fp8_quotient(v[3], g), p, true);
+}
+
+// d[i] (row 4 * (lane >> 4) + i of a, row lane & 15 of b) = sum over 128 of a * b, from 0.  A lane holds 32 codes of row lane & 15 of
+// either operand; which 32 is free as long as both agree.
+__device__ __forceinline__ v4f mfma_e4m3(const v8i a, const v8i b) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0, 0, 0);
+}
+
+// The same with every product and the sum to fp32's precision: e4m3 values are halves, four of the half instructions take them.
+// The e4m3 instruction lines the products up on the largest and drops what lies far below it: measured against 64 bits, normal operands
+// 1.4e-5 of the result, operands of very different sizes 6e-5, whichever of its forms (16x16x32, 16x16x128, 32x32x64); this one 1e-8 to 1e-7.
+// That is below a step of bf16 or fp16 and far above one of fp32, and what is quantised behind it moves codes.
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ v8h e4m3_halves(int lo, int hi) {
+  const v2h a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+  const v2h c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+  return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __forceinline__ v4f mfma_e4m3_exact(const v8i a, const v8i b) {
+  v4f d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < 8; i += 2)
+    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(e4m3_halves(a[i], a[i + 1]), e4m3_halves(b[i], b[i + 1]), d, 0, 0, 0);
+  return d;
+}
+// For a result that is kept in DT.
+template <int DT> __device__ __forceinline__ v4f mfma_e4m3_for(const v8i a, const v8i b) {
+  if constexpr (DT == LO_F32) return mfma_e4m3_exact(a, b);
+  else return mfma_e4m3(a, b);
+}
+
+__device__ __forceinline__ v8i join(const v4i a, const v4i b) {
+  return v8i{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// Eight values from x + at, as floats.
+template <int DT> __device__ __forceinline__ void load8(const void *x, int64_t at, float (&v)[8]) {
+  if constexpr (DT == LO_F32) {
+    const float *const p = static_cast<const float *>(x) + at;
+    const v4f a = *reinterpret_cast<const v4f *>(p), b = *reinterpret_cast<const v4f *>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = a[i], v[i + 4] = b[i];
+  } else {
+    const v8u16 r = *reinterpret_cast<const v8u16 *>(static_cast<const uint16_t *>(x) + at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32<DT>(r[i]);
+  }
+}
+template <int DT> __device__ __forceinline__ void store8(void *x, int64_t at, const float (&v)[8]) {
+  if constexpr (DT == LO_F32) {
+    float *const p = static_cast<float *>(x) + at;
+    *reinterpret_cast<v4f *>(p) = v4f{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<v4f *>(p + 4) = v4f{v[4], v[5], v[6], v[7]};
+  } else {
+    v8u16 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = from_f32<DT>(v[i]);
+    *reinterpret_cast<v8u16 *>(static_cast<uint16_t *>(x) + at) = r;
+  }
+}
+
+// act(g) * u in fp32, nothing rounded to 16 bits on the way.
+// SiLU: exp(-g) as 2^(-g log2 e) with the product's rounding error and the constant's given back, so that far gates keep their digits.
+__device__ __forceinline__ float silu_f32(float g) {
+  const float n = g * -1.44269502f;
+  const float lost = __builtin_fmaf(g, -1.44269502f, -n) + g * -1.92596299e-8f;
+  const float e = __builtin_amdgcn_exp2f(n);
+  // (past the ends of the exponential there is nothing to correct, and an infinite n has no difference)
+  const float e1 = fabsf(n) < 126.0f ? __builtin_fmaf(e, lost * 0.693147182f, e) : e;
+  return g * __builtin_amdgcn_rcpf(1.0f + e1);
+}
+// GELU in its erf form; the complement keeps the digits that 1 + erf loses left of zero.
+__device__ __forceinline__ float gelu_f32(float g) { return 0.5f * g * erfcf(g * -0.707106769f); }
+template <int ACT> __device__ __forceinline__ float act_mul_f32(float g, float u) {
+  return (ACT == LO_ACT_GELU ? gelu_f32(g) : silu_f32(g)) * u;
+}
+
+} // namespace lo

@@ -1,4 +1,5 @@
-// Host path of the calls a serving loop makes on every step: the whole fused-experts layer and the two routers.
+// Host path of the calls a serving loop makes on every step: the whole fused-experts layer, the two routers and the 8-bit operators
+// beside them.
 //
 // A one-token layer is two kernel launches, 17 us of GPU time; marshalling the same call through Python (argument
 // checks on fifteen tensors, ctypes conversions, stream and workspace look-ups) took 25-27 us of host time and set
@@ -35,6 +36,12 @@ decltype(&lo_fused_experts_workspace_bytes) g_ws_bytes = nullptr;
 decltype(&lo_topk_softmax) g_topk_softmax = nullptr;
 decltype(&lo_moe_fused_gate) g_gate = nullptr;
 decltype(&lo_last_error) g_last_error = nullptr;
+decltype(&lo_rms_norm_quant) g_norm = nullptr;
+decltype(&lo_per_token_group_quant_fp8) g_quant_fp8 = nullptr;
+decltype(&lo_act_mul_group_quant_fp8) g_act_fp8 = nullptr;
+decltype(&lo_gemm_w8a8_fp8_block) g_gemm_fp8 = nullptr;
+decltype(&lo_fused_experts_fp8) g_experts_fp8 = nullptr;
+decltype(&lo_fused_experts_fp8_workspace_bytes) g_experts_fp8_bytes = nullptr;
 
 PyObject *s_preshuffled, *s_int4, *s_kmajor; // attribute names of weights in their load-time layout
 
@@ -356,17 +363,234 @@ PyObject *fused_gate(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- 8-bit operators beside the int8 experts ---------------------------------------------------------------
+
+// Whether the kernels take the tensor as it is.
+bool plain16(const at::Tensor &t, int device) {
+  return plain(t, device) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
+// A tuple of what was made; null tensors become None.
+PyObject *tuple_of(at::Tensor *t, int n) {
+  PyObject *out = PyTuple_New(n);
+  if (!out) return nullptr;
+  for (int i = 0; i < n; ++i) {
+    PyObject *o = t[i].defined() ? THPVariable_Wrap(std::move(t[i])) : Py_NewRef(Py_None);
+    if (!o) {
+      Py_DECREF(out);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(out, i, o);
+  }
+  return out;
+}
+
+// rms_norm_quant(x, weight, residual, residual_out, eps, form, return_normed) -> (q, scale, residual or None, normed or None), or None:
+// not an ordinary call.
+PyObject *rms_norm_quant(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  if (nargs != 7) {
+    PyErr_SetString(PyExc_TypeError, "rms_norm_quant takes 7 arguments");
+    return nullptr;
+  }
+  const at::Tensor *x = tensor_of(args[0]), *w = tensor_of(args[1]), *r = nullptr, *to = nullptr;
+  if (!x || !w || (args[2] != Py_None && !(r = tensor_of(args[2]))) || (args[3] != Py_None && !(to = tensor_of(args[3])))) Py_RETURN_NONE;
+  if (!(PyFloat_Check(args[4]) || PyLong_Check(args[4])) || !PyLong_Check(args[5])) Py_RETURN_NONE;
+  const double eps = PyFloat_AsDouble(args[4]);
+  const long form = PyLong_AsLong(args[5]);
+  const int normed = PyObject_IsTrue(args[6]);
+  if (normed < 0 || PyErr_Occurred()) return nullptr;
+  HANDLE_TH_ERRORS
+  if (!x->is_cuda() || x->get_device() != device_now() || x->dim() < 1) Py_RETURN_NONE;
+  const int dev = x->get_device(), dtype = dtype_code(x->scalar_type()), wtype = dtype_code(w->scalar_type());
+  const int64_t H = x->size(-1), unit = form == LO_Q_INT8_ROWS ? 8 : 128;
+  if (dtype < 0 || H == 0 || H % unit || x->numel() == 0) Py_RETURN_NONE;
+  if (!plain16(*x, dev) || !plain16(*w, dev) || w->dim() != 1 || w->size(0) != H || (wtype != dtype && wtype != LO_F32)) Py_RETURN_NONE;
+  if (r && (!plain16(*r, dev) || r->scalar_type() != x->scalar_type() || r->sizes() != x->sizes())) Py_RETURN_NONE;
+  if (to && (!r || !plain16(*to, dev) || to->scalar_type() != x->scalar_type() || to->sizes() != x->sizes())) Py_RETURN_NONE;
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream();
+  const int64_t rows = x->numel() / H;
+  const void *xp = x->data_ptr(), *wp = w->data_ptr(), *rp = r ? r->data_ptr() : nullptr;
+  auto sizes = x->sizes().vec();
+  const auto opts = x->options().requires_grad(false);
+  at::Tensor out[4]; // q, scale, residual, normed
+  if (to) out[2] = *to;
+  int rc;
+  {
+    const NoGil nogil;
+    out[0] = at::empty(sizes, opts.dtype(form == LO_Q_FP8_GROUPS ? at::kFloat8_e4m3fn : at::kChar));
+    if (r && !to) out[2] = at::empty(sizes, opts);
+    if (normed) out[3] = at::empty(sizes, opts);
+    sizes.back() = form == LO_Q_INT8_ROWS ? 1 : H / 128;
+    out[1] = at::empty(sizes, opts.dtype(at::kFloat));
+    rc = g_norm(xp, dtype, H, rp, H, wp, wtype, rows, H, static_cast<float>(eps), static_cast<int>(form), r ? out[2].data_ptr() : nullptr,
+                normed ? out[3].data_ptr() : nullptr, out[0].data_ptr(), out[1].data_ptr<float>(), stream);
+  }
+  if (rc < 0) return raise(rc);
+  return tuple_of(out, 4);
+  END_HANDLE_TH_ERRORS
+}
+
+// group_quant_fp8(x, activation, eps) -> (q, scale), or None: not an ordinary call.  activation: -1 none, else LO_ACT_* of [..., 2I].
+PyObject *group_quant_fp8(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  if (nargs != 3) {
+    PyErr_SetString(PyExc_TypeError, "group_quant_fp8 takes 3 arguments");
+    return nullptr;
+  }
+  const at::Tensor *x = tensor_of(args[0]);
+  if (!x || !PyLong_Check(args[1]) || !(PyFloat_Check(args[2]) || PyLong_Check(args[2]))) Py_RETURN_NONE;
+  const long act = PyLong_AsLong(args[1]);
+  const double eps = PyFloat_AsDouble(args[2]);
+  if (PyErr_Occurred()) return nullptr;
+  HANDLE_TH_ERRORS
+  if (!x->is_cuda() || x->get_device() != device_now() || x->dim() < 1 || x->numel() == 0) Py_RETURN_NONE;
+  const int dev = x->get_device(), dtype = dtype_code(x->scalar_type());
+  const int64_t width = x->size(-1), I = act < 0 ? width : width / 2;
+  if (dtype < 0 || width % (act < 0 ? 128 : 256) || !plain16(*x, dev)) Py_RETURN_NONE;
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream();
+  const int64_t rows = x->numel() / width;
+  const void *xp = x->data_ptr();
+  auto sizes = x->sizes().vec();
+  const auto opts = x->options().requires_grad(false);
+  at::Tensor out[2];
+  int rc;
+  {
+    const NoGil nogil;
+    sizes.back() = I;
+    out[0] = at::empty(sizes, opts.dtype(at::kFloat8_e4m3fn));
+    sizes.back() = I / 128;
+    out[1] = at::empty(sizes, opts.dtype(at::kFloat));
+    rc = act < 0 ? g_quant_fp8(xp, dtype, rows, I, static_cast<float>(eps), out[0].data_ptr(), out[1].data_ptr<float>(), stream)
+                 : g_act_fp8(xp, dtype, static_cast<int>(act), rows, I, out[0].data_ptr(), out[1].data_ptr<float>(), stream);
+  }
+  if (rc < 0) return raise(rc);
+  return tuple_of(out, 2);
+  END_HANDLE_TH_ERRORS
+}
+
+// gemm_fp8(a, b, a_scale, b_scale, dtype) -> tensor, or None: not an ordinary call.  dtype: LO_* of the result.
+PyObject *gemm_fp8(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  if (nargs != 5) {
+    PyErr_SetString(PyExc_TypeError, "gemm_fp8 takes 5 arguments");
+    return nullptr;
+  }
+  const at::Tensor *t[4];
+  for (int i = 0; i < 4; ++i)
+    if (!(t[i] = tensor_of(args[i]))) Py_RETURN_NONE;
+  if (!PyLong_Check(args[4])) Py_RETURN_NONE;
+  const long dtype = PyLong_AsLong(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  HANDLE_TH_ERRORS
+  const at::Tensor &a = *t[0], &b = *t[1], &as = *t[2], &bs = *t[3];
+  if (!a.is_cuda() || a.get_device() != device_now() || a.dim() < 1 || b.dim() != 2 || dtype < 0) Py_RETURN_NONE;
+  const int dev = a.get_device();
+  for (const at::Tensor *v : t)
+    if (!plain(*v, dev)) Py_RETURN_NONE;
+  const int64_t K = b.size(1), N = b.size(0), M = K ? a.numel() / K : 0;
+  if (a.scalar_type() != at::kFloat8_e4m3fn || b.scalar_type() != at::kFloat8_e4m3fn || as.scalar_type() != at::kFloat ||
+      bs.scalar_type() != at::kFloat || K == 0 || K % 128 || a.size(-1) != K || M == 0 || N == 0 || !plain16(a, dev) || !plain16(b, dev))
+    Py_RETURN_NONE;
+  auto sizes = a.sizes().vec();
+  sizes.back() = K / 128;
+  if (as.sizes() != at::IntArrayRef(sizes) || bs.sizes() != at::IntArrayRef({(N + 127) / 128, K / 128})) Py_RETURN_NONE;
+  sizes.back() = N;
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream();
+  const void *ap = a.data_ptr(), *bp = b.data_ptr();
+  const float *asp = as.data_ptr<float>(), *bsp = bs.data_ptr<float>();
+  const auto opts = a.options().requires_grad(false).dtype(dtype == LO_BF16 ? at::kBFloat16 : dtype == LO_F16 ? at::kHalf : at::kFloat);
+  at::Tensor out;
+  int rc;
+  {
+    const NoGil nogil;
+    out = at::empty(sizes, opts);
+    rc = g_gemm_fp8(ap, asp, bp, bsp, out.data_ptr(), static_cast<int>(dtype), M, N, K, stream);
+  }
+  if (rc < 0) return raise(rc);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// experts_fp8(hidden, w1, w2, topk_weights, topk_ids, w1_scale, w2_scale, expert_map, shared_output, activation, global_num_experts,
+//             factor) -> tensor, or None: not an ordinary call.
+PyObject *experts_fp8(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  if (nargs != 12) {
+    PyErr_SetString(PyExc_TypeError, "experts_fp8 takes 12 arguments");
+    return nullptr;
+  }
+  const at::Tensor *t[9];
+  for (int i = 0; i < 9; ++i) {
+    t[i] = nullptr;
+    if (!(i >= 7 && args[i] == Py_None) && !(t[i] = tensor_of(args[i]))) Py_RETURN_NONE;
+  }
+  if (!PyLong_Check(args[9]) || !PyLong_Check(args[10]) || !(PyFloat_Check(args[11]) || PyLong_Check(args[11]))) Py_RETURN_NONE;
+  const long act = PyLong_AsLong(args[9]);
+  long long experts = PyLong_AsLongLong(args[10]);
+  const double factor = PyFloat_AsDouble(args[11]);
+  if (PyErr_Occurred()) return nullptr;
+  HANDLE_TH_ERRORS
+  const at::Tensor &x = *t[0], &w1 = *t[1], &w2 = *t[2], &tw = *t[3], &ids = *t[4], &s1 = *t[5], &s2 = *t[6];
+  if (!x.is_cuda() || x.get_device() != device_now()) Py_RETURN_NONE;
+  const int dev = x.get_device(), dtype = dtype_code(x.scalar_type());
+  for (int i = 0; i < 9; ++i)
+    if (t[i] && !(i < 3 ? plain16(*t[i], dev) : plain(*t[i], dev))) Py_RETURN_NONE;
+  if (!(dtype == LO_BF16 || dtype == LO_F16) || x.dim() != 2 || w1.dim() != 3 || ids.dim() != 2 || tw.sizes() != ids.sizes()) Py_RETURN_NONE;
+  const int64_t M = x.size(0), H = x.size(1), E = w1.size(0), I = w1.size(1) / 2, k = ids.size(1);
+  if (M == 0 || ids.size(0) != M || w1.size(1) % 256 || H % 128 || H == 0 || I == 0 || w1.size(2) != H ||
+      w2.sizes() != at::IntArrayRef({E, H, I}) || s1.sizes() != at::IntArrayRef({E, 2 * I / 128, H / 128}) ||
+      s2.sizes() != at::IntArrayRef({E, H / 128, I / 128}))
+    Py_RETURN_NONE;
+  if (w1.scalar_type() != at::kFloat8_e4m3fn || w2.scalar_type() != at::kFloat8_e4m3fn || tw.scalar_type() != at::kFloat ||
+      s1.scalar_type() != at::kFloat || s2.scalar_type() != at::kFloat)
+    Py_RETURN_NONE;
+  const bool ids64 = ids.scalar_type() == at::kLong;
+  if (!ids64 && ids.scalar_type() != at::kInt) Py_RETURN_NONE;
+  if (experts == -1) experts = E;
+  if (experts < E || experts > INT32_MAX || k < 1 || k > INT32_MAX || M > INT32_MAX) Py_RETURN_NONE;
+  if (t[7] && (t[7]->scalar_type() != at::kInt || t[7]->numel() < experts)) Py_RETURN_NONE;
+  if (t[8] && (t[8]->scalar_type() != x.scalar_type() || t[8]->sizes() != x.sizes())) Py_RETURN_NONE;
+  const int64_t bytes = g_experts_fp8_bytes(M, static_cast<int32_t>(k), I, static_cast<int32_t>(E));
+  if (bytes < 0) return raise(static_cast<int>(bytes));
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream();
+  if (capturing(stream)) Py_RETURN_NONE; // (its scratch belongs to the graph)
+  const auto sizes = x.sizes().vec();
+  const auto opts = x.options().requires_grad(false);
+  const void *xp = x.data_ptr(), *w1p = w1.data_ptr(), *w2p = w2.data_ptr(), *idp = ids.data_ptr(), *sh = t[8] ? t[8]->data_ptr() : nullptr;
+  const float *s1p = s1.data_ptr<float>(), *s2p = s2.data_ptr<float>(), *twp = tw.data_ptr<float>();
+  const int32_t *map = t[7] ? t[7]->data_ptr<int32_t>() : nullptr;
+  at::Tensor out;
+  int rc;
+  {
+    const NoGil nogil;
+    const std::shared_ptr<Scratch> ws = workspace_for(bytes, dev, stream);
+    out = at::empty(sizes, opts);
+    const std::lock_guard<std::mutex> lock(ws->busy);
+    rc = g_experts_fp8(xp, dtype, M, H, I, static_cast<int32_t>(E), static_cast<int32_t>(experts), static_cast<int32_t>(k), w1p, s1p, w2p,
+                       s2p, twp, idp, ids64 ? LO_I64 : LO_I32, map, static_cast<int>(act), static_cast<float>(factor), sh, out.data_ptr(),
+                       ws->buf.data_ptr(), ws->buf.numel(), stream);
+  }
+  if (rc < 0) return raise(rc);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(lo_fused_experts_block_int8, lo_fused_experts_channel_int8, lo_fused_experts_workspace_bytes, lo_topk_softmax,
-//      lo_moe_fused_gate, lo_last_error): addresses of the library's functions.
+//      lo_moe_fused_gate, lo_last_error, lo_rms_norm_quant, lo_per_token_group_quant_fp8, lo_act_mul_group_quant_fp8,
+//      lo_gemm_w8a8_fp8_block, lo_fused_experts_fp8, lo_fused_experts_fp8_workspace_bytes): addresses of the library's functions.
 PyObject *bind(PyObject *, PyObject *args) {
-  unsigned long long a[6];
-  if (!PyArg_ParseTuple(args, "KKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5])) return nullptr;
+  unsigned long long a[12];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9], &a[10], &a[11]))
+    return nullptr;
   g_block = reinterpret_cast<decltype(g_block)>(a[0]);
   g_channel = reinterpret_cast<decltype(g_channel)>(a[1]);
   g_ws_bytes = reinterpret_cast<decltype(g_ws_bytes)>(a[2]);
   g_topk_softmax = reinterpret_cast<decltype(g_topk_softmax)>(a[3]);
   g_gate = reinterpret_cast<decltype(g_gate)>(a[4]);
   g_last_error = reinterpret_cast<decltype(g_last_error)>(a[5]);
+  g_norm = reinterpret_cast<decltype(g_norm)>(a[6]);
+  g_quant_fp8 = reinterpret_cast<decltype(g_quant_fp8)>(a[7]);
+  g_act_fp8 = reinterpret_cast<decltype(g_act_fp8)>(a[8]);
+  g_gemm_fp8 = reinterpret_cast<decltype(g_gemm_fp8)>(a[9]);
+  g_experts_fp8 = reinterpret_cast<decltype(g_experts_fp8)>(a[10]);
+  g_experts_fp8_bytes = reinterpret_cast<decltype(g_experts_fp8_bytes)>(a[11]);
   Py_RETURN_NONE;
 }
 
@@ -375,6 +599,10 @@ PyMethodDef methods[] = {
     {"fused_experts", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(fused_experts)), METH_FASTCALL, nullptr},
     {"topk_softmax", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(topk_softmax)), METH_FASTCALL, nullptr},
     {"fused_gate", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(fused_gate)), METH_FASTCALL, nullptr},
+    {"rms_norm_quant", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(rms_norm_quant)), METH_FASTCALL, nullptr},
+    {"group_quant_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(group_quant_fp8)), METH_FASTCALL, nullptr},
+    {"gemm_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(gemm_fp8)), METH_FASTCALL, nullptr},
+    {"experts_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(experts_fp8)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,4 +1,4 @@
-"""Grouped-GEMM stage of the per-channel W8A8 MoE (reference: lightop.gemmopt.moe_gemm_w8a8,
+"""Grouped-GEMM stage of the per-channel W8A8 MoE, and the dense e4m3 product with block scales (reference: lightop.gemmopt.moe_gemm_w8a8,
 python/lightop/gemmopt.py:437-457; native side csrc/moe_gemm/w8a8/moe_w8a8.cu:2389-2536)."""
 from __future__ import annotations
 
@@ -7,7 +7,10 @@ from typing import Any, Dict, Optional
 import torch
 
 from . import _lib
-from .op import _act_dtype, _on_device, _require_cuda
+from .op import _act_dtype, _on_device, _one_device, _require_cuda, _rows16
+
+
+_OUT_DTYPES = {torch.bfloat16: _lib.LO_BF16, torch.float16: _lib.LO_F16, torch.float32: _lib.LO_F32}
 
 
 def moe_gemm_w8a8(input: torch.Tensor, b_qweight: torch.Tensor, output: torch.Tensor, a_scale: torch.Tensor,
@@ -44,4 +47,47 @@ def moe_gemm_w8a8(input: torch.Tensor, b_qweight: torch.Tensor, output: torch.Te
     return output
 
 
-__all__ = ["moe_gemm_w8a8"]
+def gemm_w8a8_fp8_block(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor,
+                        out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Dense product of e4m3 operands with block scales, as a shared expert or a projection of an fp8 checkpoint needs:
+    ``out[m, n] = sum_kb (a[m, kb] . b[n, kb]) * a_scale[m, kb] * b_scale[n // 128, kb]`` over K blocks of 128, summed in fp32
+    and rounded once to ``out_dtype`` (bfloat16, float16 or float32).
+
+    ``a`` [..., K] with ``a_scale`` [..., K/128] (``per_token_group_quant_fp8``), ``b`` [N, K] row-major as a checkpoint holds it,
+    ``b_scale`` [ceil(N/128), K/128] fp32; any number of rows, any N, K a multiple of 128.  Written into ``out`` (contiguous)
+    where the caller brings it."""
+    if out is None:
+        made = (_lib._host or _lib.host()).gemm_fp8(a, b, a_scale, b_scale, _OUT_DTYPES.get(out_dtype, -1))
+        if made is not None:
+            return made
+    _one_device(a, b, a_scale, b_scale, out)
+    if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn:
+        raise RuntimeError(f"gemm_w8a8_fp8_block: a and b must be float8_e4m3fn, got {a.dtype} and {b.dtype}")
+    if a.dim() < 1 or b.dim() != 2 or a.shape[-1] != b.shape[1]:
+        raise RuntimeError(f"gemm_w8a8_fp8_block: a must be [..., K] and b [N, K], got {tuple(a.shape)} and {tuple(b.shape)}")
+    N, K = b.shape
+    if K == 0 or K % 128:
+        raise RuntimeError(f"gemm_w8a8_fp8_block: K must be a multiple of 128, got {K}")
+    if a_scale.shape != a.shape[:-1] + (K // 128,) or b_scale.shape != ((N + 127) // 128, K // 128):
+        raise RuntimeError("gemm_w8a8_fp8_block: scales must be [..., K/128] and [ceil(N/128), K/128], got "
+                           f"{tuple(a_scale.shape)} and {tuple(b_scale.shape)}")
+    if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
+        raise RuntimeError("gemm_w8a8_fp8_block: scales must be float32")
+    shape = a.shape[:-1] + (N,)
+    if out_dtype not in _OUT_DTYPES:
+        raise RuntimeError(f"gemm_w8a8_fp8_block: out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype, device=a.device)
+    elif out.shape != shape or out.dtype != out_dtype or not out.is_contiguous():
+        raise RuntimeError(f"gemm_w8a8_fp8_block: out must be a contiguous {out_dtype} tensor of shape {tuple(shape)}")
+    dtype = _OUT_DTYPES[out_dtype]
+    if out.numel() == 0:
+        return out
+    a, b, a_scale, b_scale = _rows16(a), _rows16(b), a_scale.contiguous(), b_scale.contiguous()
+    with _on_device(a):
+        _lib.check(_lib.lib().lo_gemm_w8a8_fp8_block(_lib.ptr(a), _lib.ptr(a_scale), _lib.ptr(b), _lib.ptr(b_scale), _lib.ptr(out),
+                                                     dtype, out.numel() // N, N, K, _lib.stream_of(a)))
+    return out
+
+
+__all__ = ["moe_gemm_w8a8", "gemm_w8a8_fp8_block"]

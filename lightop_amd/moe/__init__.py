@@ -19,6 +19,8 @@ _NATIVE_APIS = {
     "silu_and_mul",
     "gelu_and_mul",
     "act_and_mul_group_quant",
+    "act_and_mul_group_quant_fp8",
+    "fused_experts_decode_fp8",
     "fused_experts_workspace_bytes",
     "fused_experts_workspace_views",
     "preshuffle_moe_weight",
@@ -36,6 +38,8 @@ def __getattr__(name):
 
 __all__ = [
     "act_and_mul_group_quant",
+    "act_and_mul_group_quant_fp8",
+    "fused_experts_decode_fp8",
     "fused_experts_impl_int8",
     "fused_experts_impl_w4a8",
     "fused_experts_workspace_bytes",

@@ -11,7 +11,7 @@ import torch
 
 from .. import _lib, envs
 from ..gemmopt import moe_gemm_w8a8
-from ..op import _act_dtype, _ids_dtype, _on_device, _require_cuda
+from ..op import _act_dtype, _float_dtype, _ids_dtype, _on_device, _one_device, _require_cuda, _rows16
 
 
 # forms of a whole-path call, as csrc/host_binding.cpp numbers them
@@ -333,6 +333,31 @@ def act_and_mul_group_quant(x: torch.Tensor, activation: str = "silu", row_mask:
     return q, s
 
 
+def act_and_mul_group_quant_fp8(x: torch.Tensor, activation: str = "silu") -> Tuple[torch.Tensor, torch.Tensor]:
+    """The gated activation of ``x`` [..., 2I] in fp32, ``act(x[..., :I]) * x[..., I:]``, and its e4m3 codes in groups of 128 by the
+    rule of ``per_token_group_quant_fp8``: (q [..., I] float8_e4m3fn, s [..., I/128] f32), in one launch.  Unlike the int8 form
+    nothing is rounded to 16 bits before the codes.  ``x`` is bf16, fp16 or fp32."""
+    if activation not in ("silu", "gelu"):
+        raise ValueError(f"Unsupported FusedMoe activation: {activation}")
+    pair = (_lib._host or _lib.host()).group_quant_fp8(x, _lib.LO_ACT_GELU if activation == "gelu" else _lib.LO_ACT_SILU, 1e-10)
+    if pair is not None:
+        return pair
+    _require_cuda(x)
+    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 256:
+        raise RuntimeError(f"act_and_mul_group_quant_fp8: x must be [..., 2 * I] with I a multiple of 128, got {tuple(x.shape)}")
+    I = x.shape[-1] // 2
+    q = torch.empty(x.shape[:-1] + (I,), dtype=torch.float8_e4m3fn, device=x.device)
+    s = torch.empty(x.shape[:-1] + (I // 128,), dtype=torch.float32, device=x.device)
+    if q.numel() == 0:
+        return q, s
+    x = _rows16(x)
+    with _on_device(x):
+        _lib.check(_lib.lib().lo_act_mul_group_quant_fp8(
+            _lib.ptr(x), _float_dtype(x, "x"), _lib.LO_ACT_GELU if activation == "gelu" else _lib.LO_ACT_SILU, q.numel() // I, I,
+            _lib.ptr(q), _lib.ptr(s), _lib.stream_of(x)))
+    return q, s
+
+
 @functools.lru_cache(maxsize=256)
 def fused_experts_workspace_bytes(M: int, top_k: int, H: int, I: int, num_experts: int,
                                   block_size_m: int = 0) -> int:
@@ -599,6 +624,83 @@ def fused_experts_impl_w4a8(hidden_states: torch.Tensor,
                               int(extra.get("lightop_amd_block_size_m", 0)), workspace=extra.get("lightop_amd_workspace"))
 
 
+def fused_experts_decode_fp8(hidden_states: torch.Tensor,
+                             w1: torch.Tensor,
+                             w2: torch.Tensor,
+                             topk_weights: torch.Tensor,
+                             topk_ids: torch.Tensor,
+                             w1_scale: torch.Tensor,
+                             w2_scale: torch.Tensor,
+                             activation: str = "silu",
+                             global_num_experts: int = -1,
+                             expert_map: Optional[torch.Tensor] = None,
+                             routed_scaling_factor: float = 1.0,
+                             shared_output: Optional[torch.Tensor] = None,
+                             inplace: bool = False) -> torch.Tensor:
+    """The routed experts of a decode batch (at most 64 tokens and 1024 slots) with e4m3 weights, in two launches.
+
+    ``hidden_states`` [M, H] bf16 or fp16; ``w1`` [E, 2I, H], ``w2`` [E, H, I] float8_e4m3fn, row-major as a checkpoint holds them,
+    with one fp32 scale for 128 x 128: ``w1_scale`` [E, 2I/128, H/128], ``w2_scale`` [E, H/128, I/128].  Rows are quantised in front
+    of either product by the rule of ``per_token_group_quant_fp8``, act(gate) * up stays in fp32 until then, and
+    ``out = routed_scaling_factor * sum_k topk_weights * y (+ shared_output)`` is rounded once.  ``activation``: "silu" or "gelu".
+    Arguments of ``fused_experts_impl_int8`` by the same names mean the same; slots whose expert is not here (-1 in
+    ``expert_map``, or an id out of range) add nothing."""
+    if activation not in ("silu", "gelu"):
+        raise ValueError(f"Unsupported FusedMoe activation: {activation}")
+    if not inplace:
+        out = (_lib._host or _lib.host()).experts_fp8(
+            hidden_states, w1, w2, topk_weights, topk_ids, w1_scale, w2_scale, expert_map, shared_output,
+            _lib.LO_ACT_GELU if activation == "gelu" else _lib.LO_ACT_SILU, global_num_experts, routed_scaling_factor)
+        if out is not None:
+            return out
+    _one_device(hidden_states, w1, w2, topk_weights, topk_ids, w1_scale, w2_scale, expert_map, shared_output)
+    if w1.dtype != torch.float8_e4m3fn or w2.dtype != torch.float8_e4m3fn:
+        raise RuntimeError(f"fused_experts_decode_fp8: weights must be float8_e4m3fn, got {w1.dtype} and {w2.dtype}")
+    if hidden_states.dtype not in (torch.bfloat16, torch.float16):
+        raise NotImplementedError("lightop_amd: hidden_states must be bfloat16 or float16")
+    assert hidden_states.dim() == 2 and w1.dim() == 3 and hidden_states.shape[1] == w1.shape[2], "Hidden size mismatch"
+    assert topk_weights.shape == topk_ids.shape and topk_ids.dim() == 2, "topk shape mismatch"
+    M, H = hidden_states.shape
+    E, N = w1.shape[0], w1.shape[1]
+    I = N // 2
+    assert topk_ids.shape[0] == M, "topk shape mismatch"
+    assert N % 256 == 0 and H % 128 == 0 and I > 0 and H > 0, "hidden and intermediate sizes must be multiples of 128"
+    assert w2.shape == (E, H, I), "w2 must be [E, H, I]"
+    assert w1.is_contiguous() and w2.is_contiguous(), "expert weights must be contiguous"
+    assert w1_scale.shape == (E, N // 128, H // 128) and w2_scale.shape == (E, H // 128, I // 128), "scales are one for 128 x 128"
+    if global_num_experts in (-1, None):
+        global_num_experts = E
+    if expert_map is not None and expert_map.numel() < global_num_experts:
+        raise RuntimeError(f"fused_experts_decode_fp8: expert_map holds {expert_map.numel()} of {global_num_experts} experts")
+    if shared_output is not None and (shared_output.shape != hidden_states.shape or shared_output.dtype != hidden_states.dtype):
+        raise RuntimeError("fused_experts_decode_fp8: shared_output must have the shape and type of hidden_states")
+    if inplace and not hidden_states.is_contiguous():
+        raise RuntimeError("fused_experts_decode_fp8: hidden_states must be contiguous to be written in place")
+    top_k = topk_ids.shape[1]
+    out = hidden_states if inplace else torch.empty_like(hidden_states, memory_format=torch.contiguous_format)
+    if M == 0:
+        return out
+    x = _rows16(hidden_states)
+    ids = topk_ids.contiguous()
+    f32 = lambda t: t.to(torch.float32).contiguous()
+    weights, s1, s2 = f32(topk_weights), f32(w1_scale), f32(w2_scale)
+    emap = None if expert_map is None else expert_map.to(torch.int32).contiguous()
+    shared = None if shared_output is None else shared_output.contiguous()
+    w1, w2 = _rows16(w1), _rows16(w2)
+    lib = _lib.lib()
+    nbytes = lib.lo_fused_experts_fp8_workspace_bytes(M, top_k, I, E)
+    _lib.check(nbytes)
+    with _on_device(x):
+        stream = torch.cuda.current_stream(x.device).cuda_stream
+        workspace = _scratch(nbytes, x.device, stream)
+        _lib.check(lib.lo_fused_experts_fp8(
+            _lib.ptr(x), _act_dtype(x), M, H, I, E, int(global_num_experts), top_k, _lib.ptr(w1), _lib.ptr(s1), _lib.ptr(w2),
+            _lib.ptr(s2), _lib.ptr(weights), _lib.ptr(ids), _ids_dtype(ids), _lib.ptr(emap),
+            _lib.LO_ACT_GELU if activation == "gelu" else _lib.LO_ACT_SILU, float(routed_scaling_factor), _lib.ptr(shared),
+            _lib.ptr(out), _lib.ptr(workspace), workspace.numel(), ctypes_void(stream)))
+    return out
+
+
 @functools.lru_cache(maxsize=256)
 def _workspace_bytes_cached(M: int, top_k: int, H: int, I: int, num_experts: int) -> int:
     return fused_experts_workspace_bytes(M, top_k, H, I, num_experts, 0)
@@ -738,5 +840,6 @@ __all__ = ["fused_experts_impl_int8", "fused_experts_impl_w4a8", "get_w8a8moe_js
            "preshuffle_moe_weight",
            "preshuffle_moe_weight_int4", "preshuffle_moe_scale_int4", "invoke_fused_moe_kernel_int8",
            "invoke_fused_moe_kernel_w4a8",
-           "invoke_fused_moe_gemm1_silu_quant", "silu_and_mul", "gelu_and_mul", "act_and_mul_group_quant", "fused_experts_workspace_bytes",
+           "invoke_fused_moe_gemm1_silu_quant", "silu_and_mul", "gelu_and_mul", "act_and_mul_group_quant",
+           "act_and_mul_group_quant_fp8", "fused_experts_decode_fp8", "fused_experts_workspace_bytes",
            "fused_experts_workspace_views", "moe_gemm_w8a8"]

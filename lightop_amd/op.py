@@ -18,6 +18,19 @@ def _require_cuda(*tensors):
             raise RuntimeError("lightop_amd: tensors must live on the GPU (there is no CPU path)")
 
 
+def _one_device(*tensors):
+    """Every tensor is on one GPU."""
+    _require_cuda(*tensors)
+    if len({t.device for t in tensors if t is not None}) > 1:
+        raise RuntimeError("lightop_amd: tensors must live on one device")
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and 16-byte aligned: itself or a copy."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 @contextlib.contextmanager
 def _on_device(t: torch.Tensor):
     if torch.cuda.current_device() == t.device.index:

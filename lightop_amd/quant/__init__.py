@@ -1,4 +1,4 @@
-"""INT8 activation quantisation of the fused-MoE path: 1x128 groups and per token (reference:
+"""INT8 activation quantisation of the fused-MoE path: 1x128 groups and per token, and e4m3 in 1x128 groups (reference:
 python/lightop/_lmslim_native/layers/gemm/int8_utils.py:125-195 and :20-71; public names
 lightop.quant.per_token_group_quant_int8 and lightop.quant.per_token_quant_int8,
 python/lightop/quant/int8.py:13-16, :35)."""
@@ -9,7 +9,7 @@ from typing import Tuple
 import torch
 
 from .. import _lib
-from ..op import _act_dtype, _on_device, _require_cuda
+from ..op import _act_dtype, _float_dtype, _on_device, _require_cuda, _rows16
 
 
 def per_token_group_quant_int8(
@@ -60,7 +60,39 @@ def per_token_quant_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return x_q, scales
 
 
-__all__ = ["per_token_group_quant_int8", "per_token_quant_int8"]
+def per_token_group_quant_fp8(
+    x: torch.Tensor,
+    group_size: int,
+    eps: float = 1e-10,
+    dtype: torch.dtype = torch.float8_e4m3fn,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Quantise every ``group_size`` contiguous values of the last dimension to e4m3: ``top = max(|x|.max(), eps); s = top / 448;
+    q = e4m3(448 x / top)``, to nearest, ties to even.  Returns ``(x_q, x_s)`` with ``x_s`` of shape
+    ``x.shape[:-1] + (x.shape[-1] // group_size,)`` in fp32.  Built for ``group_size == 128``; ``x`` is bf16, fp16 or fp32.
+    A NaN stays one and is left out of the maximum."""
+    assert x.shape[-1] % group_size == 0, "the last dimension of `x` must be divisible by `group_size`"
+    if dtype != torch.float8_e4m3fn:
+        raise RuntimeError("per_token_group_quant_fp8: only torch.float8_e4m3fn output is supported")
+    if group_size != 128:
+        raise RuntimeError("per_token_group_quant_fp8: group_size must be 128")
+    pair = (_lib._host or _lib.host()).group_quant_fp8(x, -1, eps)
+    if pair is not None:
+        return pair
+    _require_cuda(x)
+    x_q = torch.empty(x.shape, device=x.device, dtype=dtype)
+    x_s = torch.empty(x.shape[:-1] + (x.shape[-1] // group_size,), device=x.device, dtype=torch.float32)
+    if x.numel() == 0:
+        return x_q, x_s
+    x = _rows16(x)
+    cols = x.shape[-1]
+    with _on_device(x):
+        _lib.check(_lib.lib().lo_per_token_group_quant_fp8(
+            _lib.ptr(x), _float_dtype(x, "x"), x.numel() // cols, cols, float(eps), _lib.ptr(x_q), _lib.ptr(x_s),
+            _lib.stream_of(x)))
+    return x_q, x_s
+
+
+__all__ = ["per_token_group_quant_int8", "per_token_quant_int8", "per_token_group_quant_fp8"]
 
 # ``quant.int8`` (python/lightop/quant/int8.py in the reference) is this module: the attribute makes
 # ``import lightop.quant.int8 as q`` and ``from lightop_amd.quant import int8`` resolve as well.

@@ -1,0 +1,123 @@
+"""What the 8-bit operators refuse, before any GPU call: through the C entry points, and through Python on CPU tensors."""
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from lightop_amd import _lib
+
+    return _lib.lib()
+
+
+P = 4096  # stands for an aligned pointer; nothing below gets as far as using it
+
+
+def _norm(lib, **k):
+    a = dict(x=P, dtype=0, xs=256, r=P, rs=256, w=P, wt=0, M=2, H=256, eps=1e-6, form=0, z=P, y=0, q=P, s=P)
+    a.update(k)
+    return lib.lo_rms_norm_quant(a["x"], a["dtype"], a["xs"], a["r"], a["rs"], a["w"], a["wt"], a["M"], a["H"], a["eps"], a["form"], a["z"],
+                                 a["y"], a["q"], a["s"], None)
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=3), dict(wt=1), dict(form=3), dict(form=-1), dict(H=0), dict(H=260), dict(form=1, H=264),
+                                 dict(form=2, H=8), dict(H=65544), dict(eps=-1.0), dict(eps=float("nan")), dict(x=0), dict(w=0), dict(q=0),
+                                 dict(s=0), dict(z=0), dict(M=-1), dict(xs=128), dict(rs=0), dict(xs=260), dict(x=P + 2), dict(w=P + 8),
+                                 dict(q=P + 4), dict(s=P + 2), dict(z=P + 4), dict(y=P + 4), dict(r=P + 4)], ids=str)
+def test_norm_refuses(lib, bad):
+    assert _norm(lib, **bad) < 0
+    assert b"rms_norm_quant" in lib.lo_last_error()
+
+
+def test_no_rows_is_no_error(lib):
+    assert _norm(lib, M=0, x=0, w=0, q=0, s=0, z=0) == 0
+    assert lib.lo_per_token_group_quant_fp8(None, 0, 0, 128, 1e-10, None, None, None) == 0
+    assert lib.lo_act_mul_group_quant_fp8(None, 0, 0, 0, 128, None, None, None) == 0
+    assert lib.lo_gemm_w8a8_fp8_block(None, None, None, None, None, 0, 0, 128, 128, None) == 0
+    assert lib.lo_gemm_w8a8_fp8_block(None, None, None, None, None, 0, 128, 0, 128, None) == 0
+    assert _experts(lib, M=0, x=0, out=0, ws=0) == 0
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=7), dict(rows=-1), dict(cols=0), dict(cols=192), dict(x=0), dict(q=0), dict(s=0), dict(x=P + 8),
+                                 dict(q=P + 4), dict(s=P + 1), dict(eps=0.0), dict(eps=1e-31), dict(eps=float("inf")), dict(eps=float("nan"))],
+                         ids=str)
+def test_group_quant_refuses(lib, bad):
+    a = dict(x=P, dtype=0, rows=1, cols=128, eps=1e-10, q=P, s=P)
+    a.update(bad)
+    assert lib.lo_per_token_group_quant_fp8(a["x"], a["dtype"], a["rows"], a["cols"], a["eps"], a["q"], a["s"], None) < 0
+    if "eps" not in bad:
+        assert lib.lo_act_mul_group_quant_fp8(a["x"], a["dtype"], 0, a["rows"], a["cols"], a["q"], a["s"], None) < 0
+    assert b"group_quant_fp8" in lib.lo_last_error()
+
+
+def test_act_refuses_unknown_activation(lib):
+    assert lib.lo_act_mul_group_quant_fp8(P, 0, 2, 1, 128, P, P, None) < 0
+
+
+@pytest.mark.parametrize("bad", [dict(M=-1), dict(N=-1), dict(K=0), dict(K=64), dict(K=1 << 23), dict(M=1 << 25), dict(N=1 << 25),
+                                 dict(dt=3), dict(a=0), dict(b=0), dict(sa=0), dict(sb=0), dict(c=0), dict(a=P + 8), dict(b=P + 1),
+                                 dict(sa=P + 2), dict(c=P + 1)], ids=str)
+def test_gemm_refuses(lib, bad):
+    a = dict(a=P, sa=P, b=P, sb=P, c=P, dt=0, M=1, N=16, K=128)
+    a.update(bad)
+    assert lib.lo_gemm_w8a8_fp8_block(a["a"], a["sa"], a["b"], a["sb"], a["c"], a["dt"], a["M"], a["N"], a["K"], None) < 0
+    assert b"gemm_w8a8_fp8_block" in lib.lo_last_error()
+
+
+def _experts(lib, **k):
+    a = dict(x=P, dt=0, M=2, H=256, I=128, E=4, Eg=4, top_k=2, w1=P, s1=P, w2=P, s2=P, tw=P, ids=P, it=0, map=0, act=0, sh=0, out=P, ws=P,
+             n=1 << 20)
+    a.update(k)
+    return lib.lo_fused_experts_fp8(a["x"], a["dt"], a["M"], a["H"], a["I"], a["E"], a["Eg"], a["top_k"], a["w1"], a["s1"], a["w2"], a["s2"],
+                                    a["tw"], a["ids"], a["it"], a["map"], a["act"], 1.0, a["sh"], a["out"], a["ws"], a["n"], None)
+
+
+@pytest.mark.parametrize("bad", [dict(dt=2), dict(it=2), dict(act=2), dict(M=-1), dict(H=64), dict(H=320), dict(I=64), dict(E=0), dict(Eg=3),
+                                 dict(Eg=8), dict(top_k=0), dict(M=65), dict(M=64, top_k=17), dict(x=0), dict(w1=0), dict(w2=0), dict(s1=0),
+                                 dict(s2=0), dict(tw=0), dict(ids=0), dict(out=0), dict(ws=0), dict(n=100), dict(x=P + 8), dict(ws=P + 4),
+                                 dict(w2=P + 4), dict(E=4096, Eg=4096), dict(H=1 << 21)], ids=str)
+def test_experts_refuses(lib, bad):
+    assert _experts(lib, **bad) < 0
+    assert b"fused_experts_fp8" in lib.lo_last_error()
+
+
+def test_experts_workspace(lib):
+    n = lib.lo_fused_experts_fp8_workspace_bytes
+    assert n(1, 8, 768, 128) == 8 * 768 * 4 + 8 * 65 * 4
+    assert n(64, 8, 2048, 32) == 512 * 2048 * 4 + 32 * 65 * 4
+    assert n(-1, 8, 768, 128) < 0 and n(1, 0, 768, 128) < 0 and n(1, 1, 64, 1) < 0
+
+
+def test_python_needs_the_gpu():
+    from lightop_amd.gemmopt import gemm_w8a8_fp8_block
+    from lightop_amd.moe import act_and_mul_group_quant_fp8, fused_experts_decode_fp8
+    from lightop_amd.norm import rms_norm_quant
+    from lightop_amd.quant import per_token_group_quant_fp8
+
+    x, f8 = torch.zeros(2, 256, dtype=torch.bfloat16), torch.zeros(256, 256).to(torch.float8_e4m3fn)
+    s = torch.zeros(2, 2)
+    for call in (lambda: rms_norm_quant(x, x[0]), lambda: per_token_group_quant_fp8(x, 128), lambda: act_and_mul_group_quant_fp8(x),
+                 lambda: gemm_w8a8_fp8_block(f8[:2], f8, s, s),
+                 lambda: fused_experts_decode_fp8(x, f8[None], f8[None, :, :128], s, s.int(), s[None], s[None, :, :1])):
+        with pytest.raises(RuntimeError, match="GPU"):
+            call()
+    with pytest.raises(RuntimeError, match="group_size"):
+        rms_norm_quant(x, x[0], quant_dtype=torch.float8_e4m3fn)
+    with pytest.raises(RuntimeError, match="float8_e4m3fn"):
+        per_token_group_quant_fp8(x, 128, dtype=torch.int8)
+    with pytest.raises(RuntimeError, match="128"):
+        per_token_group_quant_fp8(x, 64)
+    with pytest.raises(ValueError):
+        act_and_mul_group_quant_fp8(x, "relu")
+
+
+def test_names_are_reachable():
+    import lightop
+    import lightop.norm
+    import lightop_amd
+
+    assert lightop.norm.rms_norm_quant is lightop_amd.norm.rms_norm_quant is lightop.rms_norm_quant
+    assert lightop.moe.fused_experts_decode_fp8 is lightop_amd.moe.fused_experts_decode_fp8
+    assert lightop.gemmopt.gemm_w8a8_fp8_block and lightop.quant.per_token_group_quant_fp8

@@ -1,0 +1,159 @@
+"""Dense e4m3 product with block scales against float64."""
+import pytest
+import torch
+
+import fp8_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def _make(M, N, K, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed + M * 7 + N * 3 + K)
+    quotient, s = ref.groups_fp8(ref.rows(M, K, g, "cuda").double())
+    b, bs = ref.weights((N, K), g, "cuda")
+    return quotient.float().to(ref.FP8), b, s.float(), bs
+
+
+def _bound(a, b, sa, sb, dtype, exact):
+    """An e4m3 instruction is off by at most 2^-11 of the block's largest product (the bits of the others that it keeps), the exact one by
+    fp32 roundings of 128 products; K / 128 fp32 steps on top, and half a step of the output."""
+    KB = a.shape[1] // 128
+    tops = lambda t: t.double().abs().unflatten(-1, (-1, 128)).amax(-1)
+    rows = sb.double().repeat_interleave(128, 0)[:b.shape[0]]
+    spread = (a.double().abs().unflatten(-1, (-1, 128)) * sa.double().unsqueeze(-1)).flatten(-2) @ ref.dequant(b.float().abs(), rows).T
+    off = spread * (KB + 132 + 4) * ref.ULP32
+    if dtype != torch.float32:
+        off = off + 2.0 ** -11 * ((tops(a) * sa.double()) @ (tops(b) * rows).T)
+    return off + 1.01 * ref.half_step(dtype, exact)
+
+
+def _check(out, a, b, sa, sb):
+    exact = ref.dequant(a, sa) @ ref.dequant_weight(b, sb).T
+    assert out.shape == exact.shape
+    assert ((out.double() - exact).abs() <= _bound(a, b, sa, sb, out.dtype, exact)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 33, 48, 64, 65, 100, 128, 129, 200, 257, 400, 777])
+@pytest.mark.parametrize("N,K", [(1, 128), (17, 384), (128, 1024), (576, 2048), (1001, 640), (2048, 768)])
+def test_sizes(dtype, M, N, K):
+    from lightop_amd.gemmopt import gemm_w8a8_fp8_block
+
+    print("[case] gemm", dtype, M, N, K, flush=True)
+    a, b, sa, sb = _make(M, N, K)
+    _check(gemm_w8a8_fp8_block(a, b, sa, sb, out_dtype=dtype), a, b, sa, sb)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 7168), (48, 7168, 2048), (333, 576, 7168), (1531, 7168, 2048), (4099, 4096, 1152), (300, 264, 16384),
+                                   (2048, 2048, 2048)])
+def test_full_sizes(M, N, K):
+    from lightop_amd.gemmopt import gemm_w8a8_fp8_block
+
+    print("[case] gemm", M, N, K, flush=True)
+    a, b, sa, sb = _make(M, N, K)
+    out = gemm_w8a8_fp8_block(a, b, sa, sb)
+    _check(out, a, b, sa, sb)
+    assert torch.equal(out, gemm_w8a8_fp8_block(a, b, sa, sb))  # one order of the sum
+
+
+@pytest.mark.parametrize("M", [3, 40, 70, 300, 600])
+@pytest.mark.parametrize("N", [40, 250, 520])
+def test_nothing_else_is_written_and_nans_stay_in_their_row(M, N):
+    from lightop_amd.gemmopt import gemm_w8a8_fp8_block
+
+    a, b, sa, sb = _make(M, N, 512)
+    room = torch.full((M * N + 4096,), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = room[2048:2048 + M * N].view(M, N)
+    want = gemm_w8a8_fp8_block(a, b, sa, sb)
+    got = gemm_w8a8_fp8_block(a, b, sa, sb, out=out)
+    assert got.data_ptr() == out.data_ptr() and torch.equal(out, want)
+    assert (room[:2048] == 7).all() and (room[2048 + M * N:] == 7).all()
+    nan = torch.tensor(float("nan"), device="cuda").to(ref.FP8)
+    a, b = a.clone(), b.clone()
+    a.view(torch.uint8)[M - 1, 5] = nan.view(torch.uint8)
+    b.view(torch.uint8)[N - 1, 200] = nan.view(torch.uint8)
+    got = gemm_w8a8_fp8_block(a, b, sa, sb)
+    assert got[M - 1].isnan().all() and got[:, N - 1].isnan().all() and torch.equal(got[:-1, :-1], want[:-1, :-1])
+    sa = sa.clone()
+    sa[0, 1] = float("inf")
+    assert (~got[1:-1, :-1].isnan()).all() and (~gemm_w8a8_fp8_block(a, b, sa, sb)[0].isfinite()).all()
+
+
+def test_zero_rows_and_columns():
+    from lightop_amd.gemmopt import gemm_w8a8_fp8_block
+
+    a, b, sa, sb = _make(70, 130, 256)
+    assert gemm_w8a8_fp8_block(a[:0], b, sa[:0], sb).shape == (0, 130)
+    assert gemm_w8a8_fp8_block(a, b[:0], sa, sb[:0]).shape == (70, 0)
+    zero = torch.zeros_like(a.float()).to(ref.FP8)
+    assert (gemm_w8a8_fp8_block(zero, b, torch.zeros_like(sa), sb) == 0).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(310000, 24, 7168), (40, 310000, 7168), (70000, 16384, 128)])
+def test_offsets_past_32_bits(M, N, K):
+    """Operands and results of more than 2 GiB: the last rows and columns."""
+    from lightop_amd.gemmopt import gemm_w8a8_fp8_block
+
+    print("[case] gemm", M, N, K, flush=True)
+    g = torch.Generator(device="cuda").manual_seed(5)
+
+    def codes(n):
+        return torch.randint(0, 0x7f, (n, K), generator=g, dtype=torch.uint8, device="cuda").view(ref.FP8)
+
+    a, b = codes(M), codes(N)
+    sa = torch.rand(M, K // 128, generator=g, device="cuda") * 1e-3
+    sb = torch.rand(-(-N // 128), K // 128, generator=g, device="cuda") * 1e-3
+    out = gemm_w8a8_fp8_block(a, b, sa, sb)
+    m, n = min(M, 200), min(N, 128 + N % 128)
+    m0, n0 = M - m, (N - n) // 128 * 128
+    _check(out[m0:, n0:], a[m0:], b[n0:], sa[m0:], sb[n0 // 128:])
+    _check(out[:m, :n], a[:m], b[:n], sa[:m], sb[:-(-n // 128)])
+
+
+def test_strides_batches_and_marshalling(monkeypatch):
+    from lightop_amd import _lib
+    from lightop_amd.gemmopt import gemm_w8a8_fp8_block
+
+    a, b, sa, sb = _make(24, 96, 256)
+    want = gemm_w8a8_fp8_block(a, b, sa, sb)
+    got = gemm_w8a8_fp8_block(a.view(2, 12, 256), b, sa.view(2, 12, 2), sb)
+    assert got.shape == (2, 12, 96) and torch.equal(got.view(24, 96), want)
+    off = torch.zeros(24 * 256 + 1, dtype=torch.uint8, device="cuda")[1:].view(24, 256).copy_(a.view(torch.uint8)).view(ref.FP8)
+    turned = sa.t().contiguous().t()
+    assert torch.equal(gemm_w8a8_fp8_block(off, b, turned, sb), want)
+    wide = torch.zeros(96, 512, dtype=torch.uint8, device="cuda").view(ref.FP8)
+    wide.view(torch.uint8)[:, 256:] = b.view(torch.uint8)
+    assert torch.equal(gemm_w8a8_fp8_block(a, wide[:, 256:], sa, sb), want)
+    monkeypatch.setattr(_lib, "_host", _lib._NoHost())
+    assert torch.equal(gemm_w8a8_fp8_block(a, b, sa, sb), want)
+    for bad in (lambda: gemm_w8a8_fp8_block(a.float(), b, sa, sb), lambda: gemm_w8a8_fp8_block(a, b[:, :128], sa, sb),
+                lambda: gemm_w8a8_fp8_block(a, b, sa[:, :1], sb), lambda: gemm_w8a8_fp8_block(a, b, sa, sb.double()),
+                lambda: gemm_w8a8_fp8_block(a, b, sa, sb, out_dtype=torch.float64), lambda: gemm_w8a8_fp8_block(a, b, sa, sb.cpu()),
+                lambda: gemm_w8a8_fp8_block(a, b, sa, sb, out=want[:, :90]), lambda: gemm_w8a8_fp8_block(a[:, :64], b[:, :64], sa, sb)):
+        with pytest.raises(RuntimeError):
+            bad()
+
+
+@pytest.mark.parametrize("M", [4, 60, 300])
+def test_streams_and_graphs(M):
+    from lightop_amd.gemmopt import gemm_w8a8_fp8_block
+
+    a, b, sa, sb = _make(M, 640, 1024)
+    want = gemm_w8a8_fp8_block(a, b, sa, sb)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = gemm_w8a8_fp8_block(a, b, sa, sb)
+    side.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    sx = sa.clone()
+    with torch.cuda.graph(graph):
+        one = gemm_w8a8_fp8_block(a, b, sx, sb)
+        two = gemm_w8a8_fp8_block(a, b, sx, sb, out_dtype=torch.float32)
+    for k in range(3):
+        sx.copy_(sa * (k + 1))
+        graph.replay()
+        eager = gemm_w8a8_fp8_block(a, b, sa * (k + 1), sb), gemm_w8a8_fp8_block(a, b, sa * (k + 1), sb, out_dtype=torch.float32)
+        torch.cuda.synchronize()
+        assert torch.equal(one, eager[0]) and torch.equal(two, eager[1])

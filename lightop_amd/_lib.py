@@ -110,7 +110,8 @@ SIGNATURES = {
     "lo_per_token_group_quant_fp8": (c_int, [c_void_p, c_int, c_int64, c_int64, c_float, c_void_p, c_void_p, c_void_p]),
     "lo_act_mul_group_quant_fp8": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "lo_gemm_w8a8_fp8_block": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64,
-                                       c_void_p]),
+                                       c_void_p, c_int64, c_void_p]),
+    "lo_gemm_w8a8_fp8_block_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int]),
     "lo_fused_experts_fp8_workspace_bytes": (c_int64, [c_int64, c_int32, c_int64, c_int32]),
     "lo_fused_experts_fp8": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p,
                                      c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_float, c_void_p,
@@ -181,7 +182,7 @@ def host():
             "lo_fused_experts_block_int8", "lo_fused_experts_channel_int8", "lo_fused_experts_workspace_bytes",
             "lo_topk_softmax", "lo_moe_fused_gate", "lo_last_error", "lo_rms_norm_quant", "lo_per_token_group_quant_fp8",
             "lo_act_mul_group_quant_fp8", "lo_gemm_w8a8_fp8_block", "lo_fused_experts_fp8",
-            "lo_fused_experts_fp8_workspace_bytes")))
+            "lo_fused_experts_fp8_workspace_bytes", "lo_gemm_w8a8_fp8_block_workspace_bytes")))
         _host = mod
     return _host
 

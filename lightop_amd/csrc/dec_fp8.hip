@@ -40,14 +40,6 @@ __device__ __forceinline__ int local_expert(const Fp8ExpertsArgs &a, int s) {
   return e >= 0 && e < a.E ? e : -1;
 }
 
-// What lanes of this wave have written to LDS is there for its other lanes (LDS operations of a wave execute in order), and what they
-// have read may be overwritten.
-__device__ __forceinline__ void lds_order() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // A group's codes and scale from eight values on each of 16 lanes, to a row of 128 bytes whose 16-byte pieces are swizzled by the row.
 __device__ __forceinline__ void codes_to_lds(const float (&v)[8], int sub, int row, int8_t *rows, float *scales) {
   float top = 0.0f;

@@ -67,6 +67,14 @@ __device__ __forceinline__ v8i join(const v4i a, const v4i b) {
   return v8i{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
+// What lanes of this wave have written to LDS is there for its other lanes (LDS operations of a wave execute in order), and what they
+// have read may be overwritten.
+__device__ __forceinline__ void lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Eight values from x + at, as floats.
 template <int DT> __device__ __forceinline__ void load8(const void *x, int64_t at, float (&v)[8]) {
   if constexpr (DT == LO_F32) {

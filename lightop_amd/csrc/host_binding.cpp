@@ -40,6 +40,7 @@ decltype(&lo_rms_norm_quant) g_norm = nullptr;
 decltype(&lo_per_token_group_quant_fp8) g_quant_fp8 = nullptr;
 decltype(&lo_act_mul_group_quant_fp8) g_act_fp8 = nullptr;
 decltype(&lo_gemm_w8a8_fp8_block) g_gemm_fp8 = nullptr;
+decltype(&lo_gemm_w8a8_fp8_block_workspace_bytes) g_gemm_fp8_bytes = nullptr;
 decltype(&lo_fused_experts_fp8) g_experts_fp8 = nullptr;
 decltype(&lo_fused_experts_fp8_workspace_bytes) g_experts_fp8_bytes = nullptr;
 
@@ -494,6 +495,9 @@ PyObject *gemm_fp8(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   if (as.sizes() != at::IntArrayRef(sizes) || bs.sizes() != at::IntArrayRef({(N + 127) / 128, K / 128})) Py_RETURN_NONE;
   sizes.back() = N;
   const hipStream_t stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream();
+  const int64_t bytes = g_gemm_fp8_bytes(M, N, K, static_cast<int>(dtype));
+  if (bytes < 0) return raise(static_cast<int>(bytes));
+  if (bytes > 0 && capturing(stream)) Py_RETURN_NONE; // (its scratch belongs to the graph)
   const void *ap = a.data_ptr(), *bp = b.data_ptr();
   const float *asp = as.data_ptr<float>(), *bsp = bs.data_ptr<float>();
   const auto opts = a.options().requires_grad(false).dtype(dtype == LO_BF16 ? at::kBFloat16 : dtype == LO_F16 ? at::kHalf : at::kFloat);
@@ -502,7 +506,13 @@ PyObject *gemm_fp8(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   {
     const NoGil nogil;
     out = at::empty(sizes, opts);
-    rc = g_gemm_fp8(ap, asp, bp, bsp, out.data_ptr(), static_cast<int>(dtype), M, N, K, stream);
+    if (bytes == 0) {
+      rc = g_gemm_fp8(ap, asp, bp, bsp, out.data_ptr(), static_cast<int>(dtype), M, N, K, nullptr, 0, stream);
+    } else {
+      const std::shared_ptr<Scratch> ws = workspace_for(bytes, dev, stream);
+      const std::lock_guard<std::mutex> lock(ws->busy);
+      rc = g_gemm_fp8(ap, asp, bp, bsp, out.data_ptr(), static_cast<int>(dtype), M, N, K, ws->buf.data_ptr(), bytes, stream);
+    }
   }
   if (rc < 0) return raise(rc);
   return THPVariable_Wrap(std::move(out));
@@ -574,10 +584,11 @@ PyObject *experts_fp8(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 
 // bind(lo_fused_experts_block_int8, lo_fused_experts_channel_int8, lo_fused_experts_workspace_bytes, lo_topk_softmax,
 //      lo_moe_fused_gate, lo_last_error, lo_rms_norm_quant, lo_per_token_group_quant_fp8, lo_act_mul_group_quant_fp8,
-//      lo_gemm_w8a8_fp8_block, lo_fused_experts_fp8, lo_fused_experts_fp8_workspace_bytes): addresses of the library's functions.
+//      lo_gemm_w8a8_fp8_block, lo_fused_experts_fp8, lo_fused_experts_fp8_workspace_bytes, lo_gemm_w8a8_fp8_block_workspace_bytes): addresses of the library's functions.
 PyObject *bind(PyObject *, PyObject *args) {
-  unsigned long long a[12];
-  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9], &a[10], &a[11]))
+  unsigned long long a[13];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9], &a[10], &a[11],
+                        &a[12]))
     return nullptr;
   g_block = reinterpret_cast<decltype(g_block)>(a[0]);
   g_channel = reinterpret_cast<decltype(g_channel)>(a[1]);
@@ -591,6 +602,7 @@ PyObject *bind(PyObject *, PyObject *args) {
   g_gemm_fp8 = reinterpret_cast<decltype(g_gemm_fp8)>(a[9]);
   g_experts_fp8 = reinterpret_cast<decltype(g_experts_fp8)>(a[10]);
   g_experts_fp8_bytes = reinterpret_cast<decltype(g_experts_fp8_bytes)>(a[11]);
+  g_gemm_fp8_bytes = reinterpret_cast<decltype(g_gemm_fp8_bytes)>(a[12]);
   Py_RETURN_NONE;
 }
 

@@ -7,7 +7,7 @@ from typing import Any, Dict, Optional
 import torch
 
 from . import _lib
-from .op import _act_dtype, _on_device, _one_device, _require_cuda, _rows16
+from .op import _act_dtype, _on_device, _one_device, _require_cuda, _rows16, _scratch
 
 
 _OUT_DTYPES = {torch.bfloat16: _lib.LO_BF16, torch.float16: _lib.LO_F16, torch.float32: _lib.LO_F32}
@@ -84,9 +84,14 @@ def gemm_w8a8_fp8_block(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor,
     if out.numel() == 0:
         return out
     a, b, a_scale, b_scale = _rows16(a), _rows16(b), a_scale.contiguous(), b_scale.contiguous()
+    lib, M = _lib.lib(), out.numel() // N
+    nbytes = lib.lo_gemm_w8a8_fp8_block_workspace_bytes(M, N, K, dtype)
+    _lib.check(nbytes)
     with _on_device(a):
-        _lib.check(_lib.lib().lo_gemm_w8a8_fp8_block(_lib.ptr(a), _lib.ptr(a_scale), _lib.ptr(b), _lib.ptr(b_scale), _lib.ptr(out),
-                                                     dtype, out.numel() // N, N, K, _lib.stream_of(a)))
+        stream = torch.cuda.current_stream(a.device).cuda_stream
+        scratch = _scratch(nbytes, a.device, stream) if nbytes else None
+        _lib.check(lib.lo_gemm_w8a8_fp8_block(_lib.ptr(a), _lib.ptr(a_scale), _lib.ptr(b), _lib.ptr(b_scale), _lib.ptr(out), dtype, M, N, K,
+                                              _lib.ptr(scratch), nbytes, _lib.stream_of(a)))
     return out
 
 

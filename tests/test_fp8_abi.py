@@ -35,8 +35,8 @@ def test_no_rows_is_no_error(lib):
     assert _norm(lib, M=0, x=0, w=0, q=0, s=0, z=0) == 0
     assert lib.lo_per_token_group_quant_fp8(None, 0, 0, 128, 1e-10, None, None, None) == 0
     assert lib.lo_act_mul_group_quant_fp8(None, 0, 0, 0, 128, None, None, None) == 0
-    assert lib.lo_gemm_w8a8_fp8_block(None, None, None, None, None, 0, 0, 128, 128, None) == 0
-    assert lib.lo_gemm_w8a8_fp8_block(None, None, None, None, None, 0, 128, 0, 128, None) == 0
+    assert lib.lo_gemm_w8a8_fp8_block(None, None, None, None, None, 0, 0, 128, 128, None, 0, None) == 0
+    assert lib.lo_gemm_w8a8_fp8_block(None, None, None, None, None, 0, 128, 0, 128, None, 0, None) == 0
     assert _experts(lib, M=0, x=0, out=0, ws=0) == 0
 
 
@@ -58,11 +58,12 @@ def test_act_refuses_unknown_activation(lib):
 
 @pytest.mark.parametrize("bad", [dict(M=-1), dict(N=-1), dict(K=0), dict(K=64), dict(K=1 << 23), dict(M=1 << 25), dict(N=1 << 25),
                                  dict(dt=3), dict(a=0), dict(b=0), dict(sa=0), dict(sb=0), dict(c=0), dict(a=P + 8), dict(b=P + 1),
-                                 dict(sa=P + 2), dict(c=P + 1)], ids=str)
+                                 dict(sa=P + 2), dict(c=P + 1), dict(ws=P + 8, n=64), dict(ws=P, n=-1)], ids=str)
 def test_gemm_refuses(lib, bad):
-    a = dict(a=P, sa=P, b=P, sb=P, c=P, dt=0, M=1, N=16, K=128)
+    a = dict(a=P, sa=P, b=P, sb=P, c=P, dt=0, M=1, N=16, K=128, ws=0, n=0)
     a.update(bad)
-    assert lib.lo_gemm_w8a8_fp8_block(a["a"], a["sa"], a["b"], a["sb"], a["c"], a["dt"], a["M"], a["N"], a["K"], None) < 0
+    assert lib.lo_gemm_w8a8_fp8_block(a["a"], a["sa"], a["b"], a["sb"], a["c"], a["dt"], a["M"], a["N"], a["K"], a["ws"], a["n"],
+                                      None) < 0
     assert b"gemm_w8a8_fp8_block" in lib.lo_last_error()
 
 
@@ -81,6 +82,14 @@ def _experts(lib, **k):
 def test_experts_refuses(lib, bad):
     assert _experts(lib, **bad) < 0
     assert b"fused_experts_fp8" in lib.lo_last_error()
+
+
+def test_gemm_workspace(lib):
+    n = lib.lo_gemm_w8a8_fp8_block_workspace_bytes
+    assert n(1, 4096, 7168, 0) == 0 and n(8192, 4096, 7168, 0) == 0  # no parts
+    assert n(333, 576, 7168, 0) > 0 and n(333, 576, 7168, 0) % (333 * 576 * 4) == 0
+    assert n(333, 575, 7168, 0) % (333 * 576 * 4) == 0               # rows of a part begin on 16 bytes
+    assert n(-1, 16, 128, 0) < 0 and n(1, 16, 100, 0) < 0 and n(100, 0, 128, 0) == 0
 
 
 def test_experts_workspace(lib):

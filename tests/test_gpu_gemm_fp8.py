@@ -157,3 +157,25 @@ def test_streams_and_graphs(M):
         eager = gemm_w8a8_fp8_block(a, b, sa * (k + 1), sb), gemm_w8a8_fp8_block(a, b, sa * (k + 1), sb, out_dtype=torch.float32)
         torch.cuda.synchronize()
         assert torch.equal(one, eager[0]) and torch.equal(two, eager[1])
+
+
+@pytest.mark.parametrize("M,N,K", [(20, 576, 7168), (333, 576, 7168), (333, 577, 4096), (333, 577, 7168), (600, 4096, 7168), (130, 300, 16384)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_without_room_for_parts(M, N, K, dtype):
+    """The C entry point with no workspace, and with one that is too small by a byte: K in one piece.  (Which sizes are split
+    differs by the output's type; the smallest and narrowest are.)"""
+    from lightop_amd import _lib
+
+    a, b, sa, sb = _make(M, N, K)
+    lib, code = _lib.lib(), {torch.bfloat16: 0, torch.float32: 2}[dtype]
+    need = lib.lo_gemm_w8a8_fp8_block_workspace_bytes(M, N, K, code)
+    assert need > 0 or M * N > 150000
+    room = torch.full((need + 256,), 0xff, dtype=torch.uint8, device="cuda")
+    outs = []
+    for n in sorted({0, max(need - 1, 0), need}):
+        out = torch.empty(M, N, dtype=dtype, device="cuda")
+        _lib.check(lib.lo_gemm_w8a8_fp8_block(_lib.ptr(a), _lib.ptr(sa), _lib.ptr(b), _lib.ptr(sb), _lib.ptr(out), code, M, N, K,
+                                              _lib.ptr(room if n else None), n, _lib.stream_of(a)))
+        _check(out, a, b, sa, sb)
+        outs.append(out)
+    assert (room[need:] == 0xff).all()

@@ -1,12 +1,13 @@
 // The experts of a few tokens with e4m3 weights (128 x 128 blocks) in two launches:
 //   h = xq w1[e]^T,  v = act(h[:I]) * h[I:],  y = vq w2[e]^T,  out[t] = factor * sum_j w[t, j] * y[t, e_j] (+ shared[t]),
 // xq and vq the e4m3 codes of rows in groups of 128 (fp8.h).  At these sizes the layer is a stream of the hit experts' weights:
-//   up     one workgroup per (expert hit, 16 columns of I).  It finds the slots of its expert, its waves share the K blocks of the 16 gate
-//          and 16 up rows and quantise their part of the token rows into LDS while the weights are on their way, and the sums meet in
-//          LDS.  v goes to the workspace in fp32: rounded on the way it would move codes of the second quantisation.
+//   up     one workgroup per (expert hit, 16 columns of I).  Its waves share the K blocks of the 16 gate and 16 up rows and quantise their part
+//          of the token rows into LDS while the weights are on their way; the sums meet in LDS.  v goes to the workspace in fp32: rounded
+//          on the way it would move codes of the second quantisation.
 //   down   one workgroup per 16 columns of the output.  Its waves share (expert hit, part of K) and leave each slot's 16 values in LDS;
-//          then every token's slots are added up in their order.  No atomics: the order of every sum is fixed.
-// Both products are the exact ones (fp8.h): the matrix cores have time, and an error of 1e-5 moves codes of the second quantisation.
+//          then every token's slots are added up in their order.  No atomics on results: the order of every sum is fixed.
+// Both find the experts hit from the ids by themselves.  Both
+// products are the exact ones (fp8.h): the matrix cores have time, and an error of 1e-5 moves codes of the second quantisation.
 // Ids that no expert of this rank answers to (out of range, or -1 in the map) add nothing.  An id that a token has twice is computed once
 // and counted with both weights.
 #include "gemm.h"
@@ -14,10 +15,11 @@
 
 namespace lo {
 
-constexpr int kFewTokens = 64;  // one expert's list
-constexpr int kFewSlots = 1024; // of a call
-constexpr int kUpU = 3, kDownU = 2; // K blocks of a wave in flight
-constexpr int kFewWaves = 8;
+constexpr int kFewTokens = 64;   // of a call
+constexpr int kFewSlots = 1024;
+constexpr int kFewExperts = 2048;
+constexpr int kFewU = 4;         // K blocks of a wave in flight
+constexpr int kFewMaxWaves = 16;
 
 struct Fp8ExpertsArgs {
   const void *x, *ids, *shared;
@@ -26,9 +28,8 @@ struct Fp8ExpertsArgs {
   const int32_t *map;
   void *out;
   float *act;       // [slots, I]
-  int32_t *counts;  // [units] tokens of the unit's expert
-  int32_t *lists;   // [units, kFewTokens] their slots
   int32_t S, H, I, E, Eg, top_k, units, parts;
+  int32_t rows;     // of a wave's codes: min(tokens, 16)
   float factor;
   bool ids64, by_slot;
 };
@@ -39,6 +40,50 @@ __device__ __forceinline__ int local_expert(const Fp8ExpertsArgs &a, int s) {
   const int e = a.map ? a.map[id] : static_cast<int>(id);
   return e >= 0 && e < a.E ? e : -1;
 }
+
+// ---- which experts are hit, and by which slots --------------------------------------------------------------------------------
+// SMALL (up to 64 slots): a wave has a slot a lane and needs nobody.  Else the slots' experts are in LDS.
+template <bool SMALL> struct Route {
+  const Fp8ExpertsArgs &a;
+  int16_t *keys; // LDS, [slots]: expert, -1 for none here
+  int lane;
+  int key = -1;  // SMALL: expert of slot `lane`
+
+  __device__ __forceinline__ Route(const Fp8ExpertsArgs &args, int16_t *k, int ln) : a(args), keys(k), lane(ln) {
+    if constexpr (SMALL) {
+      if (lane < a.S) key = local_expert(a, lane);
+    } else {
+      for (int s = threadIdx.x; s < a.S; s += blockDim.x) keys[s] = static_cast<int16_t>(local_expert(a, s));
+      __syncthreads();
+    }
+  }
+  __device__ __forceinline__ int slot_expert(int s) const {
+    return SMALL ? __builtin_amdgcn_readlane(key, s) : __builtin_amdgcn_readfirstlane(keys[s]);
+  }
+  // The expert's slots, one a token, into the wave's list, and how many; none if `lead` is not negative and not the first of them.
+  __device__ __forceinline__ int slots(int e, int lead, int16_t *list) const {
+    int count = 0;
+    for (int base = 0; base < (SMALL ? 1 : a.S); base += 64) {
+      const int s = base + lane;
+      bool hit = SMALL ? key == e : s < a.S && keys[s] == e;
+      const uint64_t all = __builtin_amdgcn_ballot_w64(hit);
+      if (!all) continue;
+      if (lead >= 0 && count == 0 && base + __builtin_ctzll(all) != lead) return 0;
+      if constexpr (SMALL) { // (not a token's later slots with this expert)
+        hit = hit && !(all & earlier_of_token());
+      } else if (hit) {
+        for (int j = s / a.top_k * a.top_k; j < s; ++j) hit = hit && keys[j] != e;
+      }
+      const uint64_t hits = __builtin_amdgcn_ballot_w64(hit);
+      if (hit) list[count + __popcll(hits & ((1ull << lane) - 1))] = static_cast<int16_t>(s);
+      count += __popcll(hits);
+    }
+    lds_order();
+    return __builtin_amdgcn_readfirstlane(count);
+  }
+  // SMALL: lanes of the token's slots before this one
+  __device__ __forceinline__ uint64_t earlier_of_token() const { return (1ull << lane) - (1ull << lane / a.top_k * a.top_k); }
+};
 
 // A group's codes and scale from eight values on each of 16 lanes, to a row of 128 bytes whose 16-byte pieces are swizzled by the row.
 __device__ __forceinline__ void codes_to_lds(const float (&v)[8], int sub, int row, int8_t *rows, float *scales) {
@@ -58,37 +103,25 @@ __device__ __forceinline__ v8i codes_from_lds(const int8_t *rows, int r, int q) 
               *reinterpret_cast<const v4i *>(rows + r * kGroup + (((q + 4) ^ (r & 7)) * 16)));
 }
 
-template <int DT, int ACT>
-__global__ __launch_bounds__(kFewWaves * 64) void experts_fp8_up_kernel(const Fp8ExpertsArgs a) {
-  __shared__ __attribute__((aligned(16))) int8_t codes[kFewWaves][kUpU][16 * kGroup];
-  __shared__ float scales[kFewWaves][kUpU][16];
-  __shared__ int16_t key[kFewSlots];
-  __shared__ int16_t list[kFewWaves][kFewTokens];
-  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
+// LDS of a wave: codes of kFewU K blocks, their scales, two lists of slots
+__host__ __device__ constexpr int few_wave_lds(int rows) { return kFewU * (rows * kGroup + 64) + 2 * kFewTokens * 2; }
+constexpr int kFewRed = 2048; // gate and up sums of a wave (up)
+
+// A unit is a slot where there are fewer slots than experts (the first of its expert's; the others' workgroups end), else an expert.
+template <int DT, int ACT, bool SMALL>
+__global__ __launch_bounds__(512) void experts_fp8_up_kernel(const Fp8ExpertsArgs a) {
+  extern __shared__ __attribute__((aligned(16))) int8_t smem[]; // [wave] codes, scales, list; [wave] sums; slots' experts
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int u = blockIdx.y, n0 = blockIdx.x * 16, H = a.H, I = a.I, KB = H / kGroup;
-  for (int s = tid; s < a.S; s += kFewWaves * 64) key[s] = static_cast<int16_t>(local_expert(a, s));
-  __syncthreads();
-  // the expert's slots in their order, one a token; every wave has its own list
-  const int e = __builtin_amdgcn_readfirstlane(a.by_slot ? key[u] : u);
-  int count = 0;
-  if (e >= 0)
-    for (int base = 0; base < a.S; base += 64) {
-      const int s = base + lane;
-      bool hit = s < a.S && key[s] == e;
-      if (hit)
-        for (int j = s / a.top_k * a.top_k; j < s; ++j) hit = hit && key[j] != e;
-      const uint64_t hits = __builtin_amdgcn_ballot_w64(hit);
-      if (hit) list[wave][count + __popcll(hits & ((1ull << lane) - 1))] = static_cast<int16_t>(s);
-      count += __popcll(hits);
-    }
-  lds_order();
-  if (a.by_slot && count && list[wave][0] != u) count = 0; // an earlier slot's workgroups have this expert
-  count = __builtin_amdgcn_readfirstlane(count);
-  if (n0 == 0 && wave == 0) {
-    if (lane == 0) a.counts[u] = count;
-    if (lane < count) a.lists[u * kFewTokens + lane] = list[0][lane];
-  }
+  const int n0 = blockIdx.x * 16, u = blockIdx.y, H = a.H, I = a.I, KB = H / kGroup, R = a.rows, per = few_wave_lds(R);
+  int8_t *const codes = smem + wave * per;
+  float *const scales = reinterpret_cast<float *>(codes + kFewU * R * kGroup);
+  int16_t *const list = reinterpret_cast<int16_t *>(scales + kFewU * 16);
+  float *const red = reinterpret_cast<float *>(smem + waves * per); // [wave][gate, up][token][column]
+  const Route<SMALL> route(a, reinterpret_cast<int16_t *>(smem + waves * (per + kFewRed)), lane);
+  const int e = a.by_slot ? route.slot_expert(u) : u;
+  if (e < 0) return;
+  const int count = route.slots(e, a.by_slot ? u : -1, list);
   if (!count) return;
 
   const int8_t *const w = a.w1 + static_cast<int64_t>(e) * 2 * I * H;
@@ -96,31 +129,34 @@ __global__ __launch_bounds__(kFewWaves * 64) void experts_fp8_up_kernel(const Fp
   const brsrc rU = make_rsrc(w + static_cast<int64_t>(I + n0) * H, static_cast<uint32_t>(16 * H));
   const float *const sg = a.w1s + (static_cast<int64_t>(e) * (2 * I / kGroup) + n0 / kGroup) * KB;
   const float *const su = sg + static_cast<int64_t>(I / kGroup) * KB;
-  for (int f = 0; f < count; f += 16) {
+  for (int f = 0; f < count; f += 16) { // (more than 16 tokens of one expert read its weights again, out of L2)
     const int n = count - f < 16 ? count - f : 16;
     v4f acc[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
-    for (int kb0 = wave; kb0 < KB; kb0 += kFewWaves * kUpU) {
-      v8i wg[kUpU], wu[kUpU];
+    for (int kb0 = wave; kb0 < KB; kb0 += waves * kFewU) {
+      v8i wg[kFewU], wu[kFewU];
+      float bg[kFewU], bu[kFewU];
 #pragma unroll
-      for (int k = 0; k < kUpU; ++k) {
-        const int kb = kb0 + k * kFewWaves, at = r * H + q * 16 + (kb < KB ? kb : kb0) * kGroup;
+      for (int k = 0; k < kFewU; ++k) {
+        const int kb = kb0 + k * waves, kc = kb < KB ? kb : kb0, at = r * H + q * 16 + kc * kGroup;
         wg[k] = join(bld16(rG, at, 0), bld16(rG, at + 64, 0));
         wu[k] = join(bld16(rU, at, 0), bld16(rU, at + 64, 0));
+        bg[k] = sg[kc];
+        bu[k] = su[kc];
       }
-      for (int g = q; g < n * kUpU; g += 4) { // 16 lanes a group
-        const int row = g / kUpU, k = g % kUpU, kb = kb0 + k * kFewWaves;
+      for (int g = q; g < n * kFewU; g += 4) { // 16 lanes a group
+        const int row = g / kFewU, k = g % kFewU, kb = kb0 + k * waves;
         if (kb >= KB) continue;
         float v[8];
-        load8<DT>(a.x, static_cast<int64_t>(list[wave][f + row] / a.top_k) * H + kb * kGroup + r * 8, v);
-        codes_to_lds(v, r, row, codes[wave][k], scales[wave][k]);
+        load8<DT>(a.x, static_cast<int64_t>(list[f + row] / a.top_k) * H + kb * kGroup + r * 8, v);
+        codes_to_lds(v, r, row, codes + k * R * kGroup, scales + k * 16);
       }
       lds_order();
 #pragma unroll
-      for (int k = 0; k < kUpU; ++k) {
-        const int kb = kb0 + k * kFewWaves;
-        if (kb >= KB) break;
-        const v8i x = codes_from_lds(codes[wave][k], r, q); // (rows from n on hold anything: columns that are not kept)
-        const float s = scales[wave][k][r], s0 = s * sg[kb], s1 = s * su[kb];
+      for (int k = 0; k < kFewU; ++k) {
+        if (kb0 + k * waves >= KB) break;
+        const int row = r < n ? r : 0; // (columns from n on are not kept)
+        const v8i x = codes_from_lds(codes + k * R * kGroup, row, q);
+        const float s = scales[k * 16 + row], s0 = s * bg[k], s1 = s * bu[k];
         const v4f d0 = mfma_e4m3_exact(wg[k], x), d1 = mfma_e4m3_exact(wu[k], x);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -130,120 +166,216 @@ __global__ __launch_bounds__(kFewWaves * 64) void experts_fp8_up_kernel(const Fp
       }
       lds_order();
     }
-    // [gate, up][token][column] of the wave, over its codes
-    const auto red = [&](int w) { return reinterpret_cast<float *>(codes[w][0]); };
-    lds_order();
+    if (f) __syncthreads();
 #pragma unroll
-    for (int h = 0; h < 2; ++h) *reinterpret_cast<v4f *>(red(wave) + h * 256 + r * 16 + 4 * q) = acc[h];
+    for (int h = 0; h < 2; ++h) *reinterpret_cast<v4f *>(red + wave * 512 + h * 256 + r * 16 + 4 * q) = acc[h];
     __syncthreads();
-    if (tid < n * 16) {
+    for (int o = tid; o < n * 16; o += blockDim.x) {
       float g = 0.0f, up = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kFewWaves; ++i) g += red(i)[tid], up += red(i)[256 + tid];
-      a.act[static_cast<int64_t>(list[0][f + (tid >> 4)]) * I + n0 + (tid & 15)] = act_mul_f32<ACT>(g, up);
+      for (int i = 0; i < waves; ++i) g += red[i * 512 + o], up += red[i * 512 + 256 + o];
+      a.act[static_cast<int64_t>(list[f + (o >> 4)]) * I + n0 + (o & 15)] = act_mul_f32<ACT>(g, up);
     }
-    __syncthreads();
   }
 }
 
-template <int DT>
-__global__ __launch_bounds__(kFewWaves * 64) void experts_fp8_down_kernel(const Fp8ExpertsArgs a) {
-  __shared__ __attribute__((aligned(16))) int8_t codes[kFewWaves][kDownU][16 * kGroup];
-  __shared__ float scales[kFewWaves][kDownU][16];
-  __shared__ int16_t key[kFewSlots];
-  __shared__ int16_t unit[kFewSlots]; // units with tokens
-  __shared__ int units;
-  extern __shared__ __attribute__((aligned(16))) float ys[]; // [part][slot][column]
-  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
+template <int DT, bool SMALL>
+__global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8ExpertsArgs a) {
+  // [wave] codes, scales, lists; [part][slot][column] results; [slot] weight; [slot] the token's first one with this expert, -1: none here;
+  // [slot] expert; the experts hit
+  extern __shared__ __attribute__((aligned(16))) int8_t smem[];
+  __shared__ uint32_t present[kFewExperts / 32];
+  __shared__ int number;
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n0 = blockIdx.x * 16, I = a.I, KB = I / kGroup;
-  for (int s = tid; s < a.S; s += kFewWaves * 64) key[s] = static_cast<int16_t>(local_expert(a, s));
-  if (wave == 0) {
-    int found = 0;
-    for (int base = 0; base < a.units; base += 64) {
-      const bool hit = base + lane < a.units && a.counts[base + lane] > 0;
-      const uint64_t hits = __builtin_amdgcn_ballot_w64(hit);
-      if (hit) unit[found + __popcll(hits & ((1ull << lane) - 1))] = static_cast<int16_t>(base + lane);
-      found += __popcll(hits);
-    }
-    if (lane == 0) units = found;
-  }
-  __syncthreads();
-  const int items = units * a.parts;
-  for (int it = wave; it < items; it += kFewWaves) {
-    const int part = it % a.parts, u = __builtin_amdgcn_readfirstlane(unit[it / a.parts]);
-    const int count = a.counts[u];
-    const int32_t *const list = a.lists + u * kFewTokens;
-    const int e = __builtin_amdgcn_readfirstlane(key[list[0]]);
-    const int lo = KB * part / a.parts, hi = KB * (part + 1) / a.parts;
-    const brsrc rW = make_rsrc(a.w2 + (static_cast<int64_t>(e) * a.H + n0) * I, static_cast<uint32_t>(16 * I));
-    const float *const sw = a.w2s + (static_cast<int64_t>(e) * (a.H / kGroup) + n0 / kGroup) * KB;
-    for (int f = 0; f < count; f += 16) {
-      const int n = count - f < 16 ? count - f : 16;
-      v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int kb0 = lo; kb0 < hi; kb0 += kDownU) {
-        v8i w[kDownU];
-#pragma unroll
-        for (int k = 0; k < kDownU; ++k) {
-          const int at = r * I + q * 16 + (kb0 + k < hi ? kb0 + k : kb0) * kGroup;
-          w[k] = join(bld16(rW, at, 0), bld16(rW, at + 64, 0));
-        }
-        for (int g = q; g < n * kDownU; g += 4) {
-          const int row = g / kDownU, k = g % kDownU, kb = kb0 + k;
-          if (kb >= hi) continue;
-          float v[8];
-          load8<LO_F32>(a.act, static_cast<int64_t>(list[f + row]) * I + kb * kGroup + r * 8, v);
-          codes_to_lds(v, r, row, codes[wave][k], scales[wave][k]);
-        }
-        lds_order();
-#pragma unroll
-        for (int k = 0; k < kDownU; ++k) {
-          if (kb0 + k >= hi) break;
-          const v4f d = mfma_e4m3_exact(w[k], codes_from_lds(codes[wave][k], r, q));
-          const float s = scales[wave][k][r] * sw[kb0 + k];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s, acc[i]);
-        }
-        lds_order();
+  const int n0 = blockIdx.x * 16, I = a.I, KB = I / kGroup, R = a.rows, per = few_wave_lds(R), parts = a.parts, S = a.S, M = S / a.top_k;
+  int8_t *const codes = smem + wave * per;
+  float *const scales = reinterpret_cast<float *>(codes + kFewU * R * kGroup);
+  int16_t *const lists = reinterpret_cast<int16_t *>(scales + kFewU * 16);
+  float *const ys = reinterpret_cast<float *>(smem + waves * per), *const weight = ys + parts * S * 16;
+  int16_t *const from = reinterpret_cast<int16_t *>(weight + S), *const keys = from + S, *const hit = keys + S;
+  for (int s = tid; s < S; s += blockDim.x) weight[s] = a.topk_w[s];
+  // (asked for here, not behind the last product)
+  float shared = 0.0f;
+  if (a.shared && tid < M * 16) shared = to_f32<DT>(static_cast<const uint16_t *>(a.shared)[static_cast<int64_t>(tid >> 4) * a.H + n0 + (tid & 15)]);
+  if constexpr (!SMALL)
+    for (int i = tid; i < kFewExperts / 32; i += blockDim.x) present[i] = 0;
+  const Route<SMALL> route(a, keys, lane);
+  uint64_t leaders = 0; // SMALL: first slots of the experts hit
+  int experts = 0;
+  if constexpr (SMALL) {
+    uint64_t left = __builtin_amdgcn_ballot_w64(route.key >= 0);
+    int mine = -1;
+    while (left) { // an expert at a time
+      const int s = __builtin_ctzll(left);
+      const uint64_t same = __builtin_amdgcn_ballot_w64(route.key == __builtin_amdgcn_readlane(route.key, s));
+      if (same >> lane & 1) {
+        const uint64_t before = same & route.earlier_of_token();
+        mine = before ? __builtin_ctzll(before) : lane;
       }
-      if (r < n) *reinterpret_cast<v4f *>(ys + (part * a.S + list[f + r]) * 16 + 4 * q) = acc;
+      left &= ~same;
+      leaders |= 1ull << s;
+      ++experts;
     }
+    if (wave == 0 && lane < S) from[lane] = static_cast<int16_t>(mine);
+  } else {
+    for (int s = tid; s < S; s += blockDim.x) {
+      const int e = keys[s], s0 = s / a.top_k * a.top_k;
+      int j = s0;
+      while (j < s && keys[j] != e) ++j;
+      from[s] = static_cast<int16_t>(e < 0 ? -1 : j);
+      if (e >= 0) atomicOr(&present[e >> 5], 1u << (e & 31));
+    }
+    __syncthreads();
+    if (wave == 0) {
+      static_assert(kFewExperts / 32 == 64, "a word a lane");
+      uint32_t left = present[lane];
+      int before = __popc(left), all = before; // of the lanes up to this one
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(all, d);
+        if (lane >= d) all += o;
+      }
+      before = all - before;
+      for (; left; left &= left - 1) hit[before++] = static_cast<int16_t>(lane * 32 + __builtin_ctz(left));
+      if (lane == 63) number = all;
+    }
+    __syncthreads();
+    experts = number;
+  }
+
+  // The wave's work: (expert, part of K, 16 of its tokens), every `waves`-th (expert, part); up to kFewU K blocks at a time, the next ones'
+  // weights asked for before these are used.
+  const int items = experts * parts;
+  struct Piece {
+    int it, e, part, f, count, kb, hi, list;
+  };
+  auto begin = [&](int it, int list) __attribute__((always_inline)) {
+    Piece p{it, 0, 0, 0, 0, 0, 0, list};
+    if (it >= items) return p;
+    int at = it / parts;
+    p.part = it - at * parts;
+    if constexpr (SMALL) {
+      uint64_t left = leaders;
+      for (; at > 0; --at) left &= left - 1;
+      p.e = route.slot_expert(__builtin_ctzll(left));
+    } else {
+      p.e = __builtin_amdgcn_readfirstlane(hit[at]);
+    }
+    p.kb = KB * p.part / parts;
+    p.hi = KB * (p.part + 1) / parts;
+    return p;
+  };
+  auto find = [&](Piece &p) __attribute__((always_inline)) { // behind the loads of its weights
+    if (p.it < items && p.f == 0 && p.kb == KB * p.part / parts) p.count = route.slots(p.e, -1, lists + p.list * kFewTokens);
+  };
+  auto next = [&](Piece p) __attribute__((always_inline)) {
+    if (p.kb + kFewU < p.hi) {
+      p.kb += kFewU;
+    } else if (p.f + 16 < p.count) {
+      p.f += 16;
+      p.kb = KB * p.part / parts;
+    } else {
+      p = begin(p.it + waves, p.list ^ 1);
+    }
+    return p;
+  };
+  v8i w[2][kFewU];
+  float b[2][kFewU];
+  auto load = [&](const Piece &p, v8i (&to)[kFewU], float (&sc)[kFewU]) __attribute__((always_inline)) {
+    if (p.it >= items) return;
+    const brsrc rW = make_rsrc(a.w2 + (static_cast<int64_t>(p.e) * a.H + n0) * I, static_cast<uint32_t>(16 * I));
+    const float *const sw = a.w2s + (static_cast<int64_t>(p.e) * (a.H / kGroup) + n0 / kGroup) * KB;
+#pragma unroll
+    for (int k = 0; k < kFewU; ++k) {
+      const int kc = p.kb + k < p.hi ? p.kb + k : p.hi - 1, at = r * I + q * 16 + kc * kGroup;
+      to[k] = join(bld16(rW, at, 0), bld16(rW, at + 64, 0));
+      sc[k] = sw[kc];
+    }
+  };
+  v4f acc;
+  auto work = [&](const Piece &p, const v8i (&wk)[kFewU], const float (&bk)[kFewU]) __attribute__((always_inline)) {
+    if (p.kb == KB * p.part / parts) acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    const int16_t *const list = lists + p.list * kFewTokens + p.f;
+    const int n = p.count - p.f < 16 ? p.count - p.f : 16;
+    for (int g = q; g < n * kFewU; g += 4) {
+      const int row = g / kFewU, k = g % kFewU, kb = p.kb + k;
+      if (kb >= p.hi) continue;
+      float v[8];
+      load8<LO_F32>(a.act, static_cast<int64_t>(list[row]) * I + kb * kGroup + r * 8, v);
+      codes_to_lds(v, r, row, codes + k * R * kGroup, scales + k * 16);
+    }
+    lds_order();
+    const int row = r < n ? r : 0; // (columns from n on are not kept)
+#pragma unroll
+    for (int k = 0; k < kFewU; ++k) {
+      if (p.kb + k >= p.hi) break;
+      const v4f d = mfma_e4m3_exact(wk[k], codes_from_lds(codes + k * R * kGroup, row, q));
+      const float s = scales[k * 16 + row] * bk[k];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s, acc[i]);
+    }
+    if (p.kb + kFewU >= p.hi && r < n) *reinterpret_cast<v4f *>(ys + (p.part * S + list[r]) * 16 + 4 * q) = acc;
+    lds_order();
+  };
+  Piece p = begin(wave, 0);
+  load(p, w[0], b[0]);
+  find(p);
+  while (p.it < items) { // two at a time, so that the buffers' names stand
+    Piece p1 = next(p);
+    load(p1, w[1], b[1]);
+    find(p1);
+    work(p, w[0], b[0]);
+    if (p1.it >= items) break;
+    p = next(p1);
+    load(p, w[0], b[0]);
+    find(p);
+    work(p1, w[1], b[1]);
   }
   __syncthreads();
-  const int M = a.S / a.top_k;
-  for (int o = tid; o < M * 16; o += kFewWaves * 64) {
+  for (int o = tid; o < M * 16; o += blockDim.x) {
     const int t = o >> 4, c = o & 15, s0 = t * a.top_k;
     float v = 0.0f;
     for (int j = 0; j < a.top_k; ++j) {
-      const int e = key[s0 + j];
-      if (e < 0) continue;
-      int from = 0;
-      while (key[s0 + from] != e) ++from; // the slot that holds the token's result of this expert
+      const int s = from[s0 + j];
+      if (s < 0) continue;
       float y = 0.0f;
-      for (int p = 0; p < a.parts; ++p) y += ys[(p * a.S + s0 + from) * 16 + c];
-      v = __builtin_fmaf(a.topk_w[s0 + j], y, v);
+      for (int k = 0; k < parts; ++k) y += ys[(k * S + s) * 16 + c];
+      v = __builtin_fmaf(weight[s0 + j], y, v);
     }
     v *= a.factor;
     const int64_t at = static_cast<int64_t>(t) * a.H + n0 + c;
-    if (a.shared) v += to_f32<DT>(static_cast<const uint16_t *>(a.shared)[at]);
+    if (a.shared) v += o == tid ? shared : to_f32<DT>(static_cast<const uint16_t *>(a.shared)[at]);
     static_cast<uint16_t *>(a.out)[at] = from_f32<DT>(v);
   }
 }
 
-static int64_t few_units(int64_t S, int64_t E) { return S < E ? S : E; }
-
-template <int DT> static int launch_experts_fp8(const Fp8ExpertsArgs &a, int activation, hipStream_t stream) {
-  const dim3 up(static_cast<unsigned>(a.I / 16), static_cast<unsigned>(a.units)), down(static_cast<unsigned>(a.H / 16));
-  if (activation == LO_ACT_GELU) hipLaunchKernelGGL((experts_fp8_up_kernel<DT, LO_ACT_GELU>), up, dim3(kFewWaves * 64), 0, stream, a);
-  else hipLaunchKernelGGL((experts_fp8_up_kernel<DT, LO_ACT_SILU>), up, dim3(kFewWaves * 64), 0, stream, a);
-  const int rc = check_launch("fused_experts_fp8");
-  if (rc) return rc;
-  const auto kernel = experts_fp8_down_kernel<DT>;
+template <int DT, int ACT, bool SMALL> static int launch_up(const Fp8ExpertsArgs &a, hipStream_t stream) {
+  // waves that have kFewU K blocks each, in as few rounds as eight of them need
+  const int KB = a.H / kGroup, rounds = (KB + 8 * kFewU - 1) / (8 * kFewU), waves = (KB + rounds * kFewU - 1) / (rounds * kFewU);
+  const int lds = waves * (few_wave_lds(a.rows) + kFewRed) + (SMALL ? 0 : a.S * 2);
+  const auto kernel = experts_fp8_up_kernel<DT, ACT, SMALL>;
   static unsigned long long done = 0;
-  const int rc2 = reserve_lds_once(reinterpret_cast<const void *>(kernel), kFewSlots * 64, &done);
-  if (rc2) return rc2;
-  hipLaunchKernelGGL(kernel, down, dim3(kFewWaves * 64), a.parts * a.S * 64, stream, a);
+  const int rc = reserve_lds_once(reinterpret_cast<const void *>(kernel), 8 * (few_wave_lds(16) + kFewRed) + kFewSlots * 2, &done);
+  if (rc) return rc;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.I / 16), static_cast<unsigned>(a.units)), dim3(waves * 64), lds, stream, a);
   return check_launch("fused_experts_fp8");
+}
+template <int DT, bool SMALL> static int launch_down(const Fp8ExpertsArgs &a, hipStream_t stream) {
+  constexpr int kLds = 160 * 1024 - 512; // (static variables beside it)
+  const int rest = a.parts * a.S * 64 + a.S * 12;
+  int waves = kFewMaxWaves;
+  while (waves * few_wave_lds(a.rows) + rest > kLds) waves /= 2;
+  static_assert(8 * few_wave_lds(16) + kFewSlots * 64 + kFewSlots * 12 <= kLds, "eight waves always fit");
+  const auto kernel = experts_fp8_down_kernel<DT, SMALL>;
+  static unsigned long long done = 0;
+  const int rc = reserve_lds_once(reinterpret_cast<const void *>(kernel), kLds, &done);
+  if (rc) return rc;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.H / 16)), dim3(waves * 64), waves * few_wave_lds(a.rows) + rest, stream, a);
+  return check_launch("fused_experts_fp8");
+}
+template <int DT, bool SMALL> static int launch_experts_fp8(const Fp8ExpertsArgs &a, int activation, hipStream_t stream) {
+  const int rc = activation == LO_ACT_GELU ? launch_up<DT, LO_ACT_GELU, SMALL>(a, stream) : launch_up<DT, LO_ACT_SILU, SMALL>(a, stream);
+  return rc ? rc : launch_down<DT, SMALL>(a, stream);
 }
 
 } // namespace lo
@@ -251,7 +383,7 @@ template <int DT> static int launch_experts_fp8(const Fp8ExpertsArgs &a, int act
 extern "C" int64_t lo_fused_experts_fp8_workspace_bytes(int64_t M, int32_t top_k, int64_t I, int32_t E) {
   using namespace lo;
   if (M < 0 || top_k < 1 || I < kGroup || E < 1) return LO_EINVAL;
-  return M * top_k * I * 4 + few_units(M * top_k, E) * (kFewTokens + 1) * 4;
+  return M * top_k * I * 4;
 }
 
 extern "C" int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t H, int64_t I, int32_t E, int32_t num_experts,
@@ -266,7 +398,7 @@ extern "C" int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t
   LO_REQUIRE(M >= 0 && H >= kGroup && H % kGroup == 0 && I >= kGroup && I % kGroup == 0, LO_EINVAL,
              "fused_experts_fp8: hidden (%lld) and intermediate (%lld) sizes must be multiples of 128", (long long)H, (long long)I);
   LO_REQUIRE(H <= (1 << 20) && I <= (1 << 20), LO_ENOTSUP, "fused_experts_fp8: hidden and intermediate sizes are at most 2^20");
-  LO_REQUIRE(E >= 1 && E <= 2048 && num_experts >= E && top_k >= 1, LO_EINVAL, "fused_experts_fp8: bad expert counts");
+  LO_REQUIRE(E >= 1 && E <= kFewExperts && num_experts >= E && top_k >= 1, LO_EINVAL, "fused_experts_fp8: bad expert counts");
   LO_REQUIRE(num_experts == E || expert_map, LO_EINVAL, "fused_experts_fp8: %d experts routed over, %d here, and no expert_map", num_experts, E);
   LO_REQUIRE(M <= kFewTokens && M * top_k <= kFewSlots, LO_ENOTSUP,
              "fused_experts_fp8: %lld tokens of %d slots (at most %d tokens and %d slots)", (long long)M, top_k, kFewTokens, kFewSlots);
@@ -282,18 +414,20 @@ extern "C" int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t
   a.x = x; a.ids = topk_ids; a.shared = shared_output;
   a.w1 = static_cast<const int8_t *>(w1); a.w2 = static_cast<const int8_t *>(w2);
   a.w1s = w1s; a.w2s = w2s; a.topk_w = topk_w; a.map = expert_map; a.out = out;
+  a.act = static_cast<float *>(workspace);
   a.S = static_cast<int32_t>(M * top_k); a.H = static_cast<int32_t>(H); a.I = static_cast<int32_t>(I);
   a.E = E; a.Eg = num_experts; a.top_k = top_k; a.factor = routed_scaling_factor;
   a.ids64 = ids_dtype == LO_I64;
-  a.units = static_cast<int32_t>(few_units(a.S, E));
   a.by_slot = a.S < E;
-  a.act = static_cast<float *>(workspace);
-  a.counts = reinterpret_cast<int32_t *>(a.act + static_cast<int64_t>(a.S) * I);
-  a.lists = a.counts + a.units;
-  // parts of K: enough for every wave where few experts are hit, and their results fit LDS
+  a.units = a.by_slot ? a.S : E;
+  a.rows = static_cast<int32_t>(M < 16 ? M : 16);
+  // parts of the second product's K: what a wave has in flight at once, while eight of them and their results fit LDS
   const int KB = a.I / kGroup;
-  a.parts = 8;
-  while (a.parts > 1 && (a.parts > KB || a.parts * a.S > kFewSlots)) a.parts /= 2;
-  return dtype == LO_F16 ? launch_experts_fp8<LO_F16>(a, activation, static_cast<hipStream_t>(stream))
-                         : launch_experts_fp8<LO_BF16>(a, activation, static_cast<hipStream_t>(stream));
+  a.parts = (KB + kFewU - 1) / kFewU;
+  a.parts = a.parts < 8 ? a.parts : 8;
+  while (a.parts * a.S > kFewSlots) --a.parts;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a.S <= 64)
+    return dtype == LO_F16 ? launch_experts_fp8<LO_F16, true>(a, activation, s) : launch_experts_fp8<LO_BF16, true>(a, activation, s);
+  return dtype == LO_F16 ? launch_experts_fp8<LO_F16, false>(a, activation, s) : launch_experts_fp8<LO_BF16, false>(a, activation, s);
 }

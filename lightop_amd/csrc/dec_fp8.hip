@@ -6,8 +6,9 @@
 //          on the way it would move codes of the second quantisation.
 //   down   one workgroup per 16 columns of the output.  Its waves share (expert hit, part of K) and leave each slot's 16 values in LDS;
 //          then every token's slots are added up in their order.  No atomics on results: the order of every sum is fixed.
-// Both find the experts hit from the ids by themselves.  Both
-// products are the exact ones (fp8.h): the matrix cores have time, and an error of 1e-5 moves codes of the second quantisation.
+// Both find the experts hit from the ids by themselves.  The
+// first product is the exact one (fp8.h): the matrix cores have time, and an error of 1e-5 moves codes of the second quantisation; behind the
+// second one stands a rounding to 16 bits.
 // Ids that no expert of this rank answers to (out of range, or -1 in the map) add nothing.  An id that a token has twice is computed once
 // and counted with both weights.
 #include "gemm.h"
@@ -19,7 +20,9 @@ constexpr int kFewTokens = 64;   // of a call
 constexpr int kFewSlots = 1024;
 constexpr int kFewExperts = 2048;
 constexpr int kFewU = 4;         // K blocks of a wave in flight
-constexpr int kFewMaxWaves = 16;
+constexpr int kFewMaxWaves = 16; // (down)
+constexpr int kFewGroup = 8;     // tokens of a workgroup (down), at the most
+constexpr int kFewParts = 4;     // of the second product's K, at the most
 
 struct Fp8ExpertsArgs {
   const void *x, *ids, *shared;
@@ -29,7 +32,8 @@ struct Fp8ExpertsArgs {
   void *out;
   float *act;       // [slots, I]
   int32_t S, H, I, E, Eg, top_k, units, parts;
-  int32_t rows;     // of a wave's codes: min(tokens, 16)
+  int32_t rows;     // of a wave's codes: tokens that an expert may have at a time
+  int32_t group;    // tokens of a workgroup (down)
   float factor;
   bool ids64, by_slot;
 };
@@ -46,14 +50,15 @@ __device__ __forceinline__ int local_expert(const Fp8ExpertsArgs &a, int s) {
 template <bool SMALL> struct Route {
   const Fp8ExpertsArgs &a;
   int16_t *keys; // LDS, [slots]: expert, -1 for none here
-  int lane;
+  int lane, S;
   int key = -1;  // SMALL: expert of slot `lane`
 
-  __device__ __forceinline__ Route(const Fp8ExpertsArgs &args, int16_t *k, int ln) : a(args), keys(k), lane(ln) {
+  // S slots from slot0 on, which begins a token
+  __device__ __forceinline__ Route(const Fp8ExpertsArgs &args, int16_t *k, int ln, int slot0, int slots) : a(args), keys(k), lane(ln), S(slots) {
     if constexpr (SMALL) {
-      if (lane < a.S) key = local_expert(a, lane);
+      if (lane < S) key = local_expert(a, slot0 + lane);
     } else {
-      for (int s = threadIdx.x; s < a.S; s += blockDim.x) keys[s] = static_cast<int16_t>(local_expert(a, s));
+      for (int s = threadIdx.x; s < S; s += blockDim.x) keys[s] = static_cast<int16_t>(local_expert(a, slot0 + s));
       __syncthreads();
     }
   }
@@ -63,9 +68,9 @@ template <bool SMALL> struct Route {
   // The expert's slots, one a token, into the wave's list, and how many; none if `lead` is not negative and not the first of them.
   __device__ __forceinline__ int slots(int e, int lead, int16_t *list) const {
     int count = 0;
-    for (int base = 0; base < (SMALL ? 1 : a.S); base += 64) {
+    for (int base = 0; base < (SMALL ? 1 : S); base += 64) {
       const int s = base + lane;
-      bool hit = SMALL ? key == e : s < a.S && keys[s] == e;
+      bool hit = SMALL ? key == e : s < S && keys[s] == e;
       const uint64_t all = __builtin_amdgcn_ballot_w64(hit);
       if (!all) continue;
       if (lead >= 0 && count == 0 && base + __builtin_ctzll(all) != lead) return 0;
@@ -103,13 +108,17 @@ __device__ __forceinline__ v8i codes_from_lds(const int8_t *rows, int r, int q) 
               *reinterpret_cast<const v4i *>(rows + r * kGroup + (((q + 4) ^ (r & 7)) * 16)));
 }
 
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
 // LDS of a wave: codes of kFewU K blocks, their scales, two lists of slots
 __host__ __device__ constexpr int few_wave_lds(int rows) { return kFewU * (rows * kGroup + 64) + 2 * kFewTokens * 2; }
 constexpr int kFewRed = 2048; // gate and up sums of a wave (up)
 
 // A unit is a slot where there are fewer slots than experts (the first of its expert's; the others' workgroups end), else an expert.
 template <int DT, int ACT, bool SMALL>
-__global__ __launch_bounds__(512) void experts_fp8_up_kernel(const Fp8ExpertsArgs a) {
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void experts_fp8_up_kernel(const Fp8ExpertsArgs a) {
   extern __shared__ __attribute__((aligned(16))) int8_t smem[]; // [wave] codes, scales, list; [wave] sums; slots' experts
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -118,7 +127,7 @@ __global__ __launch_bounds__(512) void experts_fp8_up_kernel(const Fp8ExpertsArg
   float *const scales = reinterpret_cast<float *>(codes + kFewU * R * kGroup);
   int16_t *const list = reinterpret_cast<int16_t *>(scales + kFewU * 16);
   float *const red = reinterpret_cast<float *>(smem + waves * per); // [wave][gate, up][token][column]
-  const Route<SMALL> route(a, reinterpret_cast<int16_t *>(smem + waves * (per + kFewRed)), lane);
+  const Route<SMALL> route(a, reinterpret_cast<int16_t *>(smem + waves * (per + kFewRed)), lane, 0, a.S);
   const int e = a.by_slot ? route.slot_expert(u) : u;
   if (e < 0) return;
   const int count = route.slots(e, a.by_slot ? u : -1, list);
@@ -133,22 +142,25 @@ __global__ __launch_bounds__(512) void experts_fp8_up_kernel(const Fp8ExpertsArg
     const int n = count - f < 16 ? count - f : 16;
     v4f acc[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
     for (int kb0 = wave; kb0 < KB; kb0 += waves * kFewU) {
+      // the first rows' values in front of the weights: what is asked for first comes first, and they are quantised meanwhile
+      float v[8];
+      auto rows_at = [&](int g) __attribute__((always_inline)) { // of group g: 16 lanes, eight values each
+        const int kb = kb0 + g % kFewU * waves;
+        load8<DT>(a.x, static_cast<int64_t>(list[f + g / kFewU] / a.top_k) * H + (kb < KB ? kb : kb0) * kGroup + r * 8, v);
+      };
+      if (q < n * kFewU) rows_at(q);
       v8i wg[kFewU], wu[kFewU];
-      float bg[kFewU], bu[kFewU];
 #pragma unroll
       for (int k = 0; k < kFewU; ++k) {
         const int kb = kb0 + k * waves, kc = kb < KB ? kb : kb0, at = r * H + q * 16 + kc * kGroup;
         wg[k] = join(bld16(rG, at, 0), bld16(rG, at + 64, 0));
         wu[k] = join(bld16(rU, at, 0), bld16(rU, at + 64, 0));
-        bg[k] = sg[kc];
-        bu[k] = su[kc];
       }
-      for (int g = q; g < n * kFewU; g += 4) { // 16 lanes a group
-        const int row = g / kFewU, k = g % kFewU, kb = kb0 + k * waves;
-        if (kb >= KB) continue;
-        float v[8];
-        load8<DT>(a.x, static_cast<int64_t>(list[f + row] / a.top_k) * H + kb * kGroup + r * 8, v);
-        codes_to_lds(v, r, row, codes + k * R * kGroup, scales + k * 16);
+      const int mine = kb0 + lane % kFewU * waves; // scales of the weights, a K block a lane
+      const float bg = sg[mine < KB ? mine : kb0], bu = su[mine < KB ? mine : kb0];
+      for (int g = q; g < n * kFewU; g += 4) {
+        if (g >= 4) rows_at(g);
+        codes_to_lds(v, r, g / kFewU, codes + g % kFewU * R * kGroup, scales + g % kFewU * 16);
       }
       lds_order();
 #pragma unroll
@@ -156,7 +168,7 @@ __global__ __launch_bounds__(512) void experts_fp8_up_kernel(const Fp8ExpertsArg
         if (kb0 + k * waves >= KB) break;
         const int row = r < n ? r : 0; // (columns from n on are not kept)
         const v8i x = codes_from_lds(codes + k * R * kGroup, row, q);
-        const float s = scales[k * 16 + row], s0 = s * bg[k], s1 = s * bu[k];
+        const float s = scales[k * 16 + row], s0 = s * lane_value(bg, k), s1 = s * lane_value(bu, k);
         const v4f d0 = mfma_e4m3_exact(wg[k], x), d1 = mfma_e4m3_exact(wu[k], x);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -178,174 +190,136 @@ __global__ __launch_bounds__(512) void experts_fp8_up_kernel(const Fp8ExpertsArg
   }
 }
 
-template <int DT, bool SMALL>
+// Tokens in groups of up to 64 slots, one to blockIdx.y: a wave holds the group's routing in its lanes, and an expert has 16 tokens at the most.
+// (An expert that several groups hit is read again, out of L2: neighbouring blockIdx.x are what one XCD gets of every group.)
+template <int DT>
 __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8ExpertsArgs a) {
-  // [wave] codes, scales, lists; [part][slot][column] results; [slot] weight; [slot] the token's first one with this expert, -1: none here;
-  // [slot] expert; the experts hit
+  // [wave] codes, scales, lists; [part][slot][column] results; [slot] weight; [slot] the token's first one with this expert, -1: none here
   extern __shared__ __attribute__((aligned(16))) int8_t smem[];
-  __shared__ uint32_t present[kFewExperts / 32];
-  __shared__ int number;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n0 = blockIdx.x * 16, I = a.I, KB = I / kGroup, R = a.rows, per = few_wave_lds(R), parts = a.parts, S = a.S, M = S / a.top_k;
+  const int n0 = blockIdx.x * 16, I = a.I, KB = I / kGroup, R = a.rows, per = few_wave_lds(R), parts = a.parts;
+  const int first = blockIdx.y * a.group, M = a.S / a.top_k - first < a.group ? a.S / a.top_k - first : a.group;
+  const int S = M * a.top_k, slot0 = first * a.top_k; // of the group
   int8_t *const codes = smem + wave * per;
   float *const scales = reinterpret_cast<float *>(codes + kFewU * R * kGroup);
   int16_t *const lists = reinterpret_cast<int16_t *>(scales + kFewU * 16);
-  float *const ys = reinterpret_cast<float *>(smem + waves * per), *const weight = ys + parts * S * 16;
-  int16_t *const from = reinterpret_cast<int16_t *>(weight + S), *const keys = from + S, *const hit = keys + S;
-  for (int s = tid; s < S; s += blockDim.x) weight[s] = a.topk_w[s];
+  float *const ys = reinterpret_cast<float *>(smem + waves * per), *const weight = ys + parts * 64 * 16;
+  int16_t *const from = reinterpret_cast<int16_t *>(weight + 64);
+  const Route<true> route(a, nullptr, lane, slot0, S);
   // (asked for here, not behind the last product)
+  if (tid < S) weight[tid] = a.topk_w[slot0 + tid];
   float shared = 0.0f;
-  if (a.shared && tid < M * 16) shared = to_f32<DT>(static_cast<const uint16_t *>(a.shared)[static_cast<int64_t>(tid >> 4) * a.H + n0 + (tid & 15)]);
-  if constexpr (!SMALL)
-    for (int i = tid; i < kFewExperts / 32; i += blockDim.x) present[i] = 0;
-  const Route<SMALL> route(a, keys, lane);
-  uint64_t leaders = 0; // SMALL: first slots of the experts hit
-  int experts = 0;
-  if constexpr (SMALL) {
-    uint64_t left = __builtin_amdgcn_ballot_w64(route.key >= 0);
-    int mine = -1;
-    while (left) { // an expert at a time
-      const int s = __builtin_ctzll(left);
-      const uint64_t same = __builtin_amdgcn_ballot_w64(route.key == __builtin_amdgcn_readlane(route.key, s));
-      if (same >> lane & 1) {
-        const uint64_t before = same & route.earlier_of_token();
-        mine = before ? __builtin_ctzll(before) : lane;
-      }
-      left &= ~same;
-      leaders |= 1ull << s;
-      ++experts;
+  if (a.shared && tid < M * 16)
+    shared = to_f32<DT>(static_cast<const uint16_t *>(a.shared)[static_cast<int64_t>(first + (tid >> 4)) * a.H + n0 + (tid & 15)]);
+  uint64_t leaders = 0; // first slots of the experts hit
+  int experts = 0, mine = -1;
+  for (uint64_t left = __builtin_amdgcn_ballot_w64(route.key >= 0); left; ++experts) { // an expert at a time
+    const int s = __builtin_ctzll(left);
+    const uint64_t same = __builtin_amdgcn_ballot_w64(route.key == __builtin_amdgcn_readlane(route.key, s));
+    if (same >> lane & 1) {
+      const uint64_t before = same & route.earlier_of_token();
+      mine = before ? __builtin_ctzll(before) : lane;
     }
-    if (wave == 0 && lane < S) from[lane] = static_cast<int16_t>(mine);
-  } else {
-    for (int s = tid; s < S; s += blockDim.x) {
-      const int e = keys[s], s0 = s / a.top_k * a.top_k;
-      int j = s0;
-      while (j < s && keys[j] != e) ++j;
-      from[s] = static_cast<int16_t>(e < 0 ? -1 : j);
-      if (e >= 0) atomicOr(&present[e >> 5], 1u << (e & 31));
-    }
-    __syncthreads();
-    if (wave == 0) {
-      static_assert(kFewExperts / 32 == 64, "a word a lane");
-      uint32_t left = present[lane];
-      int before = __popc(left), all = before; // of the lanes up to this one
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(all, d);
-        if (lane >= d) all += o;
-      }
-      before = all - before;
-      for (; left; left &= left - 1) hit[before++] = static_cast<int16_t>(lane * 32 + __builtin_ctz(left));
-      if (lane == 63) number = all;
-    }
-    __syncthreads();
-    experts = number;
+    left &= ~same;
+    leaders |= 1ull << s;
   }
+  if (wave == 0) from[lane] = static_cast<int16_t>(mine);
 
-  // The wave's work: (expert, part of K, 16 of its tokens), every `waves`-th (expert, part); up to kFewU K blocks at a time, the next ones'
-  // weights asked for before these are used.
+  // The wave's work: (expert, part of K), of every `waves`-th; up to kFewU K blocks at a time, the next ones' weights and first activations
+  // asked for before these are used.
   const int items = experts * parts;
   struct Piece {
-    int it, e, part, f, count, kb, hi, list;
+    int it, e, part, count, kb, hi, list;
   };
   auto begin = [&](int it, int list) __attribute__((always_inline)) {
-    Piece p{it, 0, 0, 0, 0, 0, 0, list};
+    Piece p{it, 0, 0, 0, 0, 0, list};
     if (it >= items) return p;
     int at = it / parts;
     p.part = it - at * parts;
-    if constexpr (SMALL) {
-      uint64_t left = leaders;
-      for (; at > 0; --at) left &= left - 1;
-      p.e = route.slot_expert(__builtin_ctzll(left));
-    } else {
-      p.e = __builtin_amdgcn_readfirstlane(hit[at]);
-    }
+    uint64_t left = leaders;
+    for (; at > 0; --at) left &= left - 1;
+    p.e = route.slot_expert(__builtin_ctzll(left));
     p.kb = KB * p.part / parts;
     p.hi = KB * (p.part + 1) / parts;
+    p.count = route.slots(p.e, -1, lists + list * kFewTokens);
     return p;
   };
-  auto find = [&](Piece &p) __attribute__((always_inline)) { // behind the loads of its weights
-    if (p.it < items && p.f == 0 && p.kb == KB * p.part / parts) p.count = route.slots(p.e, -1, lists + p.list * kFewTokens);
-  };
   auto next = [&](Piece p) __attribute__((always_inline)) {
-    if (p.kb + kFewU < p.hi) {
-      p.kb += kFewU;
-    } else if (p.f + 16 < p.count) {
-      p.f += 16;
-      p.kb = KB * p.part / parts;
-    } else {
-      p = begin(p.it + waves, p.list ^ 1);
-    }
+    if (p.kb + kFewU >= p.hi) return begin(p.it + waves, p.list ^ 1);
+    p.kb += kFewU;
     return p;
   };
   v8i w[2][kFewU];
-  float b[2][kFewU];
-  auto load = [&](const Piece &p, v8i (&to)[kFewU], float (&sc)[kFewU]) __attribute__((always_inline)) {
+  float b[2], v[8]; // scales of the weights, a K block a lane; activations
+  auto acts_at = [&](const Piece &p, int g) __attribute__((always_inline)) { // of group g: 16 lanes, eight values each
+    const int kb = p.kb + g % kFewU;
+    load8<LO_F32>(a.act, static_cast<int64_t>(slot0 + lists[p.list * kFewTokens + g / kFewU]) * I + (kb < p.hi ? kb : p.hi - 1) * kGroup + r * 8, v);
+  };
+  auto load = [&](const Piece &p, int at) __attribute__((always_inline)) {
     if (p.it >= items) return;
+    if (q < p.count * kFewU) acts_at(p, q);
     const brsrc rW = make_rsrc(a.w2 + (static_cast<int64_t>(p.e) * a.H + n0) * I, static_cast<uint32_t>(16 * I));
     const float *const sw = a.w2s + (static_cast<int64_t>(p.e) * (a.H / kGroup) + n0 / kGroup) * KB;
 #pragma unroll
     for (int k = 0; k < kFewU; ++k) {
-      const int kc = p.kb + k < p.hi ? p.kb + k : p.hi - 1, at = r * I + q * 16 + kc * kGroup;
-      to[k] = join(bld16(rW, at, 0), bld16(rW, at + 64, 0));
-      sc[k] = sw[kc];
+      const int kc = p.kb + k < p.hi ? p.kb + k : p.hi - 1, off = r * I + q * 16 + kc * kGroup;
+      w[at][k] = join(bld16(rW, off, 0), bld16(rW, off + 64, 0));
     }
+    const int mine = p.kb + lane % kFewU;
+    b[at] = sw[mine < p.hi ? mine : p.hi - 1];
   };
-  v4f acc;
-  auto work = [&](const Piece &p, const v8i (&wk)[kFewU], const float (&bk)[kFewU]) __attribute__((always_inline)) {
-    if (p.kb == KB * p.part / parts) acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    const int16_t *const list = lists + p.list * kFewTokens + p.f;
-    const int n = p.count - p.f < 16 ? p.count - p.f : 16;
-    for (int g = q; g < n * kFewU; g += 4) {
-      const int row = g / kFewU, k = g % kFewU, kb = p.kb + k;
-      if (kb >= p.hi) continue;
-      float v[8];
-      load8<LO_F32>(a.act, static_cast<int64_t>(list[row]) * I + kb * kGroup + r * 8, v);
-      codes_to_lds(v, r, row, codes + k * R * kGroup, scales + k * 16);
+  v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto quantise = [&](const Piece &p) __attribute__((always_inline)) {
+    for (int g = q; g < p.count * kFewU; g += 4) {
+      if (g >= 4) acts_at(p, g);
+      codes_to_lds(v, r, g / kFewU, codes + g % kFewU * R * kGroup, scales + g % kFewU * 16);
     }
     lds_order();
-    const int row = r < n ? r : 0; // (columns from n on are not kept)
+  };
+  auto work = [&](const Piece &p, int at) __attribute__((always_inline)) {
+    if (p.kb == KB * p.part / parts) acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    const int row = r < p.count ? r : 0; // (columns past the tokens are not kept)
 #pragma unroll
     for (int k = 0; k < kFewU; ++k) {
       if (p.kb + k >= p.hi) break;
-      const v4f d = mfma_e4m3_exact(wk[k], codes_from_lds(codes + k * R * kGroup, row, q));
-      const float s = scales[k * 16 + row] * bk[k];
+      const v4f d = mfma_e4m3(w[at][k], codes_from_lds(codes + k * R * kGroup, row, q));
+      const float s = scales[k * 16 + row] * lane_value(b[at], k);
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s, acc[i]);
     }
-    if (p.kb + kFewU >= p.hi && r < n) *reinterpret_cast<v4f *>(ys + (p.part * S + list[r]) * 16 + 4 * q) = acc;
+    if (p.kb + kFewU >= p.hi && r < p.count)
+      *reinterpret_cast<v4f *>(ys + (p.part * 64 + lists[p.list * kFewTokens + r]) * 16 + 4 * q) = acc;
     lds_order();
   };
   Piece p = begin(wave, 0);
-  load(p, w[0], b[0]);
-  find(p);
+  load(p, 0);
   while (p.it < items) { // two at a time, so that the buffers' names stand
-    Piece p1 = next(p);
-    load(p1, w[1], b[1]);
-    find(p1);
-    work(p, w[0], b[0]);
+    quantise(p);
+    const Piece p1 = next(p);
+    load(p1, 1);
+    work(p, 0);
     if (p1.it >= items) break;
+    quantise(p1);
     p = next(p1);
-    load(p, w[0], b[0]);
-    find(p);
-    work(p1, w[1], b[1]);
+    load(p, 0);
+    work(p1, 1);
   }
   __syncthreads();
   for (int o = tid; o < M * 16; o += blockDim.x) {
     const int t = o >> 4, c = o & 15, s0 = t * a.top_k;
-    float v = 0.0f;
+    float sum = 0.0f;
     for (int j = 0; j < a.top_k; ++j) {
       const int s = from[s0 + j];
       if (s < 0) continue;
       float y = 0.0f;
-      for (int k = 0; k < parts; ++k) y += ys[(k * S + s) * 16 + c];
-      v = __builtin_fmaf(weight[s0 + j], y, v);
+      for (int k = 0; k < parts; ++k) y += ys[(k * 64 + s) * 16 + c];
+      sum = __builtin_fmaf(weight[s0 + j], y, sum);
     }
-    v *= a.factor;
-    const int64_t at = static_cast<int64_t>(t) * a.H + n0 + c;
-    if (a.shared) v += o == tid ? shared : to_f32<DT>(static_cast<const uint16_t *>(a.shared)[at]);
-    static_cast<uint16_t *>(a.out)[at] = from_f32<DT>(v);
+    sum *= a.factor;
+    const int64_t at = static_cast<int64_t>(first + t) * a.H + n0 + c;
+    if (a.shared) sum += o == tid ? shared : to_f32<DT>(static_cast<const uint16_t *>(a.shared)[at]);
+    static_cast<uint16_t *>(a.out)[at] = from_f32<DT>(sum);
   }
 }
 
@@ -360,22 +334,31 @@ template <int DT, int ACT, bool SMALL> static int launch_up(const Fp8ExpertsArgs
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.I / 16), static_cast<unsigned>(a.units)), dim3(waves * 64), lds, stream, a);
   return check_launch("fused_experts_fp8");
 }
-template <int DT, bool SMALL> static int launch_down(const Fp8ExpertsArgs &a, hipStream_t stream) {
-  constexpr int kLds = 160 * 1024 - 512; // (static variables beside it)
-  const int rest = a.parts * a.S * 64 + a.S * 12;
-  int waves = kFewMaxWaves;
-  while (waves * few_wave_lds(a.rows) + rest > kLds) waves /= 2;
-  static_assert(8 * few_wave_lds(16) + kFewSlots * 64 + kFewSlots * 12 <= kLds, "eight waves always fit");
-  const auto kernel = experts_fp8_down_kernel<DT, SMALL>;
+template <int DT> static int launch_down(const Fp8ExpertsArgs &a, hipStream_t stream) {
+  const int waves = kFewMaxWaves, lds = waves * few_wave_lds(a.rows) + a.parts * 64 * 64 + 64 * 6;
+  constexpr int most = kFewMaxWaves * few_wave_lds(kFewGroup) + kFewParts * 64 * 64 + 64 * 6;
+  static_assert(most <= 160 * 1024, "LDS");
+  const auto kernel = experts_fp8_down_kernel<DT>;
   static unsigned long long done = 0;
-  const int rc = reserve_lds_once(reinterpret_cast<const void *>(kernel), kLds, &done);
+  const int rc = reserve_lds_once(reinterpret_cast<const void *>(kernel), most, &done);
   if (rc) return rc;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.H / 16)), dim3(waves * 64), waves * few_wave_lds(a.rows) + rest, stream, a);
+  const int M = a.S / a.top_k;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.H / 16), static_cast<unsigned>((M + a.group - 1) / a.group)), dim3(waves * 64), lds, stream,
+                     a);
   return check_launch("fused_experts_fp8");
 }
-template <int DT, bool SMALL> static int launch_experts_fp8(const Fp8ExpertsArgs &a, int activation, hipStream_t stream) {
-  const int rc = activation == LO_ACT_GELU ? launch_up<DT, LO_ACT_GELU, SMALL>(a, stream) : launch_up<DT, LO_ACT_SILU, SMALL>(a, stream);
-  return rc ? rc : launch_down<DT, SMALL>(a, stream);
+template <int DT> static int launch_experts_fp8(Fp8ExpertsArgs a, int activation, hipStream_t stream) {
+  const int M = a.S / a.top_k, KB = a.I / kGroup;
+  a.rows = M < 16 ? M : 16;
+  const bool gelu = activation == LO_ACT_GELU;
+  const int rc = a.S <= 64 ? (gelu ? launch_up<DT, LO_ACT_GELU, true>(a, stream) : launch_up<DT, LO_ACT_SILU, true>(a, stream))
+                           : (gelu ? launch_up<DT, LO_ACT_GELU, false>(a, stream) : launch_up<DT, LO_ACT_SILU, false>(a, stream));
+  if (rc) return rc;
+  a.group = 64 / a.top_k < kFewGroup ? 64 / a.top_k : kFewGroup;
+  a.rows = M < a.group ? M : a.group;
+  // parts of the second product's K: what a wave has in flight at once
+  a.parts = (KB + kFewU - 1) / kFewU < kFewParts ? (KB + kFewU - 1) / kFewU : kFewParts;
+  return launch_down<DT>(a, stream);
 }
 
 } // namespace lo
@@ -399,6 +382,7 @@ extern "C" int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t
              "fused_experts_fp8: hidden (%lld) and intermediate (%lld) sizes must be multiples of 128", (long long)H, (long long)I);
   LO_REQUIRE(H <= (1 << 20) && I <= (1 << 20), LO_ENOTSUP, "fused_experts_fp8: hidden and intermediate sizes are at most 2^20");
   LO_REQUIRE(E >= 1 && E <= kFewExperts && num_experts >= E && top_k >= 1, LO_EINVAL, "fused_experts_fp8: bad expert counts");
+  LO_REQUIRE(top_k <= 64, LO_ENOTSUP, "fused_experts_fp8: top_k (%d) is at most 64", top_k);
   LO_REQUIRE(num_experts == E || expert_map, LO_EINVAL, "fused_experts_fp8: %d experts routed over, %d here, and no expert_map", num_experts, E);
   LO_REQUIRE(M <= kFewTokens && M * top_k <= kFewSlots, LO_ENOTSUP,
              "fused_experts_fp8: %lld tokens of %d slots (at most %d tokens and %d slots)", (long long)M, top_k, kFewTokens, kFewSlots);
@@ -420,14 +404,6 @@ extern "C" int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t
   a.ids64 = ids_dtype == LO_I64;
   a.by_slot = a.S < E;
   a.units = a.by_slot ? a.S : E;
-  a.rows = static_cast<int32_t>(M < 16 ? M : 16);
-  // parts of the second product's K: what a wave has in flight at once, while eight of them and their results fit LDS
-  const int KB = a.I / kGroup;
-  a.parts = (KB + kFewU - 1) / kFewU;
-  a.parts = a.parts < 8 ? a.parts : 8;
-  while (a.parts * a.S > kFewSlots) --a.parts;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a.S <= 64)
-    return dtype == LO_F16 ? launch_experts_fp8<LO_F16, true>(a, activation, s) : launch_experts_fp8<LO_BF16, true>(a, activation, s);
-  return dtype == LO_F16 ? launch_experts_fp8<LO_F16, false>(a, activation, s) : launch_experts_fp8<LO_BF16, false>(a, activation, s);
+  return dtype == LO_F16 ? launch_experts_fp8<LO_F16>(a, activation, s) : launch_experts_fp8<LO_BF16>(a, activation, s);
 }

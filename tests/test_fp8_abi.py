@@ -76,7 +76,7 @@ def _experts(lib, **k):
 
 
 @pytest.mark.parametrize("bad", [dict(dt=2), dict(it=2), dict(act=2), dict(M=-1), dict(H=64), dict(H=320), dict(I=64), dict(E=0), dict(Eg=3),
-                                 dict(Eg=8), dict(top_k=0), dict(M=65), dict(M=64, top_k=17), dict(x=0), dict(w1=0), dict(w2=0), dict(s1=0),
+                                 dict(Eg=8), dict(top_k=0), dict(M=65), dict(M=64, top_k=17), dict(M=1, top_k=65), dict(x=0), dict(w1=0), dict(w2=0), dict(s1=0),
                                  dict(s2=0), dict(tw=0), dict(ids=0), dict(out=0), dict(ws=0), dict(n=100), dict(x=P + 8), dict(ws=P + 4),
                                  dict(w2=P + 4), dict(E=4096, Eg=4096), dict(H=1 << 21)], ids=str)
 def test_experts_refuses(lib, bad):

@@ -626,14 +626,15 @@ int lo_gemm_w8a8_fp8_block(const void *a, const float *a_scale, const void *b, c
                            lo_stream_t stream);
 
 /*
- * The experts of a few tokens (M <= 64, top_k <= 64, M * top_k <= 1024) with e4m3 weights, in two launches: e4m3 rows of x, first
+ * The experts of a few tokens (M <= 64, top_k <= 64, M * top_k <= 1024) with e4m3 weights, in two launches (four beyond
+ * 64 slots): e4m3 rows of x, first
  * product, act(gate) * up and its e4m3 codes, second product, weighted sum over a token's slots.
  *   w1 [E, 2I, H], w2 [E, H, I] e4m3 row-major; w1s [E, 2I/128, H/128], w2s [E, H/128, I/128] fp32
  *   topk_w, topk_ids [M, top_k]; ids without an expert here (out of range, or no entry in expert_map) add nothing
  *   out[t] = routed_scaling_factor * sum_j topk_w[t, j] * y (+ shared_output[t]); out may be x or shared_output
  *   workspace: lo_fused_experts_fp8_workspace_bytes, 16-byte aligned; one call's at a time
  */
-int64_t lo_fused_experts_fp8_workspace_bytes(int64_t M, int32_t top_k, int64_t I, int32_t E);
+int64_t lo_fused_experts_fp8_workspace_bytes(int64_t M, int32_t top_k, int64_t H, int64_t I);
 int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t H, int64_t I, int32_t E, int32_t num_experts,
                          int32_t top_k, const void *w1, const float *w1s, const void *w2, const float *w2s,
                          const float *topk_w, const void *topk_ids, int ids_dtype, const int32_t *expert_map,

@@ -1,4 +1,4 @@
-// The experts of a few tokens with e4m3 weights (128 x 128 blocks) in two launches:
+// The experts of a few tokens with e4m3 weights (128 x 128 blocks) in two launches, in four beyond 64 slots:
 //   h = xq w1[e]^T,  v = act(h[:I]) * h[I:],  y = vq w2[e]^T,  out[t] = factor * sum_j w[t, j] * y[t, e_j] (+ shared[t]),
 // xq and vq the e4m3 codes of rows in groups of 128 (fp8.h).  At these sizes the layer is a stream of the hit experts' weights:
 //   up     one workgroup per (expert hit, 16 columns of I).  Its waves share the K blocks of the 16 gate and 16 up rows and quantise their part
@@ -24,6 +24,10 @@ constexpr int kFewMaxWaves = 16; // (down)
 constexpr int kFewGroup = 8;     // tokens of a workgroup (down), at the most
 constexpr int kFewParts = 4;     // of the second product's K, at the most
 
+// Up to 64 slots in two launches, every workgroup quantising the rows that it needs; beyond, a launch in front of either product does it
+// once.
+static bool few_in_two(int64_t slots) { return slots <= 64; }
+
 struct Fp8ExpertsArgs {
   const void *x, *ids, *shared;
   const int8_t *w1, *w2;
@@ -31,6 +35,8 @@ struct Fp8ExpertsArgs {
   const int32_t *map;
   void *out;
   float *act;       // [slots, I]
+  const int8_t *xq, *aq; // CODES: rows of x [tokens, H] and of act [slots, I], and their scales
+  const float *xs, *as;
   int32_t S, H, I, E, Eg, top_k, units, parts;
   int32_t rows;     // of a wave's codes: tokens that an expert may have at a time
   int32_t group;    // tokens of a workgroup (down)
@@ -117,7 +123,7 @@ __host__ __device__ constexpr int few_wave_lds(int rows) { return kFewU * (rows 
 constexpr int kFewRed = 2048; // gate and up sums of a wave (up)
 
 // A unit is a slot where there are fewer slots than experts (the first of its expert's; the others' workgroups end), else an expert.
-template <int DT, int ACT, bool SMALL>
+template <int DT, int ACT, bool SMALL, bool CODES>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void experts_fp8_up_kernel(const Fp8ExpertsArgs a) {
   extern __shared__ __attribute__((aligned(16))) int8_t smem[]; // [wave] codes, scales, list; [wave] sums; slots' experts
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4, waves = blockDim.x >> 6;
@@ -142,13 +148,26 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void e
     const int n = count - f < 16 ? count - f : 16;
     v4f acc[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
     for (int kb0 = wave; kb0 < KB; kb0 += waves * kFewU) {
-      // the first rows' values in front of the weights: what is asked for first comes first, and they are quantised meanwhile
-      float v[8];
+      // the rows in front of the weights: what is asked for first comes first, and they are quantised meanwhile
+      float v[8], sx[kFewU];
+      v8i x[kFewU];
+      const int row = r < n ? r : 0; // (columns from n on are not kept)
       auto rows_at = [&](int g) __attribute__((always_inline)) { // of group g: 16 lanes, eight values each
         const int kb = kb0 + g % kFewU * waves;
         load8<DT>(a.x, static_cast<int64_t>(list[f + g / kFewU] / a.top_k) * H + (kb < KB ? kb : kb0) * kGroup + r * 8, v);
       };
-      if (q < n * kFewU) rows_at(q);
+      if constexpr (CODES) {
+        const int token = list[f + row] / a.top_k;
+#pragma unroll
+        for (int k = 0; k < kFewU; ++k) {
+          const int kb = kb0 + k * waves, kc = kb < KB ? kb : kb0;
+          const int8_t *const at = a.xq + static_cast<int64_t>(token) * H + kc * kGroup + q * 16;
+          x[k] = join(*reinterpret_cast<const v4i *>(at), *reinterpret_cast<const v4i *>(at + 64));
+          sx[k] = a.xs[token * KB + kc];
+        }
+      } else if (q < n * kFewU) {
+        rows_at(q);
+      }
       v8i wg[kFewU], wu[kFewU];
 #pragma unroll
       for (int k = 0; k < kFewU; ++k) {
@@ -158,18 +177,22 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void e
       }
       const int mine = kb0 + lane % kFewU * waves; // scales of the weights, a K block a lane
       const float bg = sg[mine < KB ? mine : kb0], bu = su[mine < KB ? mine : kb0];
-      for (int g = q; g < n * kFewU; g += 4) {
-        if (g >= 4) rows_at(g);
-        codes_to_lds(v, r, g / kFewU, codes + g % kFewU * R * kGroup, scales + g % kFewU * 16);
+      if constexpr (!CODES) {
+        for (int g = q; g < n * kFewU; g += 4) {
+          if (g >= 4) rows_at(g);
+          codes_to_lds(v, r, g / kFewU, codes + g % kFewU * R * kGroup, scales + g % kFewU * 16);
+        }
+        lds_order();
       }
-      lds_order();
 #pragma unroll
       for (int k = 0; k < kFewU; ++k) {
         if (kb0 + k * waves >= KB) break;
-        const int row = r < n ? r : 0; // (columns from n on are not kept)
-        const v8i x = codes_from_lds(codes + k * R * kGroup, row, q);
-        const float s = scales[k * 16 + row], s0 = s * lane_value(bg, k), s1 = s * lane_value(bu, k);
-        const v4f d0 = mfma_e4m3_exact(wg[k], x), d1 = mfma_e4m3_exact(wu[k], x);
+        if constexpr (!CODES) {
+          x[k] = codes_from_lds(codes + k * R * kGroup, row, q);
+          sx[k] = scales[k * 16 + row];
+        }
+        const float s0 = sx[k] * lane_value(bg, k), s1 = sx[k] * lane_value(bu, k);
+        const v4f d0 = mfma_e4m3_exact(wg[k], x[k]), d1 = mfma_e4m3_exact(wu[k], x[k]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           acc[0][i] = __builtin_fmaf(d0[i], s0, acc[0][i]);
@@ -192,8 +215,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void e
 
 // Tokens in groups of up to 64 slots, one to blockIdx.y: a wave holds the group's routing in its lanes, and an expert has 16 tokens at the most.
 // (An expert that several groups hit is read again, out of L2: neighbouring blockIdx.x are what one XCD gets of every group.)
-template <int DT>
+template <int DT, bool CODES>
 __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8ExpertsArgs a) {
+  constexpr int U = CODES ? 2 : kFewU; // K blocks at a time (with codes, rows and weights take registers alike)
   // [wave] codes, scales, lists; [part][slot][column] results; [slot] weight; [slot] the token's first one with this expert, -1: none here
   extern __shared__ __attribute__((aligned(16))) int8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4, waves = blockDim.x >> 6;
@@ -226,7 +250,7 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
   }
   if (wave == 0) from[lane] = static_cast<int16_t>(mine);
 
-  // The wave's work: (expert, part of K), of every `waves`-th; up to kFewU K blocks at a time, the next ones' weights and first activations
+  // The wave's work: (expert, part of K), of every `waves`-th; up to U K blocks at a time, the next ones' weights and first activations
   // asked for before these are used.
   const int items = experts * parts;
   struct Piece {
@@ -246,34 +270,48 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
     return p;
   };
   auto next = [&](Piece p) __attribute__((always_inline)) {
-    if (p.kb + kFewU >= p.hi) return begin(p.it + waves, p.list ^ 1);
-    p.kb += kFewU;
+    if (p.kb + U >= p.hi) return begin(p.it + waves, p.list ^ 1);
+    p.kb += U;
     return p;
   };
-  v8i w[2][kFewU];
+  v8i w[2][U];
   float b[2], v[8]; // scales of the weights, a K block a lane; activations
+  v8i x[2][U];
+  float sx[2][U];
   auto acts_at = [&](const Piece &p, int g) __attribute__((always_inline)) { // of group g: 16 lanes, eight values each
-    const int kb = p.kb + g % kFewU;
-    load8<LO_F32>(a.act, static_cast<int64_t>(slot0 + lists[p.list * kFewTokens + g / kFewU]) * I + (kb < p.hi ? kb : p.hi - 1) * kGroup + r * 8, v);
+    const int kb = p.kb + g % U;
+    load8<LO_F32>(a.act, static_cast<int64_t>(slot0 + lists[p.list * kFewTokens + g / U]) * I + (kb < p.hi ? kb : p.hi - 1) * kGroup + r * 8, v);
   };
   auto load = [&](const Piece &p, int at) __attribute__((always_inline)) {
     if (p.it >= items) return;
-    if (q < p.count * kFewU) acts_at(p, q);
+    if constexpr (CODES) {
+      const int64_t slot = slot0 + lists[p.list * kFewTokens + (r < p.count ? r : 0)];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int kc = p.kb + k < p.hi ? p.kb + k : p.hi - 1;
+        const int8_t *const row = a.aq + slot * I + kc * kGroup + q * 16;
+        x[at][k] = join(*reinterpret_cast<const v4i *>(row), *reinterpret_cast<const v4i *>(row + 64));
+        sx[at][k] = a.as[slot * KB + kc];
+      }
+    } else if (q < p.count * U) {
+      acts_at(p, q);
+    }
     const brsrc rW = make_rsrc(a.w2 + (static_cast<int64_t>(p.e) * a.H + n0) * I, static_cast<uint32_t>(16 * I));
     const float *const sw = a.w2s + (static_cast<int64_t>(p.e) * (a.H / kGroup) + n0 / kGroup) * KB;
 #pragma unroll
-    for (int k = 0; k < kFewU; ++k) {
+    for (int k = 0; k < U; ++k) {
       const int kc = p.kb + k < p.hi ? p.kb + k : p.hi - 1, off = r * I + q * 16 + kc * kGroup;
       w[at][k] = join(bld16(rW, off, 0), bld16(rW, off + 64, 0));
     }
-    const int mine = p.kb + lane % kFewU;
+    const int mine = p.kb + lane % U;
     b[at] = sw[mine < p.hi ? mine : p.hi - 1];
   };
   v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
   auto quantise = [&](const Piece &p) __attribute__((always_inline)) {
-    for (int g = q; g < p.count * kFewU; g += 4) {
+    if constexpr (CODES) return;
+    for (int g = q; g < p.count * U; g += 4) {
       if (g >= 4) acts_at(p, g);
-      codes_to_lds(v, r, g / kFewU, codes + g % kFewU * R * kGroup, scales + g % kFewU * 16);
+      codes_to_lds(v, r, g / U, codes + g % U * R * kGroup, scales + g % U * 16);
     }
     lds_order();
   };
@@ -281,14 +319,18 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
     if (p.kb == KB * p.part / parts) acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     const int row = r < p.count ? r : 0; // (columns past the tokens are not kept)
 #pragma unroll
-    for (int k = 0; k < kFewU; ++k) {
+    for (int k = 0; k < U; ++k) {
       if (p.kb + k >= p.hi) break;
-      const v4f d = mfma_e4m3(w[at][k], codes_from_lds(codes + k * R * kGroup, row, q));
-      const float s = scales[k * 16 + row] * lane_value(b[at], k);
+      if constexpr (!CODES) {
+        x[at][k] = codes_from_lds(codes + k * R * kGroup, row, q);
+        sx[at][k] = scales[k * 16 + row];
+      }
+      const v4f d = mfma_e4m3(w[at][k], x[at][k]);
+      const float s = sx[at][k] * lane_value(b[at], k);
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s, acc[i]);
     }
-    if (p.kb + kFewU >= p.hi && r < p.count)
+    if (p.kb + U >= p.hi && r < p.count)
       *reinterpret_cast<v4f *>(ys + (p.part * 64 + lists[p.list * kFewTokens + r]) * 16 + 4 * q) = acc;
     lds_order();
   };
@@ -323,22 +365,22 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
   }
 }
 
-template <int DT, int ACT, bool SMALL> static int launch_up(const Fp8ExpertsArgs &a, hipStream_t stream) {
+template <int DT, int ACT, bool SMALL, bool CODES> static int launch_up(const Fp8ExpertsArgs &a, hipStream_t stream) {
   // waves that have kFewU K blocks each, in as few rounds as eight of them need
   const int KB = a.H / kGroup, rounds = (KB + 8 * kFewU - 1) / (8 * kFewU), waves = (KB + rounds * kFewU - 1) / (rounds * kFewU);
   const int lds = waves * (few_wave_lds(a.rows) + kFewRed) + (SMALL ? 0 : a.S * 2);
-  const auto kernel = experts_fp8_up_kernel<DT, ACT, SMALL>;
+  const auto kernel = experts_fp8_up_kernel<DT, ACT, SMALL, CODES>;
   static unsigned long long done = 0;
   const int rc = reserve_lds_once(reinterpret_cast<const void *>(kernel), 8 * (few_wave_lds(16) + kFewRed) + kFewSlots * 2, &done);
   if (rc) return rc;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.I / 16), static_cast<unsigned>(a.units)), dim3(waves * 64), lds, stream, a);
   return check_launch("fused_experts_fp8");
 }
-template <int DT> static int launch_down(const Fp8ExpertsArgs &a, hipStream_t stream) {
+template <int DT, bool CODES> static int launch_down(const Fp8ExpertsArgs &a, hipStream_t stream) {
   const int waves = kFewMaxWaves, lds = waves * few_wave_lds(a.rows) + a.parts * 64 * 64 + 64 * 6;
   constexpr int most = kFewMaxWaves * few_wave_lds(kFewGroup) + kFewParts * 64 * 64 + 64 * 6;
   static_assert(most <= 160 * 1024, "LDS");
-  const auto kernel = experts_fp8_down_kernel<DT>;
+  const auto kernel = experts_fp8_down_kernel<DT, CODES>;
   static unsigned long long done = 0;
   const int rc = reserve_lds_once(reinterpret_cast<const void *>(kernel), most, &done);
   if (rc) return rc;
@@ -349,24 +391,56 @@ template <int DT> static int launch_down(const Fp8ExpertsArgs &a, hipStream_t st
 }
 template <int DT> static int launch_experts_fp8(Fp8ExpertsArgs a, int activation, hipStream_t stream) {
   const int M = a.S / a.top_k, KB = a.I / kGroup;
-  a.rows = M < 16 ? M : 16;
-  const bool gelu = activation == LO_ACT_GELU;
-  const int rc = a.S <= 64 ? (gelu ? launch_up<DT, LO_ACT_GELU, true>(a, stream) : launch_up<DT, LO_ACT_SILU, true>(a, stream))
-                           : (gelu ? launch_up<DT, LO_ACT_GELU, false>(a, stream) : launch_up<DT, LO_ACT_SILU, false>(a, stream));
+  const bool gelu = activation == LO_ACT_GELU, small = few_in_two(a.S);
+  // (rows that come as codes take no LDS)
+  a.rows = !small ? 0 : M < 16 ? M : 16;
+  int rc;
+  if (small) {
+    rc = gelu ? launch_up<DT, LO_ACT_GELU, true, false>(a, stream) : launch_up<DT, LO_ACT_SILU, true, false>(a, stream);
+  } else {
+    rc = lo_per_token_group_quant_fp8(a.x, DT, M, a.H, 1e-10f, const_cast<int8_t *>(a.xq), const_cast<float *>(a.xs), stream);
+    if (rc) return rc;
+    rc = gelu ? launch_up<DT, LO_ACT_GELU, false, true>(a, stream) : launch_up<DT, LO_ACT_SILU, false, true>(a, stream);
+    if (rc) return rc;
+    // (rows of slots without an expert here hold anything, and are not read)
+    rc = lo_per_token_group_quant_fp8(a.act, LO_F32, a.S, a.I, 1e-10f, const_cast<int8_t *>(a.aq), const_cast<float *>(a.as), stream);
+  }
   if (rc) return rc;
   a.group = 64 / a.top_k < kFewGroup ? 64 / a.top_k : kFewGroup;
-  a.rows = M < a.group ? M : a.group;
+  a.rows = !small ? 0 : M < a.group ? M : a.group;
   // parts of the second product's K: what a wave has in flight at once
   a.parts = (KB + kFewU - 1) / kFewU < kFewParts ? (KB + kFewU - 1) / kFewU : kFewParts;
-  return launch_down<DT>(a, stream);
+  return small ? launch_down<DT, false>(a, stream) : launch_down<DT, true>(a, stream);
 }
 
 } // namespace lo
 
-extern "C" int64_t lo_fused_experts_fp8_workspace_bytes(int64_t M, int32_t top_k, int64_t I, int32_t E) {
+namespace lo {
+struct FewLayout { // of the workspace: activations; beyond two launches codes and scales of the rows and of the activations
+  int64_t xq, xs, aq, as, total;
+};
+static FewLayout few_layout(int64_t M, int32_t top_k, int64_t H, int64_t I) {
+  const int64_t S = M * top_k;
+  FewLayout l{};
+  l.total = S * I * 4;
+  if (few_in_two(S)) return l;
+  const auto take = [&](int64_t bytes) {
+    const int64_t at = l.total;
+    l.total += (bytes + 15) / 16 * 16;
+    return at;
+  };
+  l.xq = take(M * H);
+  l.xs = take(M * (H / kGroup) * 4);
+  l.aq = take(S * I);
+  l.as = take(S * (I / kGroup) * 4);
+  return l;
+}
+} // namespace lo
+
+extern "C" int64_t lo_fused_experts_fp8_workspace_bytes(int64_t M, int32_t top_k, int64_t H, int64_t I) {
   using namespace lo;
-  if (M < 0 || top_k < 1 || I < kGroup || E < 1) return LO_EINVAL;
-  return M * top_k * I * 4;
+  if (M < 0 || top_k < 1 || H < kGroup || I < kGroup) return LO_EINVAL;
+  return few_layout(M, top_k, H, I).total;
 }
 
 extern "C" int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t H, int64_t I, int32_t E, int32_t num_experts,
@@ -391,14 +465,20 @@ extern "C" int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t
   const auto off = [](const void *p, unsigned al) { return (reinterpret_cast<uintptr_t>(p) & (al - 1)) != 0; };
   LO_REQUIRE(!off(x, 16) && !off(w1, 16) && !off(w2, 16) && !off(workspace, 16) && !off(out, 2) && !off(shared_output, 2), LO_EINVAL,
              "fused_experts_fp8: rows, weights and workspace must be 16-byte aligned");
-  const int64_t need = lo_fused_experts_fp8_workspace_bytes(M, top_k, I, E);
+  const FewLayout layout = few_layout(M, top_k, H, I);
+  const int64_t need = layout.total;
   LO_REQUIRE(workspace_bytes >= need, LO_ENOSPC, "fused_experts_fp8: workspace holds %lld bytes, needs %lld", (long long)workspace_bytes,
              (long long)need);
   Fp8ExpertsArgs a{};
   a.x = x; a.ids = topk_ids; a.shared = shared_output;
   a.w1 = static_cast<const int8_t *>(w1); a.w2 = static_cast<const int8_t *>(w2);
   a.w1s = w1s; a.w2s = w2s; a.topk_w = topk_w; a.map = expert_map; a.out = out;
-  a.act = static_cast<float *>(workspace);
+  char *const ws = static_cast<char *>(workspace);
+  a.act = reinterpret_cast<float *>(ws);
+  a.xq = reinterpret_cast<int8_t *>(ws + layout.xq);
+  a.xs = reinterpret_cast<float *>(ws + layout.xs);
+  a.aq = reinterpret_cast<int8_t *>(ws + layout.aq);
+  a.as = reinterpret_cast<float *>(ws + layout.as);
   a.S = static_cast<int32_t>(M * top_k); a.H = static_cast<int32_t>(H); a.I = static_cast<int32_t>(I);
   a.E = E; a.Eg = num_experts; a.top_k = top_k; a.factor = routed_scaling_factor;
   a.ids64 = ids_dtype == LO_I64;

@@ -557,7 +557,7 @@ PyObject *experts_fp8(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   if (experts < E || experts > INT32_MAX || k < 1 || k > INT32_MAX || M > INT32_MAX) Py_RETURN_NONE;
   if (t[7] && (t[7]->scalar_type() != at::kInt || t[7]->numel() < experts)) Py_RETURN_NONE;
   if (t[8] && (t[8]->scalar_type() != x.scalar_type() || t[8]->sizes() != x.sizes())) Py_RETURN_NONE;
-  const int64_t bytes = g_experts_fp8_bytes(M, static_cast<int32_t>(k), I, static_cast<int32_t>(E));
+  const int64_t bytes = g_experts_fp8_bytes(M, static_cast<int32_t>(k), H, I);
   if (bytes < 0) return raise(static_cast<int>(bytes));
   const hipStream_t stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream();
   if (capturing(stream)) Py_RETURN_NONE; // (its scratch belongs to the graph)

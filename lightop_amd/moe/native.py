@@ -636,7 +636,8 @@ def fused_experts_decode_fp8(hidden_states: torch.Tensor,
                              routed_scaling_factor: float = 1.0,
                              shared_output: Optional[torch.Tensor] = None,
                              inplace: bool = False) -> torch.Tensor:
-    """The routed experts of a decode batch (at most 64 tokens and 1024 slots) with e4m3 weights, in two launches.
+    """The routed experts of a decode batch (at most 64 tokens, 64 slots a token and 1024 in all) with e4m3 weights, in two
+    launches, four beyond 64 slots.
 
     ``hidden_states`` [M, H] bf16 or fp16; ``w1`` [E, 2I, H], ``w2`` [E, H, I] float8_e4m3fn, row-major as a checkpoint holds them,
     with one fp32 scale for 128 x 128: ``w1_scale`` [E, 2I/128, H/128], ``w2_scale`` [E, H/128, I/128].  Rows are quantised in front
@@ -687,7 +688,7 @@ def fused_experts_decode_fp8(hidden_states: torch.Tensor,
     shared = None if shared_output is None else shared_output.contiguous()
     w1, w2 = _rows16(w1), _rows16(w2)
     lib = _lib.lib()
-    nbytes = lib.lo_fused_experts_fp8_workspace_bytes(M, top_k, I, E)
+    nbytes = lib.lo_fused_experts_fp8_workspace_bytes(M, top_k, H, I)
     _lib.check(nbytes)
     with _on_device(x):
         stream = torch.cuda.current_stream(x.device).cuda_stream

@@ -94,9 +94,9 @@ def test_gemm_workspace(lib):
 
 def test_experts_workspace(lib):
     n = lib.lo_fused_experts_fp8_workspace_bytes
-    assert n(1, 8, 768, 128) == 8 * 768 * 4
-    assert n(64, 8, 2048, 32) == 512 * 2048 * 4
-    assert n(-1, 8, 768, 128) < 0 and n(1, 0, 768, 128) < 0 and n(1, 1, 64, 1) < 0
+    assert n(1, 8, 2048, 768) == 8 * 768 * 4
+    assert n(64, 8, 7168, 2048) == 512 * 2048 * 4 + 64 * 7168 * (1 + 4 / 128) + 512 * 2048 * (1 + 4 / 128)
+    assert n(-1, 8, 2048, 768) < 0 and n(1, 0, 2048, 768) < 0 and n(1, 1, 256, 64) < 0 and n(1, 1, 64, 256) < 0
 
 
 def test_python_needs_the_gpu():

@@ -41,7 +41,7 @@ def _run(x, w, tw, ids, emap=None, act="silu", factor=1.0, shared=None):
     M, H = x.shape
     E, I, k = w1.shape[0], w1.shape[1] // 2, ids.shape[1]
     lib = _lib.lib()
-    n = lib.lo_fused_experts_fp8_workspace_bytes(M, k, I, E)
+    n = lib.lo_fused_experts_fp8_workspace_bytes(M, k, H, I)
     ws = torch.full((n,), 0xff, dtype=torch.uint8, device="cuda")  # NaN wherever nothing is written
     out = torch.empty_like(x)
     _lib.check(lib.lo_fused_experts_fp8(

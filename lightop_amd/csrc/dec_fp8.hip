@@ -213,65 +213,108 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void e
   }
 }
 
-// Tokens in groups of up to 64 slots, one to blockIdx.y: a wave holds the group's routing in its lanes, and an expert has 16 tokens at the most.
-// (An expert that several groups hit is read again, out of L2: neighbouring blockIdx.x are what one XCD gets of every group.)
+// Without codes: tokens in groups of up to 64 slots, one to blockIdx.y; a wave holds the group's routing in its lanes, and an expert has
+// 16 tokens at the most.  With them: all tokens (read by groups, weights that several of them hit came from HBM more than once: 64 tokens of
+// a DeepSeek-V3 share 165 us), the routing in LDS.
 template <int DT, bool CODES>
 __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8ExpertsArgs a) {
   constexpr int U = CODES ? 2 : kFewU; // K blocks at a time (with codes, rows and weights take registers alike)
-  // [wave] codes, scales, lists; [part][slot][column] results; [slot] weight; [slot] the token's first one with this expert, -1: none here
+  // [wave] codes, scales, lists; [part][slot][column] results; [slot] weight; [slot] the token's first one with this expert, -1: none here;
+  // with codes: [slot] expert; the experts hit
   extern __shared__ __attribute__((aligned(16))) int8_t smem[];
+  __shared__ uint32_t present[CODES ? kFewExperts / 32 : 1];
+  __shared__ int number;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n0 = blockIdx.x * 16, I = a.I, KB = I / kGroup, R = a.rows, per = few_wave_lds(R), parts = a.parts;
-  const int first = blockIdx.y * a.group, M = a.S / a.top_k - first < a.group ? a.S / a.top_k - first : a.group;
-  const int S = M * a.top_k, slot0 = first * a.top_k; // of the group
+  const int first = CODES ? 0 : blockIdx.y * a.group, M = a.S / a.top_k - first < a.group ? a.S / a.top_k - first : a.group;
+  const int S = M * a.top_k, slot0 = first * a.top_k, pitch = CODES ? S : 64; // of the group
   int8_t *const codes = smem + wave * per;
   float *const scales = reinterpret_cast<float *>(codes + kFewU * R * kGroup);
   int16_t *const lists = reinterpret_cast<int16_t *>(scales + kFewU * 16);
-  float *const ys = reinterpret_cast<float *>(smem + waves * per), *const weight = ys + parts * 64 * 16;
-  int16_t *const from = reinterpret_cast<int16_t *>(weight + 64);
-  const Route<true> route(a, nullptr, lane, slot0, S);
+  float *const ys = reinterpret_cast<float *>(smem + waves * per), *const weight = ys + parts * pitch * 16;
+  int16_t *const from = reinterpret_cast<int16_t *>(weight + pitch), *const keys = from + pitch, *const hit = keys + pitch;
+  if constexpr (CODES)
+    for (int i = tid; i < kFewExperts / 32; i += blockDim.x) present[i] = 0;
+  const Route<!CODES> route(a, keys, lane, slot0, S);
   // (asked for here, not behind the last product)
-  if (tid < S) weight[tid] = a.topk_w[slot0 + tid];
+  for (int s = tid; s < S; s += blockDim.x) weight[s] = a.topk_w[slot0 + s];
   float shared = 0.0f;
   if (a.shared && tid < M * 16)
     shared = to_f32<DT>(static_cast<const uint16_t *>(a.shared)[static_cast<int64_t>(first + (tid >> 4)) * a.H + n0 + (tid & 15)]);
-  uint64_t leaders = 0; // first slots of the experts hit
-  int experts = 0, mine = -1;
-  for (uint64_t left = __builtin_amdgcn_ballot_w64(route.key >= 0); left; ++experts) { // an expert at a time
-    const int s = __builtin_ctzll(left);
-    const uint64_t same = __builtin_amdgcn_ballot_w64(route.key == __builtin_amdgcn_readlane(route.key, s));
-    if (same >> lane & 1) {
-      const uint64_t before = same & route.earlier_of_token();
-      mine = before ? __builtin_ctzll(before) : lane;
+  uint64_t leaders = 0; // without codes: first slots of the experts hit
+  int experts = 0;
+  if constexpr (!CODES) {
+    int mine = -1;
+    for (uint64_t left = __builtin_amdgcn_ballot_w64(route.key >= 0); left; ++experts) { // an expert at a time
+      const int s = __builtin_ctzll(left);
+      const uint64_t same = __builtin_amdgcn_ballot_w64(route.key == __builtin_amdgcn_readlane(route.key, s));
+      if (same >> lane & 1) {
+        const uint64_t before = same & route.earlier_of_token();
+        mine = before ? __builtin_ctzll(before) : lane;
+      }
+      left &= ~same;
+      leaders |= 1ull << s;
     }
-    left &= ~same;
-    leaders |= 1ull << s;
+    if (wave == 0) from[lane] = static_cast<int16_t>(mine);
+  } else {
+    for (int s = tid; s < S; s += blockDim.x) {
+      const int e = keys[s];
+      int j = s / a.top_k * a.top_k;
+      while (j < s && keys[j] != e) ++j;
+      from[s] = static_cast<int16_t>(e < 0 ? -1 : j);
+      if (e >= 0) atomicOr(&present[e >> 5], 1u << (e & 31));
+    }
+    __syncthreads();
+    if (wave == 0) {
+      static_assert(kFewExperts / 32 == 64, "a word a lane");
+      uint32_t left = present[lane];
+      int all = __popc(left); // of the lanes up to this one
+      const int own = all;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(all, d);
+        if (lane >= d) all += o;
+      }
+      for (int at = all - own; left; left &= left - 1) hit[at++] = static_cast<int16_t>(lane * 32 + __builtin_ctz(left));
+      if (lane == 63) number = all;
+    }
+    __syncthreads();
+    experts = number;
   }
-  if (wave == 0) from[lane] = static_cast<int16_t>(mine);
 
-  // The wave's work: (expert, part of K), of every `waves`-th; up to U K blocks at a time, the next ones' weights and first activations
-  // asked for before these are used.
+  // The wave's work: (expert, part of K), of every `waves`-th, 16 of the expert's tokens at a time; up to U K blocks of them at a time, the next
+  // ones' weights and rows asked for before these are used.
   const int items = experts * parts;
   struct Piece {
-    int it, e, part, count, kb, hi, list;
+    int it, e, part, count, f, kb, hi, list;
   };
   auto begin = [&](int it, int list) __attribute__((always_inline)) {
-    Piece p{it, 0, 0, 0, 0, 0, list};
+    Piece p{it, 0, 0, 0, 0, 0, 0, list};
     if (it >= items) return p;
     int at = it / parts;
     p.part = it - at * parts;
-    uint64_t left = leaders;
-    for (; at > 0; --at) left &= left - 1;
-    p.e = route.slot_expert(__builtin_ctzll(left));
+    if constexpr (CODES) {
+      p.e = __builtin_amdgcn_readfirstlane(hit[at]);
+    } else {
+      uint64_t left = leaders;
+      for (; at > 0; --at) left &= left - 1;
+      p.e = route.slot_expert(__builtin_ctzll(left));
+    }
     p.kb = KB * p.part / parts;
     p.hi = KB * (p.part + 1) / parts;
     p.count = route.slots(p.e, -1, lists + list * kFewTokens);
     return p;
   };
   auto next = [&](Piece p) __attribute__((always_inline)) {
-    if (p.kb + U >= p.hi) return begin(p.it + waves, p.list ^ 1);
-    p.kb += U;
+    if (p.kb + U < p.hi) {
+      p.kb += U;
+    } else if (CODES && p.f + 16 < p.count) {
+      p.f += 16;
+      p.kb = KB * p.part / parts;
+    } else {
+      p = begin(p.it + waves, p.list ^ 1);
+    }
     return p;
   };
   v8i w[2][U];
@@ -285,7 +328,7 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
   auto load = [&](const Piece &p, int at) __attribute__((always_inline)) {
     if (p.it >= items) return;
     if constexpr (CODES) {
-      const int64_t slot = slot0 + lists[p.list * kFewTokens + (r < p.count ? r : 0)];
+      const int64_t slot = lists[p.list * kFewTokens + (p.f + r < p.count ? p.f + r : 0)];
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         const int kc = p.kb + k < p.hi ? p.kb + k : p.hi - 1;
@@ -330,8 +373,8 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s, acc[i]);
     }
-    if (p.kb + U >= p.hi && r < p.count)
-      *reinterpret_cast<v4f *>(ys + (p.part * 64 + lists[p.list * kFewTokens + r]) * 16 + 4 * q) = acc;
+    if (p.kb + U >= p.hi && p.f + r < p.count)
+      *reinterpret_cast<v4f *>(ys + (p.part * pitch + lists[p.list * kFewTokens + p.f + r]) * 16 + 4 * q) = acc;
     lds_order();
   };
   Piece p = begin(wave, 0);
@@ -355,7 +398,7 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
       const int s = from[s0 + j];
       if (s < 0) continue;
       float y = 0.0f;
-      for (int k = 0; k < parts; ++k) y += ys[(k * 64 + s) * 16 + c];
+      for (int k = 0; k < parts; ++k) y += ys[(k * pitch + s) * 16 + c];
       sum = __builtin_fmaf(weight[s0 + j], y, sum);
     }
     sum *= a.factor;
@@ -376,21 +419,28 @@ template <int DT, int ACT, bool SMALL, bool CODES> static int launch_up(const Fp
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.I / 16), static_cast<unsigned>(a.units)), dim3(waves * 64), lds, stream, a);
   return check_launch("fused_experts_fp8");
 }
-template <int DT, bool CODES> static int launch_down(const Fp8ExpertsArgs &a, hipStream_t stream) {
-  const int waves = kFewMaxWaves, lds = waves * few_wave_lds(a.rows) + a.parts * 64 * 64 + 64 * 6;
-  constexpr int most = kFewMaxWaves * few_wave_lds(kFewGroup) + kFewParts * 64 * 64 + 64 * 6;
-  static_assert(most <= 160 * 1024, "LDS");
+template <int DT, bool CODES> static int launch_down(Fp8ExpertsArgs a, hipStream_t stream) {
+  const int M = a.S / a.top_k, KB = a.I / kGroup;
+  a.group = CODES ? M : 64 / a.top_k < kFewGroup ? 64 / a.top_k : kFewGroup;
+  a.rows = CODES ? 0 : M < a.group ? M : a.group;
+  // parts of K: what a wave has in flight at once, while the results fit LDS
+  a.parts = (KB + kFewU - 1) / kFewU < kFewParts ? (KB + kFewU - 1) / kFewU : kFewParts;
+  while (CODES && a.parts > 1 && a.parts * a.S > kFewSlots) --a.parts;
+  const int slots = CODES ? a.S : 64;
+  const int lds = kFewMaxWaves * few_wave_lds(a.rows) + slots * (a.parts * 64 + 6) + (CODES ? slots * 2 + a.E * 2 : 0);
+  constexpr int most = CODES ? kFewMaxWaves * few_wave_lds(0) + kFewSlots * (64 + 8) + kFewExperts * 2
+                             : kFewMaxWaves * few_wave_lds(kFewGroup) + 64 * (kFewParts * 64 + 6);
+  static_assert(most <= 160 * 1024 - 512, "LDS");
   const auto kernel = experts_fp8_down_kernel<DT, CODES>;
   static unsigned long long done = 0;
   const int rc = reserve_lds_once(reinterpret_cast<const void *>(kernel), most, &done);
   if (rc) return rc;
-  const int M = a.S / a.top_k;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.H / 16), static_cast<unsigned>((M + a.group - 1) / a.group)), dim3(waves * 64), lds, stream,
-                     a);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.H / 16), static_cast<unsigned>((M + a.group - 1) / a.group)), dim3(kFewMaxWaves * 64), lds,
+                     stream, a);
   return check_launch("fused_experts_fp8");
 }
 template <int DT> static int launch_experts_fp8(Fp8ExpertsArgs a, int activation, hipStream_t stream) {
-  const int M = a.S / a.top_k, KB = a.I / kGroup;
+  const int M = a.S / a.top_k;
   const bool gelu = activation == LO_ACT_GELU, small = few_in_two(a.S);
   // (rows that come as codes take no LDS)
   a.rows = !small ? 0 : M < 16 ? M : 16;
@@ -406,10 +456,6 @@ template <int DT> static int launch_experts_fp8(Fp8ExpertsArgs a, int activation
     rc = lo_per_token_group_quant_fp8(a.act, LO_F32, a.S, a.I, 1e-10f, const_cast<int8_t *>(a.aq), const_cast<float *>(a.as), stream);
   }
   if (rc) return rc;
-  a.group = 64 / a.top_k < kFewGroup ? 64 / a.top_k : kFewGroup;
-  a.rows = !small ? 0 : M < a.group ? M : a.group;
-  // parts of the second product's K: what a wave has in flight at once
-  a.parts = (KB + kFewU - 1) / kFewU < kFewParts ? (KB + kFewU - 1) / kFewU : kFewParts;
   return small ? launch_down<DT, false>(a, stream) : launch_down<DT, true>(a, stream);
 }
 

@@ -109,7 +109,8 @@ __device__ __forceinline__ float silu_f32(float g) {
   const float e = __builtin_amdgcn_exp2f(n);
   // (past the ends of the exponential there is nothing to correct, and an infinite n has no difference)
   const float e1 = fabsf(n) < 126.0f ? __builtin_fmaf(e, lost * 0.693147182f, e) : e;
-  return g * __builtin_amdgcn_rcpf(1.0f + e1);
+  const float d = 1.0f + e1, r = __builtin_amdgcn_rcpf(d);
+  return g * (r > 0.0f ? __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r) : r); // (an infinite d: 0)
 }
 // GELU in its erf form; the complement keeps the digits that 1 + erf loses left of zero.
 __device__ __forceinline__ float gelu_f32(float g) { return 0.5f * g * erfcf(g * -0.707106769f); }

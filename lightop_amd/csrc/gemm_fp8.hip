@@ -101,10 +101,16 @@ template <int DT, int TM, int TN, int WM, int WN, int ST, bool PART>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_fp8_tile_kernel(const Fp8GemmArgs a, int group_m) {
   constexpr int kWaves = WM * WN;
   constexpr int FM = TM / WM / 16, FN = TN / WN / 16;             // fragments of a wave: tokens, weights
-  constexpr int kPer = (TM + TN) / 8 / kWaves, kCopies = kPer + 1; // 1 KB copies of a stage, of a wave, and its scales
-  constexpr int kStep = (kCopies + FM - 1) / FM;                   // copies of a step
+  constexpr int kA = TM / 8 / kWaves, kB = TN / 8 / kWaves, kCopies = 1 + kA + kB; // 1 KB copies of a stage, of a wave, and its scales
+  constexpr int kStep = (kCopies + FM - 1) / FM;                                   // copies of a step
   constexpr int kStage = (TM + TN) * kGroup;
-  static_assert((TM + TN) / 8 % kWaves == 0 && TM % 64 == 0 && TM / 64 <= kWaves && (TN / WN) % 16 == 0 && 128 % (TN / WN) == 0 &&
+  // Two stages leave a copy little time.  The weights' part of a stage is free long before the tokens', once every wave has its fragments:
+  // the workgroup meets in front of step kMid too, and from there on the next but one K block's weights are asked for, its tokens
+  // behind the last step's barrier.
+  constexpr bool kApart = ST == 2;
+  constexpr int kMid = kA - 1;
+  static_assert(!kApart || (kA >= 2 && kMid < FM - 2), "steps for the copies");
+  static_assert(TM / 8 % kWaves == 0 && TN / 8 % kWaves == 0 && TM % 64 == 0 && TM / 64 <= kWaves && (TN / WN) % 16 == 0 && 128 % (TN / WN) == 0 &&
                     FM % 2 == 0 && ST <= 5, "tile");
   extern __shared__ __attribute__((aligned(16))) int8_t smem[];
   int8_t *const sS = smem + ST * kStage; // [K blocks / 4, odd or even][token][4] scales
@@ -121,10 +127,10 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_fp8_tile_kernel(const Fp8Ge
   const int8_t *const pa = a.A + m0 * K + first * kGroup, *const pb = a.B + n0 * K + first * kGroup;
   const float *const ps = a.As + m0 * allKB + first;
   const int ends = (rows * allKB - first) * 4;
-  int voff[kPer];
+  int voff[kA + kB];
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int p = wave * kPer + j, row = (p < TM / 8 ? p : p - TM / 8) * 8 + (lane >> 3);
+  for (int j = 0; j < kA + kB; ++j) {
+    const int row = (j < kA ? wave * kA + j : wave * kB + j - kA) * 8 + (lane >> 3);
     voff[j] = row * K + (((lane & 7) ^ (row & 7)) * 16);
   }
   const int sgrp = wave % (TM / 64), soff = (sgrp * 64 + lane) * allKB * 4;
@@ -137,14 +143,15 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_fp8_tile_kernel(const Fp8Ge
   };
   auto copy = [&](int c, int kb, int stage) __attribute__((always_inline)) {
     const bool in = kb < KB;
-    if (c == 0) { // once in four: those behind the ones that K block kb - ST + 1 begins
+    if (c == 0) { // once in four: those behind the ones that K block kb - 1 (two stages), kb - ST + 1 begins
       const int at = kb - ST + 1;
       copy_scales((at >> 2) + 1, (at & 3) == 0 && at > 0);
-    } else {
-      const int p = wave * kPer + c - 1;
-      const bool of_a = p < TM / 8;
-      copy16(make_rsrc(of_a ? pa : pb, in ? static_cast<uint32_t>((of_a ? rows : cols) * K - first * kGroup) : 0u), smem + stage * kStage + p * 1024,
+    } else if (c <= kA) {
+      copy16(make_rsrc(pa, in ? static_cast<uint32_t>(rows * K - first * kGroup) : 0u), smem + stage * kStage + (wave * kA + c - 1) * 1024,
              voff[c - 1], kb * kGroup);
+    } else {
+      copy16(make_rsrc(pb, in ? static_cast<uint32_t>(cols * K - first * kGroup) : 0u),
+             smem + stage * kStage + TM * kGroup + (wave * kB + c - 1 - kA) * 1024, voff[c - 1], kb * kGroup);
     }
   };
   int64_t nblk = (n0 + wn * (TN / WN)) >> 7;
@@ -171,11 +178,21 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_fp8_tile_kernel(const Fp8Ge
 
   copy_scales(0, true);
   copy_scales(1, true);
+  if constexpr (kApart) {
 #pragma unroll
-  for (int i = 0; i < ST; ++i)
+    for (int c = 1; c < kCopies; ++c) copy(c, 0, 0);
 #pragma unroll
-    for (int c = 0; c < (i < ST - 1 ? kCopies : kStep); ++c) copy(c, i, i);
-  wait_barrier<(ST - 2) * kCopies + kStep>();
+    for (int c = 1 + kA; c < kCopies; ++c) copy(c, 1, 1);
+    copy(0, 1, 1);
+    copy(1, 1, 1);
+    wait_barrier<kB + 2>();
+  } else {
+#pragma unroll
+    for (int i = 0; i < ST; ++i)
+#pragma unroll
+      for (int c = 0; c < (i < ST - 1 ? kCopies : kStep); ++c) copy(c, i, i);
+    wait_barrier<(ST - 2) * kCopies + kStep>();
+  }
   v8i w[FN], x[2];
   float s[2];
 #pragma unroll
@@ -204,15 +221,28 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_fp8_tile_kernel(const Fp8Ge
         x[cur ^ 1] = read(sa, m + 1, stage);
         s[cur ^ 1] = scale(m + 1, kb);
       } else {
-        wait_barrier<(ST - 2) * kCopies>();
+        wait_barrier<kApart ? kB : (ST - 2) * kCopies>();
         x[cur ^ 1] = read(sa, 0, next);
         s[cur ^ 1] = scale(0, kb + 1);
       }
-      // the stage that the last barrier freed
+      if constexpr (kApart) {
+        if (m == kMid) asm volatile("s_barrier" ::: "memory"); // (every wave has used its weights: they are in registers)
+        if (m + 1 == FM) {
+          copy(0, kb + 2, stage);
+          copy(1, kb + 2, stage);
+        } else if (m < kMid) {
+          if (m + 2 <= kA) copy(m + 2, kb + 1, next);
+        } else {
 #pragma unroll
-      for (int c = 0; c < kStep; ++c) {
-        const int at = (m + 1 == FM ? 0 : m + 1) * kStep + c;
-        if (at < kCopies) copy(at, m + 1 == FM ? kb + ST : kb + ST - 1, m + 1 == FM ? stage : prev);
+          for (int c = 0; c < kB; ++c)
+            if (c * (FM - 1 - kMid) / kB == m - kMid) copy(1 + kA + c, kb + 2, stage);
+        }
+      } else { // the stage that the last barrier freed
+#pragma unroll
+        for (int c = 0; c < kStep; ++c) {
+          const int at = (m + 1 == FM ? 0 : m + 1) * kStep + c;
+          if (at < kCopies) copy(at, m + 1 == FM ? kb + ST : kb + ST - 1, m + 1 == FM ? stage : prev);
+        }
       }
       v4f d[FN];
 #pragma unroll
@@ -229,7 +259,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_fp8_tile_kernel(const Fp8Ge
 #pragma unroll
         for (int n = 0; n < FN; ++n) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          if (n < kStep) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+          if (kApart ? n + 2 == FN || (n + 1 == FN && m + 1 == FM) : n < kStep) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
           if (m + 1 == FM) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
           __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
         }
@@ -342,19 +372,19 @@ template <int DT> static int join_parts(const Fp8GemmArgs &a, hipStream_t stream
 }
 
 // Which tile, and how many parts of K: the smallest estimate of the time.  A K block takes a CU t1 us with one workgroup of the tile on it and
-// tn with as many as it holds (LDS); a workgroup starts and ends in `start` us; the parts are joined by a launch of kJoinUs that moves them
-// twice at kJoinBytes a us.  The figures are fitted to 67 sizes (17 to 8192 tokens, N 576 to 7168, K 256 to 7168), each timed with every
-// tile and 1 to 12 parts: the choice is 0.4 % off the fastest on average, 5 % at the most.  us, by the largest tile / by the
-// choice: 1531 x 7168 x 2048 30.2 / 26.9 (192 x 256), 723 x 7168 x 2048 26 / 18.6 (128 x 256), 490 x 7168 x 2048 25 / 13.9 (128 x
-// 128), 333 x 576 x 7168 50 / 12.8 (64 x 64, 4 parts), 48 x 7168 x 2048 24 / 7.6 (64 x 32).
+// tn_us with as many as it holds (LDS); a workgroup starts and ends in `start` us; the parts are joined by a launch of kJoinUs that moves
+// them twice at kJoinBytes a us.  The figures are fitted to 67 sizes (17 to 8192 tokens, N 576 to 7168, K 256 to 7168), each timed with
+// every tile and 1 to 8 parts: the choice is 0.1 % off the fastest on average, 2.4 % at the most.  us, by another tile / by the choice: 1531 x
+// 7168 x 2048 28.9 (256 x 256) / 25.0 (192 x 256), 726 x 7168 x 2048 22.6 (192 x 256) / 17.9 (128 x 256), 490 x 7168 x 2048 22.1 (192 x
+// 256) / 14.2 (128 x 128), 333 x 576 x 7168 18.9 (64 x 32, whole) / 12.9 (64 x 64, four parts), 48 x 7168 x 2048 9.4 (64 x 64) / 7.6 (64 x 32).
 struct Fp8Tile {
   int tm, tn, held;
   float t1, tn_us, start;
 };
 enum { kT256, kT192, kT128x256, kT128, kT64, kT64x32, kFp8Tiles };
-constexpr Fp8Tile kFp8Tile[kFp8Tiles] = {{256, 256, 1, 1.65f, 1.65f, 3.0f}, {192, 256, 1, 1.54f, 1.54f, 3.0f}, {128, 256, 1, 1.03f, 1.03f, 2.0f},
-                                         {128, 128, 1, 0.64f, 0.64f, 2.0f}, {64, 64, 2, 0.33f, 0.58f, 1.5f},   {64, 32, 3, 0.21f, 0.47f, 1.2f}};
-constexpr float kJoinUs = 2.9f, kJoinBytes = 4.7e6f;
+constexpr Fp8Tile kFp8Tile[kFp8Tiles] = {{256, 256, 1, 1.55f, 1.55f, 3.0f}, {192, 256, 1, 1.30f, 1.30f, 3.0f}, {128, 256, 1, 0.93f, 0.93f, 2.0f},
+                                         {128, 128, 1, 0.60f, 0.60f, 2.0f}, {64, 64, 2, 0.30f, 0.54f, 1.9f},   {64, 32, 3, 0.23f, 0.60f, 1.2f}};
+constexpr float kJoinUs = 3.2f, kJoinBytes = 4.7e6f;
 constexpr int kMostParts = 8, kLeastBlocks = 4; // of K, in a part
 struct Fp8Plan {
   int tile, parts;

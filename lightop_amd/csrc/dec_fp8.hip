@@ -121,6 +121,19 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
 // LDS of a wave: codes of kFewU K blocks, their scales, two lists of slots
 __host__ __device__ constexpr int few_wave_lds(int rows) { return kFewU * (rows * kGroup + 64) + 2 * kFewTokens * 2; }
 constexpr int kFewRed = 2048; // gate and up sums of a wave (up)
+// where `ends` is in LDS (down, with codes), behind everything else
+__host__ __device__ constexpr int few_down_ends(int waves, int per_wave, int parts, int slots, int units, int E) {
+  return (waves * per_wave + slots * (parts * 64 + 4 + 3 * 2) + (units + E) * 2 + 15) / 16 * 16;
+}
+// the sum of the lanes' numbers up to this one
+__device__ __forceinline__ int upto_lane(int v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
 
 // A unit is a slot where there are fewer slots than experts (the first of its expert's; the others' workgroups end), else an expert.
 template <int DT, int ACT, bool SMALL, bool CODES>
@@ -220,7 +233,7 @@ template <int DT, bool CODES>
 __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8ExpertsArgs a) {
   constexpr int U = CODES ? 2 : kFewU; // K blocks at a time (with codes, rows and weights take registers alike)
   // [wave] codes, scales, lists; [part][slot][column] results; [slot] weight; [slot] the token's first one with this expert, -1: none here;
-  // with codes: [slot] expert; the experts hit
+  // with codes: [slot] expert; the slots by expert; the experts hit; an expert's place among them; where the slots of each end
   extern __shared__ __attribute__((aligned(16))) int8_t smem[];
   __shared__ uint32_t present[CODES ? kFewExperts / 32 : 1];
   __shared__ int number;
@@ -233,7 +246,9 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
   float *const scales = reinterpret_cast<float *>(codes + kFewU * R * kGroup);
   int16_t *const lists = reinterpret_cast<int16_t *>(scales + kFewU * 16);
   float *const ys = reinterpret_cast<float *>(smem + waves * per), *const weight = ys + parts * pitch * 16;
-  int16_t *const from = reinterpret_cast<int16_t *>(weight + pitch), *const keys = from + pitch, *const hit = keys + pitch;
+  int16_t *const from = reinterpret_cast<int16_t *>(weight + pitch), *const keys = from + pitch, *const sorted = keys + pitch;
+  int16_t *const hit = sorted + pitch, *const place = hit + a.units;
+  int32_t *const ends = reinterpret_cast<int32_t *>(smem + few_down_ends(waves, per, parts, pitch, a.units, a.E));
   if constexpr (CODES)
     for (int i = tid; i < kFewExperts / 32; i += blockDim.x) present[i] = 0;
   const Route<!CODES> route(a, keys, lane, slot0, S);
@@ -258,52 +273,70 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
     }
     if (wave == 0) from[lane] = static_cast<int16_t>(mine);
   } else {
-    for (int s = tid; s < S; s += blockDim.x) {
-      const int e = keys[s];
-      int j = s / a.top_k * a.top_k;
-      while (j < s && keys[j] != e) ++j;
-      from[s] = static_cast<int16_t>(e < 0 ? -1 : j);
-      if (e >= 0) atomicOr(&present[e >> 5], 1u << (e & 31));
+    // every expert's slots, one a token, side by side (a slot a thread; their order within an expert, which the atomics leave open, says only
+    // which column of a product a token takes)
+    static_assert(kFewSlots <= kFewMaxWaves * 64, "a slot a thread");
+    const int e = tid < S ? keys[tid] : -1;
+    int j = tid / a.top_k * a.top_k;
+    if (e >= 0) {
+      while (keys[j] != e) ++j;
+      atomicOr(&present[e >> 5], 1u << (e & 31));
     }
+    if (tid < S) from[tid] = static_cast<int16_t>(e < 0 ? -1 : j);
     __syncthreads();
     if (wave == 0) {
       static_assert(kFewExperts / 32 == 64, "a word a lane");
       uint32_t left = present[lane];
-      int all = __popc(left); // of the lanes up to this one
-      const int own = all;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(all, d);
-        if (lane >= d) all += o;
+      const int own = __popc(left), upto = upto_lane(own, lane);
+      for (int at = upto - own; left; left &= left - 1, ++at) {
+        const int x = lane * 32 + __builtin_ctz(left);
+        hit[at] = static_cast<int16_t>(x);
+        place[x] = static_cast<int16_t>(at);
+        ends[at] = 0;
       }
-      for (int at = all - own; left; left &= left - 1) hit[at++] = static_cast<int16_t>(lane * 32 + __builtin_ctz(left));
-      if (lane == 63) number = all;
+      if (lane == 63) number = upto;
     }
     __syncthreads();
     experts = number;
+    const bool counts = e >= 0 && j == tid;
+    const int at = counts ? place[e] : 0, rank = counts ? atomicAdd(&ends[at], 1) : 0;
+    __syncthreads();
+    if (wave == 0)
+      for (int base = 0, before = 0; base < experts; base += 64) {
+        const int own = base + lane < experts ? ends[base + lane] : 0, upto = before + upto_lane(own, lane);
+        if (base + lane < experts) ends[base + lane] = upto;
+        before = __builtin_amdgcn_readlane(upto, 63);
+      }
+    __syncthreads();
+    if (counts) sorted[(at ? ends[at - 1] : 0) + rank] = static_cast<int16_t>(tid);
+    __syncthreads();
   }
 
   // The wave's work: (expert, part of K), of every `waves`-th, 16 of the expert's tokens at a time; up to U K blocks of them at a time, the next
   // ones' weights and rows asked for before these are used.
   const int items = experts * parts;
   struct Piece {
-    int it, e, part, count, f, kb, hi, list;
+    int it, e, part, count, f, kb, hi;
+    int list; // with codes where its slots begin in `sorted`, else which of the wave's lists
   };
   auto begin = [&](int it, int list) __attribute__((always_inline)) {
-    Piece p{it, 0, 0, 0, 0, 0, 0, list};
-    if (it >= items) return p;
+    Piece p{it, 0, 0, 0, 0, 0, 1, list};
+    if (it >= items) return p; // (loads of nothing, below)
     int at = it / parts;
     p.part = it - at * parts;
     if constexpr (CODES) {
       p.e = __builtin_amdgcn_readfirstlane(hit[at]);
+      p.list = at ? __builtin_amdgcn_readfirstlane(ends[at - 1]) : 0;
+      p.count = __builtin_amdgcn_readfirstlane(ends[at]) - p.list;
     } else {
       uint64_t left = leaders;
       for (; at > 0; --at) left &= left - 1;
       p.e = route.slot_expert(__builtin_ctzll(left));
+      p.list = list;
+      p.count = route.slots(p.e, -1, lists + list * kFewTokens);
     }
     p.kb = KB * p.part / parts;
     p.hi = KB * (p.part + 1) / parts;
-    p.count = route.slots(p.e, -1, lists + list * kFewTokens);
     return p;
   };
   auto next = [&](Piece p) __attribute__((always_inline)) {
@@ -325,10 +358,12 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
     const int kb = p.kb + g % U;
     load8<LO_F32>(a.act, static_cast<int64_t>(slot0 + lists[p.list * kFewTokens + g / U]) * I + (kb < p.hi ? kb : p.hi - 1) * kGroup + r * 8, v);
   };
+  // With codes the same number of loads on every path, past the last piece too (there the extents are empty): a wait for what was asked for a
+  // piece ago must not become one for what was asked for just now.
   auto load = [&](const Piece &p, int at) __attribute__((always_inline)) {
-    if (p.it >= items) return;
+    if (!CODES && p.it >= items) return;
     if constexpr (CODES) {
-      const int64_t slot = lists[p.list * kFewTokens + (p.f + r < p.count ? p.f + r : 0)];
+      const int64_t slot = p.count > 0 ? sorted[p.list + (p.f + r < p.count ? p.f + r : 0)] : 0;
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         const int kc = p.kb + k < p.hi ? p.kb + k : p.hi - 1;
@@ -339,7 +374,7 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
     } else if (q < p.count * U) {
       acts_at(p, q);
     }
-    const brsrc rW = make_rsrc(a.w2 + (static_cast<int64_t>(p.e) * a.H + n0) * I, static_cast<uint32_t>(16 * I));
+    const brsrc rW = make_rsrc(a.w2 + (static_cast<int64_t>(p.e) * a.H + n0) * I, p.it < items ? static_cast<uint32_t>(16 * I) : 0u);
     const float *const sw = a.w2s + (static_cast<int64_t>(p.e) * (a.H / kGroup) + n0 / kGroup) * KB;
 #pragma unroll
     for (int k = 0; k < U; ++k) {
@@ -373,8 +408,10 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s, acc[i]);
     }
-    if (p.kb + U >= p.hi && p.f + r < p.count)
-      *reinterpret_cast<v4f *>(ys + (p.part * pitch + lists[p.list * kFewTokens + p.f + r]) * 16 + 4 * q) = acc;
+    if (p.kb + U >= p.hi && p.f + r < p.count) {
+      const int slot = CODES ? sorted[p.list + p.f + r] : lists[p.list * kFewTokens + r];
+      *reinterpret_cast<v4f *>(ys + (p.part * pitch + slot) * 16 + 4 * q) = acc;
+    }
     lds_order();
   };
   Piece p = begin(wave, 0);
@@ -426,9 +463,10 @@ template <int DT, bool CODES> static int launch_down(Fp8ExpertsArgs a, hipStream
   // parts of K: what a wave has in flight at once, while the results fit LDS
   a.parts = (KB + kFewU - 1) / kFewU < kFewParts ? (KB + kFewU - 1) / kFewU : kFewParts;
   while (CODES && a.parts > 1 && a.parts * a.S > kFewSlots) --a.parts;
-  const int slots = CODES ? a.S : 64;
-  const int lds = kFewMaxWaves * few_wave_lds(a.rows) + slots * (a.parts * 64 + 6) + (CODES ? slots * 2 + a.E * 2 : 0);
-  constexpr int most = CODES ? kFewMaxWaves * few_wave_lds(0) + kFewSlots * (64 + 8) + kFewExperts * 2
+  const int per = few_wave_lds(a.rows), units = a.S < a.E ? a.S : a.E; // experts hit, at the most
+  a.units = units;
+  const int lds = CODES ? few_down_ends(kFewMaxWaves, per, a.parts, a.S, units, a.E) + units * 4 : kFewMaxWaves * per + 64 * (a.parts * 64 + 6);
+  constexpr int most = CODES ? few_down_ends(kFewMaxWaves, few_wave_lds(0), 1, kFewSlots, kFewSlots, kFewExperts) + kFewSlots * 4
                              : kFewMaxWaves * few_wave_lds(kFewGroup) + 64 * (kFewParts * 64 + 6);
   static_assert(most <= 160 * 1024 - 512, "LDS");
   const auto kernel = experts_fp8_down_kernel<DT, CODES>;

@@ -121,6 +121,9 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
 // LDS of a wave: codes of kFewU K blocks, their scales, two lists of slots
 __host__ __device__ constexpr int few_wave_lds(int rows) { return kFewU * (rows * kGroup + 64) + 2 * kFewTokens * 2; }
 constexpr int kFewRed = 2048; // gate and up sums of a wave (up)
+constexpr int kFewSums = 2048; // slots' sums of parts of K (down, with codes)
+// K blocks of a wave at a time (down; with codes, rows and weights take registers alike)
+__host__ __device__ constexpr int few_down_blocks(bool codes) { return codes ? 2 : kFewU; }
 // where `ends` is in LDS (down, with codes), behind everything else
 __host__ __device__ constexpr int few_down_ends(int waves, int per_wave, int parts, int slots, int units, int E) {
   return (waves * per_wave + slots * (parts * 64 + 4 + 3 * 2) + (units + E) * 2 + 15) / 16 * 16;
@@ -231,7 +234,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void e
 // a DeepSeek-V3 share 165 us), the routing in LDS.
 template <int DT, bool CODES>
 __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8ExpertsArgs a) {
-  constexpr int U = CODES ? 2 : kFewU; // K blocks at a time (with codes, rows and weights take registers alike)
+  constexpr int U = few_down_blocks(CODES);
   // [wave] codes, scales, lists; [part][slot][column] results; [slot] weight; [slot] the token's first one with this expert, -1: none here;
   // with codes: [slot] expert; the slots by expert; the experts hit; an expert's place among them; where the slots of each end
   extern __shared__ __attribute__((aligned(16))) int8_t smem[];
@@ -461,12 +464,13 @@ template <int DT, bool CODES> static int launch_down(Fp8ExpertsArgs a, hipStream
   a.group = CODES ? M : 64 / a.top_k < kFewGroup ? 64 / a.top_k : kFewGroup;
   a.rows = CODES ? 0 : M < a.group ? M : a.group;
   // parts of K: what a wave has in flight at once, while the results fit LDS
-  a.parts = (KB + kFewU - 1) / kFewU < kFewParts ? (KB + kFewU - 1) / kFewU : kFewParts;
-  while (CODES && a.parts > 1 && a.parts * a.S > kFewSlots) --a.parts;
+  constexpr int U = few_down_blocks(CODES);
+  a.parts = (KB + U - 1) / U < kFewParts ? (KB + U - 1) / U : kFewParts;
+  while (CODES && a.parts * a.S > kFewSums) --a.parts;
   const int per = few_wave_lds(a.rows), units = a.S < a.E ? a.S : a.E; // experts hit, at the most
   a.units = units;
   const int lds = CODES ? few_down_ends(kFewMaxWaves, per, a.parts, a.S, units, a.E) + units * 4 : kFewMaxWaves * per + 64 * (a.parts * 64 + 6);
-  constexpr int most = CODES ? few_down_ends(kFewMaxWaves, few_wave_lds(0), 1, kFewSlots, kFewSlots, kFewExperts) + kFewSlots * 4
+  constexpr int most = CODES ? few_down_ends(kFewMaxWaves, few_wave_lds(0), kFewSums / kFewSlots, kFewSlots, kFewSlots, kFewExperts) + kFewSlots * 4
                              : kFewMaxWaves * few_wave_lds(kFewGroup) + 64 * (kFewParts * 64 + 6);
   static_assert(most <= 160 * 1024 - 512, "LDS");
   const auto kernel = experts_fp8_down_kernel<DT, CODES>;

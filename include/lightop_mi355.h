@@ -626,9 +626,9 @@ int lo_gemm_w8a8_fp8_block(const void *a, const float *a_scale, const void *b, c
                            lo_stream_t stream);
 
 /*
- * The experts of a few tokens (M <= 64, top_k <= 64, M * top_k <= 1024) with e4m3 weights, in two launches (four beyond
- * 64 slots): e4m3 rows of x, first
- * product, act(gate) * up and its e4m3 codes, second product, weighted sum over a token's slots.
+ * The experts of a few tokens (M <= 64, top_k <= 64, M * top_k <= 1024) with e4m3 weights, in two launches (four where many
+ * experts are hit): e4m3 rows of x, first product, act(gate) * up and its e4m3 codes, second product, weighted sum over a
+ * token's slots.
  *   w1 [E, 2I, H], w2 [E, H, I] e4m3 row-major; w1s [E, 2I/128, H/128], w2s [E, H/128, I/128] fp32
  *   topk_w, topk_ids [M, top_k]; ids without an expert here (out of range, or no entry in expert_map) add nothing
  *   out[t] = routed_scaling_factor * sum_j topk_w[t, j] * y (+ shared_output[t]); out may be x or shared_output

@@ -1,4 +1,4 @@
-// The experts of a few tokens with e4m3 weights (128 x 128 blocks) in two launches, in four beyond 64 slots:
+// The experts of a few tokens with e4m3 weights (128 x 128 blocks) in two launches, or in four:
 //   h = xq w1[e]^T,  v = act(h[:I]) * h[I:],  y = vq w2[e]^T,  out[t] = factor * sum_j w[t, j] * y[t, e_j] (+ shared[t]),
 // xq and vq the e4m3 codes of rows in groups of 128 (fp8.h).  At these sizes the layer is a stream of the hit experts' weights:
 //   up     one workgroup per (expert hit, 16 columns of I).  Its waves share the K blocks of the 16 gate and 16 up rows and quantise their part
@@ -6,9 +6,8 @@
 //          on the way it would move codes of the second quantisation.
 //   down   one workgroup per 16 columns of the output.  Its waves share (expert hit, part of K) and leave each slot's 16 values in LDS;
 //          then every token's slots are added up in their order.  No atomics on results: the order of every sum is fixed.
-// Both find the experts hit from the ids by themselves.  The
-// first product is the exact one (fp8.h): the matrix cores have time, and an error of 1e-5 moves codes of the second quantisation; behind the
-// second one stands a rounding to 16 bits.
+// Both find the experts hit from the ids by themselves.  The first product is the exact one (fp8.h): the matrix cores have time, and an error
+// of 1e-5 moves codes of the second quantisation; behind the second one stands a rounding to 16 bits.
 // Ids that no expert of this rank answers to (out of range, or -1 in the map) add nothing.  An id that a token has twice is computed once
 // and counted with both weights.
 #include "gemm.h"
@@ -24,9 +23,15 @@ constexpr int kFewMaxWaves = 16; // (down)
 constexpr int kFewGroup = 8;     // tokens of a workgroup (down), at the most
 constexpr int kFewParts = 4;     // of the second product's K, at the most
 
-// Up to 64 slots in two launches, every workgroup quantising the rows that it needs; beyond, a launch in front of either product does it
-// once.
-static bool few_in_two(int64_t slots) { return slots <= 64; }
+// In two launches, every workgroup quantising the rows that it needs, or in four: a launch in front of either product does it once, and the
+// second product goes over all tokens at a time.  Two where few experts are hit (for ids that spread evenly: slots that stay here, at the most
+// every expert once), as far as a wave holds the slots in its lanes.  Two / four in us: Qwen3-30B-A3B, 16 experts hit 26.0 / 29.3, 24: 38.9 /
+// 38.4, 32: 49.0 / 46.2, 64: 77.8 / 69.0; a DeepSeek-V3 share (one of 8), 64 slots of which 8 stay 76 / 80.
+constexpr int kFewTwo = 24;
+static bool few_in_two(int64_t slots, int64_t experts, int64_t routed) {
+  const int64_t here = slots * experts / routed;
+  return slots <= 64 && (here < experts ? here : experts) < kFewTwo;
+}
 
 struct Fp8ExpertsArgs {
   const void *x, *ids, *shared;
@@ -483,7 +488,7 @@ template <int DT, bool CODES> static int launch_down(Fp8ExpertsArgs a, hipStream
 }
 template <int DT> static int launch_experts_fp8(Fp8ExpertsArgs a, int activation, hipStream_t stream) {
   const int M = a.S / a.top_k;
-  const bool gelu = activation == LO_ACT_GELU, small = few_in_two(a.S);
+  const bool gelu = activation == LO_ACT_GELU, small = few_in_two(a.S, a.E, a.Eg);
   // (rows that come as codes take no LDS)
   a.rows = !small ? 0 : M < 16 ? M : 16;
   int rc;
@@ -511,7 +516,7 @@ static FewLayout few_layout(int64_t M, int32_t top_k, int64_t H, int64_t I) {
   const int64_t S = M * top_k;
   FewLayout l{};
   l.total = S * I * 4;
-  if (few_in_two(S)) return l;
+  if (S < kFewTwo) return l; // (two launches, whatever the experts)
   const auto take = [&](int64_t bytes) {
     const int64_t at = l.total;
     l.total += (bytes + 15) / 16 * 16;

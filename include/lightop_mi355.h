@@ -626,7 +626,7 @@ int lo_gemm_w8a8_fp8_block(const void *a, const float *a_scale, const void *b, c
                            lo_stream_t stream);
 
 /*
- * The experts of a few tokens (M <= 64, top_k <= 64, M * top_k <= 1024) with e4m3 weights, in two launches (four where many
+ * The experts of a few tokens (M <= 64, top_k <= 64, M * top_k <= 1024) with e4m3 weights, in two launches (four or five where many
  * experts are hit): e4m3 rows of x, first product, act(gate) * up and its e4m3 codes, second product, weighted sum over a
  * token's slots.
  *   w1 [E, 2I, H], w2 [E, H, I] e4m3 row-major; w1s [E, 2I/128, H/128], w2s [E, H/128, I/128] fp32

@@ -5,7 +5,8 @@
 //          of the token rows into LDS while the weights are on their way; the sums meet in LDS.  v goes to the workspace in fp32: rounded
 //          on the way it would move codes of the second quantisation.
 //   down   one workgroup per 16 columns of the output.  Its waves share (expert hit, part of K) and leave each slot's 16 values in LDS;
-//          then every token's slots are added up in their order.  No atomics on results: the order of every sum is fixed.
+//          then every token's slots are added up in their order, by the experts' halves where two workgroups share them (few_split).  No
+//          atomics on results: the order of every sum is fixed.
 // Both find the experts hit from the ids by themselves.  The first product is the exact one (fp8.h): the matrix cores have time, and an error
 // of 1e-5 moves codes of the second quantisation; behind the second one stands a rounding to 16 bits.
 // Ids that no expert of this rank answers to (out of range, or -1 in the map) add nothing.  An id that a token has twice is computed once
@@ -25,9 +26,12 @@ constexpr int kFewParts = 4;     // of the second product's K, at the most
 
 // In two launches, every workgroup quantising the rows that it needs, or in four: a launch in front of either product does it once, and the
 // second product goes over all tokens at a time.  Two where few experts are hit (for ids that spread evenly: slots that stay here, at the most
-// every expert once), as far as a wave holds the slots in its lanes.  Two / four in us: Qwen3-30B-A3B, 16 experts hit 26.0 / 29.3, 24: 38.9 /
-// 38.4, 32: 49.0 / 46.2, 64: 77.8 / 69.0; a DeepSeek-V3 share (one of 8), 64 slots of which 8 stay 76 / 80.
+// every expert once), as far as a wave holds the slots in its lanes.  Two / four in us: Qwen3-30B-A3B, 16 experts hit 26 / 28, 24: 39 / 37,
+// 32: 49 / 43, 64: 78 / 61; a DeepSeek-V3 share (one of 8), 64 slots of which 8 stay 76 / 80.
 constexpr int kFewTwo = 24;
+// Where the four launches' second product has fewer workgroups of 16 columns than there are CUs, two share a column block's experts and a fifth
+// launch joins them: 64 tokens of Qwen3-30B-A3B (H 2048) 132 us, with one workgroup 159, with three 151, with four 142 (one fits a CU).
+static int few_split(int64_t H) { return H / 16 < 256 ? 2 : 1; }
 static bool few_in_two(int64_t slots, int64_t experts, int64_t routed) {
   const int64_t here = slots * experts / routed;
   return slots <= 64 && (here < experts ? here : experts) < kFewTwo;
@@ -42,9 +46,11 @@ struct Fp8ExpertsArgs {
   float *act;       // [slots, I]
   const int8_t *xq, *aq; // CODES: rows of x [tokens, H] and of act [slots, I], and their scales
   const float *xs, *as;
+  float *part;           // [split, tokens, H]: outputs, of the experts of one of `split` workgroups each (down)
   int32_t S, H, I, E, Eg, top_k, units, parts;
   int32_t rows;     // of a wave's codes: tokens that an expert may have at a time
   int32_t group;    // tokens of a workgroup (down)
+  int32_t split;    // workgroups that share the experts of 16 columns (down, with codes)
   float factor;
   bool ids64, by_slot;
 };
@@ -248,7 +254,7 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n0 = blockIdx.x * 16, I = a.I, KB = I / kGroup, R = a.rows, per = few_wave_lds(R), parts = a.parts;
-  const int first = CODES ? 0 : blockIdx.y * a.group, M = a.S / a.top_k - first < a.group ? a.S / a.top_k - first : a.group;
+  const int share = blockIdx.y, first = CODES ? 0 : blockIdx.y * a.group, M = a.S / a.top_k - first < a.group ? a.S / a.top_k - first : a.group;
   const int S = M * a.top_k, slot0 = first * a.top_k, pitch = CODES ? S : 64; // of the group
   int8_t *const codes = smem + wave * per;
   float *const scales = reinterpret_cast<float *>(codes + kFewU * R * kGroup);
@@ -305,14 +311,15 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
       if (lane == 63) number = upto;
     }
     __syncthreads();
-    experts = number;
+    experts = (number - share + a.split - 1) / a.split; // every split-th of those hit
     const bool counts = e >= 0 && j == tid;
-    const int at = counts ? place[e] : 0, rank = counts ? atomicAdd(&ends[at], 1) : 0;
+    const int at = e >= 0 ? place[e] : 0, rank = counts ? atomicAdd(&ends[at], 1) : 0;
+    if (e >= 0 && at % a.split != share) from[tid] = -1;
     __syncthreads();
     if (wave == 0)
-      for (int base = 0, before = 0; base < experts; base += 64) {
-        const int own = base + lane < experts ? ends[base + lane] : 0, upto = before + upto_lane(own, lane);
-        if (base + lane < experts) ends[base + lane] = upto;
+      for (int base = 0, before = 0; base < number; base += 64) {
+        const int own = base + lane < number ? ends[base + lane] : 0, upto = before + upto_lane(own, lane);
+        if (base + lane < number) ends[base + lane] = upto;
         before = __builtin_amdgcn_readlane(upto, 63);
       }
     __syncthreads();
@@ -333,6 +340,7 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
     int at = it / parts;
     p.part = it - at * parts;
     if constexpr (CODES) {
+      at = at * a.split + share;
       p.e = __builtin_amdgcn_readfirstlane(hit[at]);
       p.list = at ? __builtin_amdgcn_readfirstlane(ends[at - 1]) : 0;
       p.count = __builtin_amdgcn_readfirstlane(ends[at]) - p.list;
@@ -446,10 +454,32 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
       for (int k = 0; k < parts; ++k) y += ys[(k * pitch + s) * 16 + c];
       sum = __builtin_fmaf(weight[s0 + j], y, sum);
     }
+    if (CODES && a.split > 1) {
+      a.part[(static_cast<int64_t>(share) * M + t) * a.H + n0 + c] = sum;
+      continue;
+    }
     sum *= a.factor;
     const int64_t at = static_cast<int64_t>(first + t) * a.H + n0 + c;
     if (a.shared) sum += o == tid ? shared : to_f32<DT>(static_cast<const uint16_t *>(a.shared)[at]);
     static_cast<uint16_t *>(a.out)[at] = from_f32<DT>(sum);
+  }
+}
+
+template <int DT> __global__ __launch_bounds__(256) void experts_fp8_join_kernel(const Fp8ExpertsArgs a, int64_t pieces) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= pieces) return;
+  float sum[8], v[8];
+  load8<LO_F32>(a.part, i * 8, sum);
+  for (int k = 1; k < a.split; ++k) {
+    load8<LO_F32>(a.part, (k * pieces + i) * 8, v);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) sum[n] += v[n];
+  }
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    sum[n] *= a.factor;
+    if (a.shared) sum[n] += to_f32<DT>(static_cast<const uint16_t *>(a.shared)[i * 8 + n]);
+    static_cast<uint16_t *>(a.out)[i * 8 + n] = from_f32<DT>(sum[n]);
   }
 }
 
@@ -482,8 +512,14 @@ template <int DT, bool CODES> static int launch_down(Fp8ExpertsArgs a, hipStream
   static unsigned long long done = 0;
   const int rc = reserve_lds_once(reinterpret_cast<const void *>(kernel), most, &done);
   if (rc) return rc;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.H / 16), static_cast<unsigned>((M + a.group - 1) / a.group)), dim3(kFewMaxWaves * 64), lds,
-                     stream, a);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.H / 16), static_cast<unsigned>(CODES ? a.split : (M + a.group - 1) / a.group)),
+                     dim3(kFewMaxWaves * 64), lds, stream, a);
+  if (CODES && a.split > 1) {
+    const int rc = check_launch("fused_experts_fp8");
+    if (rc) return rc;
+    const int64_t pieces = static_cast<int64_t>(M) * a.H / 8;
+    hipLaunchKernelGGL(experts_fp8_join_kernel<DT>, dim3(static_cast<unsigned>((pieces + 255) / 256)), dim3(256), 0, stream, a, pieces);
+  }
   return check_launch("fused_experts_fp8");
 }
 template <int DT> static int launch_experts_fp8(Fp8ExpertsArgs a, int activation, hipStream_t stream) {
@@ -510,7 +546,7 @@ template <int DT> static int launch_experts_fp8(Fp8ExpertsArgs a, int activation
 
 namespace lo {
 struct FewLayout { // of the workspace: activations; beyond two launches codes and scales of the rows and of the activations
-  int64_t xq, xs, aq, as, total;
+  int64_t xq, xs, aq, as, part, total;
 };
 static FewLayout few_layout(int64_t M, int32_t top_k, int64_t H, int64_t I) {
   const int64_t S = M * top_k;
@@ -526,6 +562,7 @@ static FewLayout few_layout(int64_t M, int32_t top_k, int64_t H, int64_t I) {
   l.xs = take(M * (H / kGroup) * 4);
   l.aq = take(S * I);
   l.as = take(S * (I / kGroup) * 4);
+  l.part = take(few_split(H) > 1 ? few_split(H) * M * H * 4 : 0);
   return l;
 }
 } // namespace lo
@@ -572,6 +609,8 @@ extern "C" int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t
   a.xs = reinterpret_cast<float *>(ws + layout.xs);
   a.aq = reinterpret_cast<int8_t *>(ws + layout.aq);
   a.as = reinterpret_cast<float *>(ws + layout.as);
+  a.part = reinterpret_cast<float *>(ws + layout.part);
+  a.split = few_split(H);
   a.S = static_cast<int32_t>(M * top_k); a.H = static_cast<int32_t>(H); a.I = static_cast<int32_t>(I);
   a.E = E; a.Eg = num_experts; a.top_k = top_k; a.factor = routed_scaling_factor;
   a.ids64 = ids_dtype == LO_I64;

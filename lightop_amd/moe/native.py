@@ -637,7 +637,7 @@ def fused_experts_decode_fp8(hidden_states: torch.Tensor,
                              shared_output: Optional[torch.Tensor] = None,
                              inplace: bool = False) -> torch.Tensor:
     """The routed experts of a decode batch (at most 64 tokens, 64 slots a token and 1024 in all) with e4m3 weights, in two
-    launches, or four where many experts are hit.
+    launches, or four to five where many experts are hit.
 
     ``hidden_states`` [M, H] bf16 or fp16; ``w1`` [E, 2I, H], ``w2`` [E, H, I] float8_e4m3fn, row-major as a checkpoint holds them,
     with one fp32 scale for 128 x 128: ``w1_scale`` [E, 2I/128, H/128], ``w2_scale`` [E, H/128, I/128].  Rows are quantised in front

@@ -595,7 +595,8 @@ enum { LO_Q_INT8_ROWS = 0, LO_Q_INT8_GROUPS = 1, LO_Q_FP8_GROUPS = 2 };
  *   z = x + residual, y = z * (mean(z^2) + eps)^-1/2 * weight, in fp32
  *   x, residual [M, H] rows of `dtype` x_stride / residual_stride values apart (multiples of 16 bytes); residual may be NULL
  *   weight [H] of `dtype` or LO_F32;  M >= 0, H <= 65536, a multiple of 128 (LO_Q_INT8_ROWS: of 8)
- *   residual_out [M, H]: z rounded once; may be x or residual itself where that is contiguous.  Not written without residual
+ *   residual_out [M, H]: z rounded once; may be x or residual itself where that is contiguous, and must not overlap them
+ *   otherwise.  Not written without residual
  *   normed_out [M, H] or NULL: y rounded once;  q [M, H], scale: codes of the fp32 y
  *   q_form  LO_Q_INT8_ROWS: scale [M], the rule of lo_per_token_quant_int8
  *           LO_Q_INT8_GROUPS: scale [M, H/128], the rule of lo_per_token_group_quant_int8 (eps 1e-10)

@@ -174,6 +174,14 @@ extern "C" int lo_rms_norm_quant(const void *x, int dtype, int64_t x_stride, con
   LO_REQUIRE(!off(x, 16) && !off(residual, 16) && !off(weight, 16) && !off(residual_out, 16) && !off(normed_out, 16) && !off(q, 8) &&
                  !off(scale, 4),
              LO_EINVAL, "rms_norm_quant: rows and weight must be 16-byte, q 8-byte aligned");
+  // the sum may take the place of a whole input, row by row; a row of it over another input row would be read too late
+  const int64_t size = dtype == LO_F32 ? 4 : 2;
+  const auto over = [&](const void *in, int64_t stride) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(in), z = reinterpret_cast<uintptr_t>(residual_out);
+    return residual && !(p == z && (stride == H || M == 1)) && p < z + M * H * size && z < p + ((M - 1) * stride + H) * size;
+  };
+  LO_REQUIRE(!over(x, x_stride) && !over(residual, residual_stride), LO_EINVAL,
+             "rms_norm_quant: residual_out overlaps an input without being it");
   NormArgs a{x, residual, weight, residual_out, normed_out, static_cast<int8_t *>(q), scale, x_stride, residual_stride,
              static_cast<int32_t>(H), weight_dtype == LO_F32, 0, eps};
   hipStream_t s = static_cast<hipStream_t>(stream);

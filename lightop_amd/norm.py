@@ -46,7 +46,8 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, res
 
     ``x`` bf16, fp16 or fp32 of any leading shape (rows may be strided), ``weight`` of its type or fp32.  The sum comes back
     in ``residual`` in x's type, in ``residual_out`` where the caller brings one (contiguous; ``residual`` itself updates it
-    in place), None without a residual; with ``return_normed`` the normed rows in x's type come back too."""
+    in place; any other overlap with an input is refused), None without a residual; with ``return_normed`` the normed rows in
+    x's type come back too."""
     form = _FORMS.get((quant_dtype, group_size))
     if form is None:
         raise RuntimeError("rms_norm_quant: built for int8 with group_size None or 128 and float8_e4m3fn with 128, "

@@ -130,3 +130,10 @@ def test_names_are_reachable():
     assert lightop.norm.rms_norm_quant is lightop_amd.norm.rms_norm_quant is lightop.rms_norm_quant
     assert lightop.moe.fused_experts_decode_fp8 is lightop_amd.moe.fused_experts_decode_fp8
     assert lightop.gemmopt.gemm_w8a8_fp8_block and lightop.quant.per_token_group_quant_fp8
+
+
+@pytest.mark.parametrize("bad", [dict(z=P + 512), dict(z=P - 512), dict(x=P + 512, r=P + 1024 * 1024, z=P), dict(x=P + 1024 * 1024, r=P + 16, z=P),
+                                 dict(xs=512), dict(rs=512), dict(M=1, z=P + 16), dict(dtype=2, wt=2, z=P + 1024)], ids=str)
+def test_norm_refuses_a_sum_over_other_rows(lib, bad):
+    assert _norm(lib, **bad) < 0
+    assert b"overlaps" in lib.lo_last_error()

@@ -220,3 +220,85 @@ def test_streams_and_graphs():
         torch.cuda.synchronize()
         assert torch.equal(graphs[0][2], want[r % 3]) and torch.equal(graphs[1][2], want[(r + 1) % 3])
         assert torch.equal(other, want[r % 3]) and torch.equal(here, want[(r + 1) % 3])
+
+
+@pytest.mark.parametrize("M,k,E", [(16, 64, 2048), (1, 64, 64), (1, 64, 2048), (64, 1, 2048), (64, 16, 2048), (13, 2, 24), (12, 2, 25), (64, 1, 1)])
+def test_limits(M, k, E):
+    """The most tokens, slots, slots a token and experts, and both sides of the step from two launches to four."""
+    print("[case] experts", M, k, E, flush=True)
+    w = _layer(E, 128, 128)
+    x, tw, ids, shared = _tokens(M, 128, E, k, torch.bfloat16)
+    _check(x, w, tw, ids, shared=shared)
+
+
+@pytest.mark.parametrize("M,E,k,H,I", [(16, 26, 4, 4096, 256), (64, 26, 3, 4224, 128), (30, 30, 6, 2048, 1152), (64, 8, 16, 256, 1024)])
+def test_widths_of_many_experts_hit(M, E, k, H, I):
+    """Column blocks of one workgroup (4096 columns up) and of two; parts of K of unequal lengths, and as many as the sums' room allows."""
+    print("[case] experts", M, E, k, H, I, flush=True)
+    w = _layer(E, H, I)
+    x, tw, ids, shared = _tokens(M, H, E, min(k, E), torch.float16)
+    if k > E:
+        ids, tw = ids.repeat(1, 2)[:, :k].contiguous(), tw.repeat(1, 2)[:, :k].contiguous()
+    a = _check(x, w, tw, ids, shared=shared, factor=0.5)
+    for _ in range(4):  # the same bits every time
+        assert torch.equal(_run(x, w, tw, ids, shared=shared, factor=0.5)[0], a)
+
+
+@pytest.mark.parametrize("M", [3, 48])
+def test_nans_and_infinities_stay_where_they_are(M):
+    w = _layer(32, 512, 256)
+    x, tw, ids, shared = _tokens(M, 512, 32, 4, torch.bfloat16)
+    want = _run(x, w, tw, ids, shared=shared)[0]
+    bad, bw, bi = x.clone(), tw.clone(), ids.clone()
+    bad[1, 7], bad[2, 300] = float("nan"), float("inf")
+    out = _run(bad, w, tw, ids, shared=shared)[0]
+    keep = [t for t in range(M) if t not in (1, 2)]
+    assert torch.equal(out[keep], want[keep]) and not out[1].isfinite().any() and not out[2].isfinite().any()
+    bi[:, 3], bw[:, 3] = -1, 0.0
+    none = _run(x, w, bw, bi, shared=shared)[0]
+    for v in (float("nan"), float("inf")):  # weights of slots without an expert are not looked at
+        bw[:, 3] = v
+        assert torch.equal(_run(x, w, bw, bi, shared=shared)[0], none)
+
+
+@pytest.mark.parametrize("M,H", [(40, 1024), (20, 4096)])
+def test_streams_graphs_and_threads_of_many_slots(M, H):
+    """Two captured graphs, a thread on a stream of its own, another one on this one's stream: each with its own scratch, or in turn."""
+    import threading
+
+    from lightop_amd.moe import fused_experts_decode_fp8
+
+    w1, w2, s1, s2 = _layer(24, H, 256)
+    sets = [_tokens(M, H, 24, 4, torch.bfloat16, seed=i) for i in range(3)]
+    f = lambda x, tw, ids, sh: fused_experts_decode_fp8(x, w1, w2, tw, ids, s1, s2, shared_output=sh)
+    want = [f(*s) for s in sets]
+    graphs = []
+    for i in range(2):
+        hold = [t.clone() for t in sets[i]]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = f(*hold)
+        graphs.append((graph, hold, out))
+    torch.cuda.synchronize()
+    main, made = torch.cuda.current_stream(), {}
+
+    def work(name, stream):
+        with torch.cuda.stream(stream):
+            made[name] = [f(*sets[i % 3]) for i in range(30)]
+            stream.synchronize()
+
+    for r in range(3):
+        threads = [threading.Thread(target=work, args=("own", torch.cuda.Stream())), threading.Thread(target=work, args=("same", main))]
+        for t in threads:
+            t.start()
+        for i, (graph, hold, out) in enumerate(graphs):
+            for h, t in zip(hold, sets[(r + i) % 3]):
+                h.copy_(t)
+            graph.replay()
+        here = [f(*sets[i % 3]) for i in range(30)]
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert torch.equal(graphs[0][2], want[r % 3]) and torch.equal(graphs[1][2], want[(r + 1) % 3])
+        for outs in (made["own"], made["same"], here):
+            assert all(torch.equal(o, want[i % 3]) for i, o in enumerate(outs))

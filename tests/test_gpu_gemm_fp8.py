@@ -179,3 +179,32 @@ def test_without_room_for_parts(M, N, K, dtype):
         _check(out, a, b, sa, sb)
         outs.append(out)
     assert (room[need:] == 0xff).all()
+
+
+def test_threads():
+    """Sizes whose parts go through scratch, from two threads on one stream and one on another."""
+    import threading
+
+    from lightop_amd.gemmopt import gemm_w8a8_fp8_block
+
+    sets = [_make(n, 576, 7168) for n in (60, 333)]
+    want = [gemm_w8a8_fp8_block(a, b, sa, sb) for a, b, sa, sb in sets]
+    torch.cuda.synchronize()
+    made = {}
+
+    def work(name, stream):
+        with torch.cuda.stream(stream):
+            made[name] = []
+            for i in range(40):
+                a, b, sa, sb = sets[i % 2]
+                made[name].append(gemm_w8a8_fp8_block(a, b, sa, sb))
+            stream.synchronize()
+
+    main = torch.cuda.current_stream()
+    threads = [threading.Thread(target=work, args=(n, s)) for n, s in (("own", torch.cuda.Stream()), ("same", main), ("too", main))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for outs in made.values():
+        assert len(outs) == 40 and all(torch.equal(o, want[i % 2]) for i, o in enumerate(outs))

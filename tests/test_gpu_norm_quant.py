@@ -182,3 +182,14 @@ def test_streams_and_graphs():
         eager = rms_norm_quant(y, w, residual=r)
         torch.cuda.synchronize()
         assert all(torch.equal(u, v) for u, v in zip(out[:3], eager[:3]))
+
+
+def test_a_sum_over_other_rows_is_refused():
+    from lightop_amd.norm import rms_norm_quant
+
+    buf = torch.zeros(6, 256, dtype=torch.bfloat16, device="cuda")
+    x, _, w = _make(5, 256, torch.bfloat16, False)
+    for out in (buf[:5], buf[1:]):
+        rms_norm_quant(x, w, residual=out, residual_out=out)
+        with pytest.raises(RuntimeError, match="overlaps"):
+            rms_norm_quant(x, w, residual=buf[1:] if out.data_ptr() == buf.data_ptr() else buf[:5], residual_out=out)

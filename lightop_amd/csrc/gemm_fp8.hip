@@ -2,7 +2,8 @@
 //   C[m, n] = sum over kb of (A[m, kb] . B[n, kb]) * As[m, kb] * Bs[n / 128, kb],
 // A [M, K] rows with one scale for 128 values, B [N, K] a weight with one for 128 x 128.  A K block's 128 products are one MFMA
 // (v_mfma_f32_16x16x128_f8f6f4, which starts from zero), its fp32 result is folded into the fp32 sum with the scales' product.
-// (An fp32 output takes the exact form of it, fp8.h.)  Weights are the A operand: a lane holds four neighbouring columns of C for one token, whose scale it carries.
+// (An fp32 output takes the exact form of it, fp8.h.)  Weights are the A operand: a lane holds four neighbouring columns of C for one token,
+// whose scale it carries.
 #include "gemm.h"
 #include "fp8.h"
 
@@ -24,7 +25,8 @@ template <int DT> __device__ __forceinline__ void store_c(void *c, int64_t at, f
 
 // ---- up to 16 tokens ---------------------------------------------------------------------------------------------------------
 // A workgroup takes 16 columns and all tokens; its waves share the K blocks and add their sums up through LDS, in the same order every time.
-// Weights are read once, straight into registers, four K blocks of a wave in flight.
+// Weights are read once, straight into registers, four K blocks of a wave in flight: HBM and the launch bound it (1 x 4096 x 7168: 29 MB in
+// 8.3 us).  Rows past the tokens are past the extents and read as zeros.
 template <int DT>
 __global__ __launch_bounds__(1024) void gemm_fp8_few_kernel(const Fp8GemmArgs a) {
   __shared__ __attribute__((aligned(16))) float red[16][256]; // [wave][token][column]
@@ -84,10 +86,17 @@ __device__ __forceinline__ bool dense_tile(int bid, int m_tiles, int n_tiles, in
 
 // ---- tiles -----------------------------------------------------------------------------------------------------------------
 // Both operands go to LDS by direct loads, a K block to a stage of a ring of ST; 16-byte pieces of a row are swizzled by the row.  The rows'
-// scales go there four K blocks at a time (a scale is a line of its own to the texture path, whatever it fetches of it).  A wave keeps its weight fragments of a K block in registers and walks through its token fragments, a step each:
-// the next token fragment is read while this one is multiplied and the one before is folded.  The workgroup meets in front of the last
-// step, when nobody reads the K block's stage any more: behind the barrier the next block's first operands are read under the step's
-// products, and the copies of the block that takes the stage over are asked for, a few a step.
+// scales go there four K blocks at a time (a scale is a line of its own to the texture path, whatever it fetches of it).  A wave keeps its
+// weight fragments of a K block in registers and walks through its token fragments, a step each: the next token fragment is read while this
+// one is multiplied and the one before is folded.  The workgroup meets in front of the last step, when nobody reads the K block's stage any
+// more: behind the barrier the next block's first operands are read under the step's products, and the copies of the block that takes the
+// stage over are asked for, a few a step.
+//
+// 8192 x 4096 x 7168 in 256 x 256 tiles, two stages: 199 us, 2.4 PFLOP/s (the library's product of 8192^3 without block scales 2.78).  The K
+// loop is bound by the MFMAs with the fold's vector instructions between them, and by the clock, 1.7 GHz under that load.  Freeing the
+// weights' and the tokens' half of a stage apart took it from 217 us; other orders of the copies, s_setprio and groups of 8 token tiles to an
+// XCD gained nothing.  Middle sizes lose to their last round of workgroups, narrow ones to a step's latency: rings of six and eight stages
+// (64 x 64, 64 x 32) and an XCD to each part of K are no faster (333 x 576 x 7168 13.1 / 13.3 us, 48 x 7168 x 2048 8.0 / 8.0).
 __device__ __forceinline__ void copy16(brsrc r, int8_t *lds, int voff, int soff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 16, voff, soff, 0, 0);
 }
@@ -429,7 +438,8 @@ template <int DT, int TM, int TN, int WM, int WN, int ST> static int launch_tile
   }
 }
 template <int DT> static int launch_gemm_fp8(const Fp8GemmArgs &a, int64_t part_bytes, hipStream_t stream) {
-  if (a.M <= 16) { // us, this / the tiles: 1 x 4096 x 7168 9.1 / 11.5, 16: 11.2 / 12.1, 16 x 7168 x 2048 7.4 / 7.4; 32 tokens in two fragments 15.7 / 12.3
+  // us, this / the tiles: 1 x 4096 x 7168 9.1 / 11.5, 16: 11.2 / 12.1, 16 x 7168 x 2048 7.4 / 7.4; 32 tokens in two fragments 15.7 / 12.3
+  if (a.M <= 16) {
     const int waves = a.KB >= 16 ? 16 : a.KB >= 8 ? 8 : 4;
     hipLaunchKernelGGL((gemm_fp8_few_kernel<DT>), dim3(static_cast<unsigned>((a.N + 15) / 16)), dim3(waves * 64), 0, stream, a);
     return LO_OK;

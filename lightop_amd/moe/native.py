@@ -4,13 +4,14 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import threading
 from typing import Any, Dict, List, Optional, Tuple
 
 import torch
 
 from .. import _lib, envs
 from ..gemmopt import moe_gemm_w8a8
-from ..op import _act_dtype, _float_dtype, _ids_dtype, _on_device, _one_device, _require_cuda, _rows16, _scratch
+from ..op import _act_dtype, _float_dtype, _ids_dtype, _on_device, _one_device, _require_cuda, _rows16
 
 
 # forms of a whole-path call, as csrc/host_binding.cpp numbers them
@@ -705,6 +706,49 @@ def fused_experts_decode_fp8(hidden_states: torch.Tensor,
 def _workspace_bytes_cached(M: int, top_k: int, H: int, I: int, num_experts: int) -> int:
     return fused_experts_workspace_bytes(M, top_k, H, I, num_experts, 0)
 
+
+_capture_lock = threading.Lock()
+_capture_seen: Tuple[Tuple[int, int], bool] = ((-1, 0), False)  # ((device, capture id), whether the graph owns what it allocates)
+_capture_kept: Dict[Tuple[int, int], List[torch.Tensor]] = {}
+
+
+def _scratch(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
+    """Scratch of one call that is marshalled here: from the caching allocator, back to it when the call's launches are
+    queued, and reused in the stream's order.
+
+    A captured call's scratch has to outlive the call, since every replay writes to it.  ``torch.cuda.graph`` sees to
+    that: what is allocated under it comes from memory that belongs to the graph (and to the graphs that share its pool)
+    until the graph is gone.  A capture that the allocator knows nothing of, begun with hipStreamBeginCapture on
+    an external stream, has no such memory: its scratch is kept for good, one piece per (device, stream) and the ones it
+    outgrew."""
+    def new():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+    if not torch.cuda.is_current_stream_capturing():
+        return new()
+    global _capture_seen
+    with _capture_lock:
+        at = (device.index, _lib.capture_id(stream))
+        if _capture_seen[0] != at:  # once per capture: a snapshot lists every block of the process
+            _capture_seen = (at, _in_graph_pool(new()))
+        if _capture_seen[1]:
+            return new()
+        kept = _capture_kept.setdefault((device.index, stream), [])
+        if not kept or kept[-1].numel() < nbytes:
+            kept.append(new())
+        return kept[-1]
+
+
+def _in_graph_pool(t: torch.Tensor) -> bool:
+    """Whether the allocator took ``t`` from a private pool, as it does under ``torch.cuda.graph``.  False where it cannot
+    say: what is kept without need costs memory, what is not kept would be written to by replays."""
+    try:
+        for seg in torch.cuda.memory_snapshot():
+            if seg["device"] == t.device.index and seg["address"] <= t.data_ptr() < seg["address"] + seg["total_size"]:
+                return tuple(seg["segment_pool_id"]) != (0, 0)
+    except (RuntimeError, KeyError):  # another allocator behind torch's, another layout of its snapshot
+        pass
+    return False
 
 def _run_fused_experts(hidden_states, w1, w2, topk_weights, topk_ids, cache13, inplace, apply_router_weight_on_input,
                        global_num_experts, expert_map, w1_scale, w2_scale, routed_scaling_factor, shared_output,

@@ -5,8 +5,7 @@ fused-MoE path, its per-channel form and the two routers that feed it exist here
 from __future__ import annotations
 
 import contextlib
-import threading
-from typing import Dict, List, Optional, Tuple
+from typing import Optional
 
 import torch
 
@@ -39,50 +38,6 @@ def _on_device(t: torch.Tensor):
     else:
         with torch.cuda.device(t.device):
             yield
-
-
-_capture_lock = threading.Lock()
-_capture_seen: Tuple[Tuple[int, int], bool] = ((-1, 0), False)  # ((device, capture id), whether the graph owns what it allocates)
-_capture_kept: Dict[Tuple[int, int], List[torch.Tensor]] = {}
-
-
-def _scratch(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
-    """Scratch of one call that is marshalled here: from the caching allocator, back to it when the call's launches are
-    queued, and reused in the stream's order.
-
-    A captured call's scratch has to outlive the call, since every replay writes to it.  ``torch.cuda.graph`` sees to
-    that: what is allocated under it comes from memory that belongs to the graph (and to the graphs that share its pool)
-    until the graph is gone.  A capture that the allocator knows nothing of, begun with hipStreamBeginCapture on
-    an external stream, has no such memory: its scratch is kept for good, one piece per (device, stream) and the ones it
-    outgrew."""
-    def new():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-
-    if not torch.cuda.is_current_stream_capturing():
-        return new()
-    global _capture_seen
-    with _capture_lock:
-        at = (device.index, _lib.capture_id(stream))
-        if _capture_seen[0] != at:  # once per capture: a snapshot lists every block of the process
-            _capture_seen = (at, _in_graph_pool(new()))
-        if _capture_seen[1]:
-            return new()
-        kept = _capture_kept.setdefault((device.index, stream), [])
-        if not kept or kept[-1].numel() < nbytes:
-            kept.append(new())
-        return kept[-1]
-
-
-def _in_graph_pool(t: torch.Tensor) -> bool:
-    """Whether the allocator took ``t`` from a private pool, as it does under ``torch.cuda.graph``.  False where it cannot
-    say: what is kept without need costs memory, what is not kept would be written to by replays."""
-    try:
-        for seg in torch.cuda.memory_snapshot():
-            if seg["device"] == t.device.index and seg["address"] <= t.data_ptr() < seg["address"] + seg["total_size"]:
-                return tuple(seg["segment_pool_id"]) != (0, 0)
-    except (RuntimeError, KeyError):  # another allocator behind torch's, another layout of its snapshot
-        pass
-    return False
 
 
 def _ids_dtype(t: torch.Tensor) -> int:

@@ -178,11 +178,12 @@ def host():
                           "time; build it with `python -m lightop_amd.build`", RuntimeWarning, stacklevel=3)
             _host = _NoHost()
             return _host
-        mod.bind(*(ctypes.cast(getattr(handle, n), c_void_p).value for n in (
-            "lo_fused_experts_block_int8", "lo_fused_experts_channel_int8", "lo_fused_experts_workspace_bytes",
-            "lo_topk_softmax", "lo_moe_fused_gate", "lo_last_error", "lo_rms_norm_quant", "lo_per_token_group_quant_fp8",
-            "lo_act_mul_group_quant_fp8", "lo_gemm_w8a8_fp8_block", "lo_fused_experts_fp8",
-            "lo_fused_experts_fp8_workspace_bytes", "lo_gemm_w8a8_fp8_block_workspace_bytes")))
+        for bind, names in ((mod.bind, ("lo_fused_experts_block_int8", "lo_fused_experts_channel_int8",
+                                        "lo_fused_experts_workspace_bytes", "lo_topk_softmax", "lo_moe_fused_gate", "lo_last_error")),
+                            (mod.bind_fp8, ("lo_rms_norm_quant", "lo_per_token_group_quant_fp8", "lo_act_mul_group_quant_fp8",
+                                            "lo_gemm_w8a8_fp8_block", "lo_fused_experts_fp8", "lo_fused_experts_fp8_workspace_bytes",
+                                            "lo_gemm_w8a8_fp8_block_workspace_bytes"))):
+            bind(*(ctypes.cast(getattr(handle, n), c_void_p).value for n in names))
         _host = mod
     return _host
 

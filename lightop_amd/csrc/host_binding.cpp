@@ -583,31 +583,36 @@ PyObject *experts_fp8(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 }
 
 // bind(lo_fused_experts_block_int8, lo_fused_experts_channel_int8, lo_fused_experts_workspace_bytes, lo_topk_softmax,
-//      lo_moe_fused_gate, lo_last_error, lo_rms_norm_quant, lo_per_token_group_quant_fp8, lo_act_mul_group_quant_fp8,
-//      lo_gemm_w8a8_fp8_block, lo_fused_experts_fp8, lo_fused_experts_fp8_workspace_bytes, lo_gemm_w8a8_fp8_block_workspace_bytes): addresses of the library's functions.
+//      lo_moe_fused_gate, lo_last_error): addresses of the library's functions.
 PyObject *bind(PyObject *, PyObject *args) {
-  unsigned long long a[13];
-  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9], &a[10], &a[11],
-                        &a[12]))
-    return nullptr;
+  unsigned long long a[6];
+  if (!PyArg_ParseTuple(args, "KKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5])) return nullptr;
   g_block = reinterpret_cast<decltype(g_block)>(a[0]);
   g_channel = reinterpret_cast<decltype(g_channel)>(a[1]);
   g_ws_bytes = reinterpret_cast<decltype(g_ws_bytes)>(a[2]);
   g_topk_softmax = reinterpret_cast<decltype(g_topk_softmax)>(a[3]);
   g_gate = reinterpret_cast<decltype(g_gate)>(a[4]);
   g_last_error = reinterpret_cast<decltype(g_last_error)>(a[5]);
-  g_norm = reinterpret_cast<decltype(g_norm)>(a[6]);
-  g_quant_fp8 = reinterpret_cast<decltype(g_quant_fp8)>(a[7]);
-  g_act_fp8 = reinterpret_cast<decltype(g_act_fp8)>(a[8]);
-  g_gemm_fp8 = reinterpret_cast<decltype(g_gemm_fp8)>(a[9]);
-  g_experts_fp8 = reinterpret_cast<decltype(g_experts_fp8)>(a[10]);
-  g_experts_fp8_bytes = reinterpret_cast<decltype(g_experts_fp8_bytes)>(a[11]);
-  g_gemm_fp8_bytes = reinterpret_cast<decltype(g_gemm_fp8_bytes)>(a[12]);
+  Py_RETURN_NONE;
+}
+// bind_fp8(lo_rms_norm_quant, lo_per_token_group_quant_fp8, lo_act_mul_group_quant_fp8, lo_gemm_w8a8_fp8_block, lo_fused_experts_fp8,
+//          lo_fused_experts_fp8_workspace_bytes, lo_gemm_w8a8_fp8_block_workspace_bytes): those of the 8-bit operators beside them.
+PyObject *bind_fp8(PyObject *, PyObject *args) {
+  unsigned long long a[7];
+  if (!PyArg_ParseTuple(args, "KKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6])) return nullptr;
+  g_norm = reinterpret_cast<decltype(g_norm)>(a[0]);
+  g_quant_fp8 = reinterpret_cast<decltype(g_quant_fp8)>(a[1]);
+  g_act_fp8 = reinterpret_cast<decltype(g_act_fp8)>(a[2]);
+  g_gemm_fp8 = reinterpret_cast<decltype(g_gemm_fp8)>(a[3]);
+  g_experts_fp8 = reinterpret_cast<decltype(g_experts_fp8)>(a[4]);
+  g_experts_fp8_bytes = reinterpret_cast<decltype(g_experts_fp8_bytes)>(a[5]);
+  g_gemm_fp8_bytes = reinterpret_cast<decltype(g_gemm_fp8_bytes)>(a[6]);
   Py_RETURN_NONE;
 }
 
 PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, nullptr},
+    {"bind_fp8", bind_fp8, METH_VARARGS, nullptr},
     {"fused_experts", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(fused_experts)), METH_FASTCALL, nullptr},
     {"topk_softmax", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(topk_softmax)), METH_FASTCALL, nullptr},
     {"fused_gate", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(fused_gate)), METH_FASTCALL, nullptr},

@@ -7,7 +7,7 @@
 // One pass: a row stays in registers between its sum of squares and its codes (and, per token, its maximum), so a value is read once and
 // every output written once.  A workgroup a row: the row's two reductions then meet in LDS, and thousands of rows fill the card; rows that
 // several workgroups shared would need a second launch.  What bounds it is HBM (8192 x 7168 bf16 with a residual, e4m3 codes: 411 MB in 82 us,
-// 5.0 TB/s, what a copy reaches), for a few hundred rows the chain of load, two barriers and store (700 x 4096 fp16: 6.2 us), for one row
+// 5.0 TB/s, what a copy reaches), for a few hundred rows the chain of load, barrier and store (700 x 4096 fp16: 6.2 us), for one row
 // the launch (2.9 us).  The weight asked for in front of the first barrier gained nothing.
 #include "fp8.h"
 

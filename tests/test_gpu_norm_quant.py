@@ -193,3 +193,34 @@ def test_a_sum_over_other_rows_is_refused():
         rms_norm_quant(x, w, residual=out, residual_out=out)
         with pytest.raises(RuntimeError, match="overlaps"):
             rms_norm_quant(x, w, residual=buf[1:] if out.data_ptr() == buf.data_ptr() else buf[:5], residual_out=out)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("M,H", [(769, 128), (1000, 1152), (769, 2048), (801, 4224), (1500, 7168), (769, 16512), (770, 65536)])
+def test_values_of_many_rows(form, dtype, M, H):
+    """More rows than take one piece a thread: two, four and eight of them, and 1024 threads for the longest rows."""
+    from lightop_amd.norm import rms_norm_quant
+
+    print("[case] norm", form, dtype, M, H, flush=True)
+    q, g = FORMS[form]
+    x, r, w = _make(M, H, dtype, True)
+    _check(rms_norm_quant(x, w, 1e-5, residual=r, quant_dtype=q, group_size=g, return_normed=True), x, r, w, form, 1e-5, True)
+    x, r, w = _make(M, H, dtype, False, 1)
+    _check(rms_norm_quant(x, w, 1e-5, quant_dtype=q, group_size=g), x, r, w, form, 1e-5, False)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_more_rows_than_a_launch_takes(form):
+    """Offsets past 32 bits, in bytes and in values, and a second launch: the rows around its first and the last ones."""
+    from lightop_amd.norm import RmsNormQuant, rms_norm_quant
+
+    M, H = 2 ** 21 + 700, 1032 if form == "int8 rows" else 1152
+    q, g = FORMS[form]
+    tile = torch.randn(4096, H, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).to(torch.bfloat16)
+    x = tile.repeat(-(-M // 4096), 1)[:M]
+    x[-5:] *= 3
+    w = torch.ones(H, dtype=torch.bfloat16, device="cuda")
+    out = rms_norm_quant(x, w, 1e-6, residual=x, quant_dtype=q, group_size=g)
+    for part in (slice(0, 300), slice(2 ** 21 - 300, 2 ** 21 + 300), slice(M - 300, M)):
+        _check(RmsNormQuant(out.q[part], out.scale[part], out.residual[part], None), x[part], x[part], w, form, 1e-6, False)

@@ -208,3 +208,19 @@ def test_threads():
         t.join()
     for outs in made.values():
         assert len(outs) == 40 and all(torch.equal(o, want[i % 2]) for i, o in enumerate(outs))
+
+
+@pytest.mark.parametrize("M,N,K", [(3990, 4001, 8448), (3990, 4002, 1152), (2001, 5003, 1152), (1337, 7003, 2048), (1337, 7004, 8576),
+                                   (1300, 3333, 2048), (557, 3999, 7168), (563, 4001, 9216), (479, 7001, 8320), (82, 4097, 7168), (90, 4003, 9088),
+                                   (150, 3001, 8320), (110, 2051, 8320), (3310, 577, 7168)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_ragged_products_of_every_tile(dtype, M, N, K):
+    """Each tile, whole and in parts, with rows and columns that end inside it, rows of the result that begin off 16 bytes, more than 64 K
+    blocks (the weights' scales come 64 at a time) and numbers of them that are no multiple of four."""
+    from lightop_amd.gemmopt import gemm_w8a8_fp8_block
+
+    print("[case] gemm", dtype, M, N, K, flush=True)
+    a, b, sa, sb = _make(M, N, K)
+    out = gemm_w8a8_fp8_block(a, b, sa, sb, out_dtype=dtype)
+    _check(out, a, b, sa, sb)
+    assert torch.equal(out, gemm_w8a8_fp8_block(a, b, sa, sb, out_dtype=dtype))

@@ -570,12 +570,22 @@ static FewLayout few_layout(int64_t M, int32_t top_k, int64_t H, int64_t I) {
   l.part = take(few_split(H) > 1 ? few_split(H) * M * H * 4 : 0);
   return l;
 }
+static int check_few_sizes(int64_t M, int32_t top_k, int64_t H, int64_t I) {
+  LO_REQUIRE(M >= 0 && H >= kGroup && H % kGroup == 0 && I >= kGroup && I % kGroup == 0, LO_EINVAL,
+             "fused_experts_fp8: hidden (%lld) and intermediate (%lld) sizes must be multiples of 128", (long long)H, (long long)I);
+  LO_REQUIRE(H <= (1 << 20) && I <= (1 << 20), LO_ENOTSUP, "fused_experts_fp8: hidden and intermediate sizes are at most 2^20");
+  LO_REQUIRE(top_k >= 1, LO_EINVAL, "fused_experts_fp8: top_k (%d) must be positive", top_k);
+  LO_REQUIRE(top_k <= 64, LO_ENOTSUP, "fused_experts_fp8: top_k (%d) is at most 64", top_k);
+  LO_REQUIRE(M <= kFewTokens && M * top_k <= kFewSlots, LO_ENOTSUP,
+             "fused_experts_fp8: %lld tokens of %d slots (at most %d tokens and %d slots)", (long long)M, top_k, kFewTokens, kFewSlots);
+  return LO_OK;
+}
 } // namespace lo
 
 extern "C" int64_t lo_fused_experts_fp8_workspace_bytes(int64_t M, int32_t top_k, int64_t H, int64_t I) {
   using namespace lo;
-  if (M < 0 || top_k < 1 || H < kGroup || I < kGroup) return LO_EINVAL;
-  return few_layout(M, top_k, H, I).total;
+  const int rc = check_few_sizes(M, top_k, H, I); // (what the call refuses takes no memory first)
+  return rc ? rc : few_layout(M, top_k, H, I).total;
 }
 
 extern "C" int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t H, int64_t I, int32_t E, int32_t num_experts,
@@ -587,14 +597,10 @@ extern "C" int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t
   LO_REQUIRE(dtype == LO_BF16 || dtype == LO_F16, LO_ENOTSUP, "fused_experts_fp8: activations are bf16 or fp16");
   LO_REQUIRE(ids_dtype == LO_I32 || ids_dtype == LO_I64, LO_EINVAL, "fused_experts_fp8: ids are int32 or int64");
   LO_REQUIRE(activation == LO_ACT_SILU || activation == LO_ACT_GELU, LO_EINVAL, "fused_experts_fp8: unknown activation %d", activation);
-  LO_REQUIRE(M >= 0 && H >= kGroup && H % kGroup == 0 && I >= kGroup && I % kGroup == 0, LO_EINVAL,
-             "fused_experts_fp8: hidden (%lld) and intermediate (%lld) sizes must be multiples of 128", (long long)H, (long long)I);
-  LO_REQUIRE(H <= (1 << 20) && I <= (1 << 20), LO_ENOTSUP, "fused_experts_fp8: hidden and intermediate sizes are at most 2^20");
-  LO_REQUIRE(E >= 1 && E <= kFewExperts && num_experts >= E && top_k >= 1, LO_EINVAL, "fused_experts_fp8: bad expert counts");
-  LO_REQUIRE(top_k <= 64, LO_ENOTSUP, "fused_experts_fp8: top_k (%d) is at most 64", top_k);
+  LO_REQUIRE(E >= 1 && E <= kFewExperts && num_experts >= E, LO_EINVAL, "fused_experts_fp8: bad expert counts");
   LO_REQUIRE(num_experts == E || expert_map, LO_EINVAL, "fused_experts_fp8: %d experts routed over, %d here, and no expert_map", num_experts, E);
-  LO_REQUIRE(M <= kFewTokens && M * top_k <= kFewSlots, LO_ENOTSUP,
-             "fused_experts_fp8: %lld tokens of %d slots (at most %d tokens and %d slots)", (long long)M, top_k, kFewTokens, kFewSlots);
+  const int bad = check_few_sizes(M, top_k, H, I);
+  if (bad) return bad;
   if (M == 0) return LO_OK;
   LO_REQUIRE(x && w1 && w1s && w2 && w2s && topk_w && topk_ids && out && workspace, LO_EINVAL, "fused_experts_fp8: null pointer");
   const auto off = [](const void *p, unsigned al) { return (reinterpret_cast<uintptr_t>(p) & (al - 1)) != 0; };

@@ -678,6 +678,9 @@ def fused_experts_decode_fp8(hidden_states: torch.Tensor,
     if inplace and not hidden_states.is_contiguous():
         raise RuntimeError("fused_experts_decode_fp8: hidden_states must be contiguous to be written in place")
     top_k = topk_ids.shape[1]
+    lib = _lib.lib()
+    nbytes = lib.lo_fused_experts_fp8_workspace_bytes(M, top_k, H, I) if M else 0
+    _lib.check(nbytes)  # sizes past the limits are refused here, before anything is allocated or copied
     out = hidden_states if inplace else torch.empty_like(hidden_states, memory_format=torch.contiguous_format)
     if M == 0:
         return out
@@ -688,9 +691,6 @@ def fused_experts_decode_fp8(hidden_states: torch.Tensor,
     emap = None if expert_map is None else expert_map.to(torch.int32).contiguous()
     shared = None if shared_output is None else shared_output.contiguous()
     w1, w2 = _rows16(w1), _rows16(w2)
-    lib = _lib.lib()
-    nbytes = lib.lo_fused_experts_fp8_workspace_bytes(M, top_k, H, I)
-    _lib.check(nbytes)
     with _on_device(x):
         stream = torch.cuda.current_stream(x.device).cuda_stream
         workspace = _scratch(nbytes, x.device, stream)
@@ -749,6 +749,7 @@ def _in_graph_pool(t: torch.Tensor) -> bool:
     except (RuntimeError, KeyError):  # another allocator behind torch's, another layout of its snapshot
         pass
     return False
+
 
 def _run_fused_experts(hidden_states, w1, w2, topk_weights, topk_ids, cache13, inplace, apply_router_weight_on_input,
                        global_num_experts, expert_map, w1_scale, w2_scale, routed_scaling_factor, shared_output,

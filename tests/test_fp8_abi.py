@@ -137,3 +137,12 @@ def test_names_are_reachable():
 def test_norm_refuses_a_sum_over_other_rows(lib, bad):
     assert _norm(lib, **bad) < 0
     assert b"overlaps" in lib.lo_last_error()
+
+
+@pytest.mark.parametrize("M,top_k,H,I", [(65, 1, 256, 128), (8192, 8, 7168, 2048), (2 ** 62, 64, 256, 128), (64, 17, 256, 128), (1, 65, 256, 128),
+                                         (1, 0, 256, 128), (1, 1, 1 << 21, 128), (1, 1, 256, 1 << 21), (1, 1, 320, 128), (1, 1, 256, 192)])
+def test_experts_workspace_refuses_what_the_call_refuses(lib, M, top_k, H, I):
+    """Whoever sizes the workspace first meets the refusal before taking memory for it."""
+    assert lib.lo_gemm_w8a8_fp8_block(0, 0, 0, 0, 0, 0, -1, 1, 128, 0, 0, None) < 0  # another operator's error before it
+    assert lib.lo_fused_experts_fp8_workspace_bytes(M, top_k, H, I) < 0
+    assert b"fused_experts_fp8" in lib.lo_last_error()

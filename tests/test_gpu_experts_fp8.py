@@ -302,3 +302,27 @@ def test_streams_graphs_and_threads_of_many_slots(M, H):
         assert torch.equal(graphs[0][2], want[r % 3]) and torch.equal(graphs[1][2], want[(r + 1) % 3])
         for outs in (made["own"], made["same"], here):
             assert all(torch.equal(o, want[i % 3]) for i, o in enumerate(outs))
+
+
+@pytest.mark.parametrize("M,k", [(8192, 2), (64, 20), (1, 65)])
+def test_a_refused_batch_takes_no_memory(monkeypatch, M, k):
+    """More tokens or slots than a call takes: refused before a workspace of that size is made, or kept."""
+    from lightop_amd import _lib
+    from lightop_amd.moe import fused_experts_decode_fp8
+
+    w1, w2, s1, s2 = _layer(4, 256, 512)
+    x = torch.zeros(M, 256, dtype=torch.bfloat16, device="cuda")
+    tw, ids = torch.ones(M, k, device="cuda"), torch.zeros(M, k, dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()  # (its own workspace, none so far)
+
+    def refused():
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        with torch.cuda.stream(side), pytest.raises(RuntimeError, match="fused_experts_fp8"):
+            fused_experts_decode_fp8(x, w1, w2, tw, ids, s1, s2)
+        assert torch.cuda.memory_allocated() == before and torch.cuda.max_memory_allocated() == before
+
+    refused()
+    monkeypatch.setattr(_lib, "_host", _lib._NoHost())
+    refused()

@@ -340,12 +340,14 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_fp8_tile_kernel(const Fp8Ge
 // The parts of K added up in their order.
 template <int DT> __global__ __launch_bounds__(256) void gemm_fp8_join_kernel(const Fp8GemmArgs a) {
   const int64_t quads = a.M * (a.pitch / 4), step = a.M * a.pitch;
+  // whole quads are stored where rows begin on a quad: c may begin on any value
+  const bool whole = (a.N & 3) == 0 && (reinterpret_cast<uintptr_t>(a.C) & (DT == LO_F32 ? 15 : 7)) == 0;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < quads; i += static_cast<int64_t>(gridDim.x) * 256) {
     const float *const p = a.part + i * 4;
     v4f v = *reinterpret_cast<const v4f *>(p);
     for (int k = 1; k < a.splits; ++k) v += *reinterpret_cast<const v4f *>(p + k * step);
     const int64_t m = i / (a.pitch / 4), n = (i - m * (a.pitch / 4)) * 4;
-    if ((a.N & 3) == 0) {
+    if (whole) {
       if constexpr (DT == LO_F32) {
         *reinterpret_cast<v4f *>(static_cast<float *>(a.C) + m * a.N + n) = v;
       } else {

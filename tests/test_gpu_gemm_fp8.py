@@ -224,3 +224,21 @@ def test_ragged_products_of_every_tile(dtype, M, N, K):
     out = gemm_w8a8_fp8_block(a, b, sa, sb, out_dtype=dtype)
     _check(out, a, b, sa, sb)
     assert torch.equal(out, gemm_w8a8_fp8_block(a, b, sa, sb, out_dtype=dtype))
+
+
+@pytest.mark.parametrize("M,N,K", [(7, 64, 256), (333, 576, 7168), (20, 576, 7168), (300, 264, 384), (300, 2048, 2048)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_an_output_that_begins_on_any_value(dtype, M, N, K, shift):
+    """Columns in fours, and an `out` that begins off 8 and 16 bytes: up to 16 rows, in parts of K and whole."""
+    from lightop_amd.gemmopt import gemm_w8a8_fp8_block
+
+    print("[case] gemm", dtype, M, N, K, shift, flush=True)
+    a, b, sa, sb = _make(M, N, K)
+    room = torch.full((M * N + 64,), 7.0, dtype=dtype, device="cuda")
+    out = room[32 + shift:32 + shift + M * N].view(M, N)
+    assert out.data_ptr() % 8 or dtype == torch.float32
+    gemm_w8a8_fp8_block(a, b, sa, sb, out_dtype=dtype, out=out)
+    assert torch.equal(out, gemm_w8a8_fp8_block(a, b, sa, sb, out_dtype=dtype))
+    _check(out, a, b, sa, sb)
+    assert (room[:32 + shift] == 7).all() and (room[32 + shift + M * N:] == 7).all()

@@ -617,7 +617,8 @@ int lo_act_mul_group_quant_fp8(const void *c1, int dtype, int activation, int64_
 /*
  * c[m, n] = sum over kb of (a[m, kb] . b[n, kb]) * a_scale[m, kb] * b_scale[n / 128, kb] over K blocks of 128.
  *   a [M, K], b [N, K] e4m3, K a multiple of 128; a_scale [M, K/128], b_scale [ceil(N/128), K/128] fp32
- *   c [M, N] of out_dtype: the fp32 sum rounded once.  The order of the sum is fixed by the sizes and the workspace.
+ *   c [M, N] of out_dtype: the fp32 sum rounded once.  The order of the sum is fixed by the sizes and by whether the
+ *   workspace is there.
  *   workspace: NULL, or at least lo_gemm_w8a8_fp8_block_workspace_bytes, 16-byte aligned, one call's at a time: parts of K for sizes
  *   whose tiles do not fill the GPU.  Without it, or with less, K is not split
  */

@@ -401,16 +401,15 @@ struct Fp8Plan {
   int tile, parts;
 };
 static int64_t part_pitch(int64_t N) { return (N + 3) / 4 * 4; }
-// most: bytes that the parts may take.
-static Fp8Plan plan_gemm_fp8(int64_t M, int64_t N, int64_t KB, bool exact, int64_t most) {
+static Fp8Plan plan_gemm_fp8(int64_t M, int64_t N, int64_t KB, bool exact, bool may_split) {
   Fp8Plan best{-1, 1};
   float least = 0.0f;
   for (int i = exact ? kT128 : 0; i < kFp8Tiles; ++i) { // (an fp32 output's products take four times as long: tiles that leave room for them)
     const Fp8Tile &t = kFp8Tile[i];
     const int64_t tiles = ((M + t.tm - 1) / t.tm) * ((N + t.tn - 1) / t.tn);
-    for (int parts = 1; parts <= (i >= kT128x256 ? kMostParts : 1); parts += parts < 4 ? 1 : 2) {
+    for (int parts = 1; parts <= (may_split && i >= kT128x256 ? kMostParts : 1); parts += parts < 4 ? 1 : 2) {
       const int64_t bytes = parts * M * part_pitch(N) * 4;
-      if (parts > 1 && (KB / parts < kLeastBlocks || bytes > most)) break;
+      if (parts > 1 && KB / parts < kLeastBlocks) break;
       const int64_t each = (tiles * parts + 255) / 256; // workgroups of a CU
       const float blocks = static_cast<float>((KB + parts - 1) / parts);
       const int64_t rounds = each / t.held, rest = each % t.held;
@@ -446,7 +445,9 @@ template <int DT> static int launch_gemm_fp8(const Fp8GemmArgs &a, int64_t part_
     hipLaunchKernelGGL((gemm_fp8_few_kernel<DT>), dim3(static_cast<unsigned>((a.N + 15) / 16)), dim3(waves * 64), 0, stream, a);
     return LO_OK;
   }
-  const Fp8Plan p = plan_gemm_fp8(a.M, a.N, a.KB, DT == LO_F32, part_bytes);
+  // (with less room than the parts take K stays whole: the order of the sum goes by whether there is a workspace, not by its size)
+  Fp8Plan p = plan_gemm_fp8(a.M, a.N, a.KB, DT == LO_F32, true);
+  if (p.parts * a.M * part_pitch(a.N) * 4 > part_bytes && p.parts > 1) p = plan_gemm_fp8(a.M, a.N, a.KB, DT == LO_F32, false);
   if constexpr (DT != LO_F32) {
     if (p.tile == kT256) return launch_tile<DT, 256, 256, 2, 4, 2>(a, 1, stream);
     if (p.tile == kT192) return launch_tile<DT, 192, 256, 2, 4, 2>(a, 1, stream);
@@ -463,7 +464,7 @@ extern "C" int64_t lo_gemm_w8a8_fp8_block_workspace_bytes(int64_t M, int64_t N, 
   using namespace lo;
   if (M < 0 || N < 0 || K <= 0 || K % kGroup) return LO_EINVAL;
   if (M <= 16 || N == 0) return 0;
-  const Fp8Plan p = plan_gemm_fp8(M, N, K / kGroup, out_dtype == LO_F32, INT64_MAX);
+  const Fp8Plan p = plan_gemm_fp8(M, N, K / kGroup, out_dtype == LO_F32, true);
   return p.parts > 1 ? p.parts * M * part_pitch(N) * 4 : 0;
 }
 

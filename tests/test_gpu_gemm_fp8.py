@@ -242,3 +242,30 @@ def test_an_output_that_begins_on_any_value(dtype, M, N, K, shift):
     assert torch.equal(out, gemm_w8a8_fp8_block(a, b, sa, sb, out_dtype=dtype))
     _check(out, a, b, sa, sb)
     assert (room[:32 + shift] == 7).all() and (room[32 + shift + M * N:] == 7).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(20, 576, 7168), (130, 300, 16384), (333, 576, 7168), (333, 577, 7168)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_less_room_than_the_parts_take_is_no_room(dtype, M, N, K):
+    """A workspace that is too small, by a byte or by half: the bits of a call without one, and nothing written to it."""
+    from lightop_amd import _lib
+
+    a, b, sa, sb = _make(M, N, K)
+    lib, code = _lib.lib(), {torch.bfloat16: 0, torch.float32: 2}[dtype]
+    need = lib.lo_gemm_w8a8_fp8_block_workspace_bytes(M, N, K, code)
+    assert need > 0
+
+    def run(n):
+        out, room = torch.empty(M, N, dtype=dtype, device="cuda"), torch.full((need,), 0xff, dtype=torch.uint8, device="cuda")
+        _lib.check(lib.lo_gemm_w8a8_fp8_block(_lib.ptr(a), _lib.ptr(sa), _lib.ptr(b), _lib.ptr(sb), _lib.ptr(out), code, M, N, K,
+                                              _lib.ptr(room if n else None), n, _lib.stream_of(a)))
+        return out, bool((room == 0xff).all())
+
+    whole, untouched = run(0)
+    assert untouched
+    for n in (need - 1, need // 2, 16):
+        out, untouched = run(n)
+        assert untouched and torch.equal(out, whole), n
+    out, untouched = run(need)
+    assert not untouched
+    _check(out, a, b, sa, sb)

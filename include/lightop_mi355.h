@@ -620,7 +620,8 @@ int lo_act_mul_group_quant_fp8(const void *c1, int dtype, int activation, int64_
  *   c [M, N] of out_dtype: the fp32 sum rounded once.  The order of the sum is fixed by the sizes and by whether the
  *   workspace is there.
  *   workspace: NULL, or at least lo_gemm_w8a8_fp8_block_workspace_bytes, 16-byte aligned, one call's at a time: parts of K for sizes
- *   whose tiles do not fill the GPU.  Without it, or with less, K is not split
+ *   whose tiles do not fill the GPU.  Without it, or with less, K is not split.
+ *   The query refuses the sizes that the call refuses
  */
 int64_t lo_gemm_w8a8_fp8_block_workspace_bytes(int64_t M, int64_t N, int64_t K, int out_dtype);
 int lo_gemm_w8a8_fp8_block(const void *a, const float *a_scale, const void *b, const float *b_scale, void *c,

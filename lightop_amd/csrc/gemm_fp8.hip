@@ -458,11 +458,21 @@ template <int DT> static int launch_gemm_fp8(const Fp8GemmArgs &a, int64_t part_
   return launch_tile<DT, 64, 32, 2, 2, 4>(a, p.parts, stream);
 }
 
+static int check_gemm_fp8_sizes(int64_t M, int64_t N, int64_t K, int out_dtype) {
+  LO_REQUIRE(M >= 0 && N >= 0, LO_EINVAL, "gemm_w8a8_fp8_block: bad sizes %lld x %lld", (long long)M, (long long)N);
+  LO_REQUIRE(K > 0 && K % kGroup == 0, LO_EINVAL, "gemm_w8a8_fp8_block: K (%lld) must be a multiple of 128", (long long)K);
+  LO_REQUIRE(K <= (1 << 22), LO_ENOTSUP, "gemm_w8a8_fp8_block: K (%lld) is at most %d", (long long)K, 1 << 22);
+  LO_REQUIRE(M <= (1 << 24) && N <= (1 << 24), LO_ENOTSUP, "gemm_w8a8_fp8_block: M and N are at most 2^24");
+  LO_REQUIRE(out_dtype == LO_BF16 || out_dtype == LO_F16 || out_dtype == LO_F32, LO_ENOTSUP, "gemm_w8a8_fp8_block: the output is bf16, fp16 or fp32");
+  return LO_OK;
+}
+
 } // namespace lo
 
 extern "C" int64_t lo_gemm_w8a8_fp8_block_workspace_bytes(int64_t M, int64_t N, int64_t K, int out_dtype) {
   using namespace lo;
-  if (M < 0 || N < 0 || K <= 0 || K % kGroup) return LO_EINVAL;
+  const int rc = check_gemm_fp8_sizes(M, N, K, out_dtype);
+  if (rc) return rc;
   if (M <= 16 || N == 0) return 0;
   const Fp8Plan p = plan_gemm_fp8(M, N, K / kGroup, out_dtype == LO_F32, true);
   return p.parts > 1 ? p.parts * M * part_pitch(N) * 4 : 0;
@@ -471,11 +481,8 @@ extern "C" int64_t lo_gemm_w8a8_fp8_block_workspace_bytes(int64_t M, int64_t N, 
 extern "C" int lo_gemm_w8a8_fp8_block(const void *a, const float *a_scale, const void *b, const float *b_scale, void *c, int out_dtype,
                                       int64_t M, int64_t N, int64_t K, void *workspace, int64_t workspace_bytes, lo_stream_t stream) {
   using namespace lo;
-  LO_REQUIRE(M >= 0 && N >= 0, LO_EINVAL, "gemm_w8a8_fp8_block: bad sizes %lld x %lld", (long long)M, (long long)N);
-  LO_REQUIRE(K > 0 && K % kGroup == 0, LO_EINVAL, "gemm_w8a8_fp8_block: K (%lld) must be a multiple of 128", (long long)K);
-  LO_REQUIRE(K <= (1 << 22), LO_ENOTSUP, "gemm_w8a8_fp8_block: K (%lld) is at most %d", (long long)K, 1 << 22);
-  LO_REQUIRE(M <= (1 << 24) && N <= (1 << 24), LO_ENOTSUP, "gemm_w8a8_fp8_block: M and N are at most 2^24");
-  LO_REQUIRE(out_dtype == LO_BF16 || out_dtype == LO_F16 || out_dtype == LO_F32, LO_ENOTSUP, "gemm_w8a8_fp8_block: the output is bf16, fp16 or fp32");
+  const int bad = check_gemm_fp8_sizes(M, N, K, out_dtype);
+  if (bad) return bad;
   if (M == 0 || N == 0) return LO_OK;
   LO_REQUIRE(a && a_scale && b && b_scale && c, LO_EINVAL, "gemm_w8a8_fp8_block: null pointer");
   const auto off = [](const void *p, unsigned al) { return (reinterpret_cast<uintptr_t>(p) & (al - 1)) != 0; };

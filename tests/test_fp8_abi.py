@@ -146,3 +146,11 @@ def test_experts_workspace_refuses_what_the_call_refuses(lib, M, top_k, H, I):
     assert lib.lo_gemm_w8a8_fp8_block(0, 0, 0, 0, 0, 0, -1, 1, 128, 0, 0, None) < 0  # another operator's error before it
     assert lib.lo_fused_experts_fp8_workspace_bytes(M, top_k, H, I) < 0
     assert b"fused_experts_fp8" in lib.lo_last_error()
+
+
+@pytest.mark.parametrize("M,N,K,dtype", [((1 << 24) + 1, 16, 128, 0), (2 ** 62, 2 ** 62, 128, 0), (100, (1 << 24) + 1, 128, 0), (100, 16, 1 << 23, 0),
+                                         (100, 16, 64, 0), (-1, 16, 128, 0), (100, 16, 128, 3)])
+def test_gemm_workspace_refuses_what_the_call_refuses(lib, M, N, K, dtype):
+    assert lib.lo_per_token_group_quant_fp8(None, 7, 0, 128, 1e-10, None, None, None) < 0  # another operator's error before it
+    assert lib.lo_gemm_w8a8_fp8_block_workspace_bytes(M, N, K, dtype) < 0
+    assert b"gemm_w8a8_fp8_block" in lib.lo_last_error()

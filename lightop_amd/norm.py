@@ -46,8 +46,8 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, res
 
     ``x`` bf16, fp16 or fp32 of any leading shape (rows may be strided), ``weight`` of its type or fp32.  The sum comes back
     in ``residual`` in x's type, in ``residual_out`` where the caller brings one (contiguous; ``residual`` itself updates it
-    in place; any other overlap with an input is refused), None without a residual; with ``return_normed`` the normed rows in
-    x's type come back too."""
+    in place; any other overlap with rows that are read where they lie is refused), None without a residual; with
+    ``return_normed`` the normed rows in x's type come back too."""
     form = _FORMS.get((quant_dtype, group_size))
     if form is None:
         raise RuntimeError("rms_norm_quant: built for int8 with group_size None or 128 and float8_e4m3fn with 128, "
@@ -78,11 +78,16 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, res
         return RmsNormQuant(q, scale, total, normed)
     rows, w = _strided_rows(x), _rows16(weight)
     res = None if residual is None else _strided_rows(residual)
+    made = total  # (contiguous rows that begin off 16 bytes take a copy, as inputs do)
+    if total is not None and total.data_ptr() % 16:
+        made = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     with _on_device(x):
         _lib.check(_lib.lib().lo_rms_norm_quant(
             _lib.ptr(rows), dtype, rows.stride(0), _lib.ptr(res), 0 if res is None else res.stride(0), _lib.ptr(w),
-            _float_dtype(w, "weight"), rows.shape[0], H, float(eps), form, _lib.ptr(total), _lib.ptr(normed), _lib.ptr(q),
+            _float_dtype(w, "weight"), rows.shape[0], H, float(eps), form, _lib.ptr(made), _lib.ptr(normed), _lib.ptr(q),
             _lib.ptr(scale), _lib.stream_of(x)))
+        if made is not total:
+            total.detach().copy_(made)
     return RmsNormQuant(q, scale, total, normed)
 
 

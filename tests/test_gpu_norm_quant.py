@@ -224,3 +224,24 @@ def test_more_rows_than_a_launch_takes(form):
     out = rms_norm_quant(x, w, 1e-6, residual=x, quant_dtype=q, group_size=g)
     for part in (slice(0, 300), slice(2 ** 21 - 300, 2 ** 21 + 300), slice(M - 300, M)):
         _check(RmsNormQuant(out.q[part], out.scale[part], out.residual[part], None), x[part], x[part], w, form, 1e-6, False)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_a_sum_that_begins_on_any_value(form, dtype):
+    """`residual_out` off 16 bytes: the residual itself, updated in place, and memory of its own, with nothing else written."""
+    from lightop_amd.norm import rms_norm_quant
+
+    q, g = FORMS[form]
+    x, r, w = _make(7, 384, dtype, True)
+    want = rms_norm_quant(x, w, residual=r, quant_dtype=q, group_size=g)
+    for own in (True, False):
+        room = torch.full((7 * 384 + 16,), 7.0, dtype=dtype, device="cuda")
+        out = room[1:1 + 7 * 384].view(7, 384)
+        assert out.data_ptr() % 16
+        if own:
+            out.copy_(r)
+        got = rms_norm_quant(x, w, residual=out if own else r, residual_out=out, quant_dtype=q, group_size=g)
+        assert got.residual is out and torch.equal(out, want.residual)
+        assert torch.equal(got.q.view(torch.int8), want.q.view(torch.int8)) and torch.equal(got.scale, want.scale)
+        assert room[0] == 7 and (room[1 + 7 * 384:] == 7).all()

@@ -635,6 +635,7 @@ int lo_gemm_w8a8_fp8_block(const void *a, const float *a_scale, const void *b, c
  *   w1 [E, 2I, H], w2 [E, H, I] e4m3 row-major; w1s [E, 2I/128, H/128], w2s [E, H/128, I/128] fp32
  *   topk_w, topk_ids [M, top_k]; ids without an expert here (out of range, or no entry in expert_map) add nothing
  *   out[t] = routed_scaling_factor * sum_j topk_w[t, j] * y (+ shared_output[t]); out may be x or shared_output
+ *   (other overlaps with shared_output are refused)
  *   workspace: lo_fused_experts_fp8_workspace_bytes, 16-byte aligned; one call's at a time.  The query refuses the sizes that the
  *   call refuses (a negative code, lo_last_error set)
  */

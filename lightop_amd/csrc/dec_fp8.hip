@@ -606,6 +606,9 @@ extern "C" int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t
   const auto off = [](const void *p, unsigned al) { return (reinterpret_cast<uintptr_t>(p) & (al - 1)) != 0; };
   LO_REQUIRE(!off(x, 16) && !off(w1, 16) && !off(w2, 16) && !off(workspace, 16) && !off(out, 2) && !off(shared_output, 2), LO_EINVAL,
              "fused_experts_fp8: rows, weights and workspace must be 16-byte aligned");
+  // (x has been read when the first output is stored; shared rows are read as they are added)
+  const uintptr_t o = reinterpret_cast<uintptr_t>(out), sh = reinterpret_cast<uintptr_t>(shared_output), size = static_cast<uintptr_t>(M * H) * 2;
+  LO_REQUIRE(!sh || sh == o || sh + size <= o || o + size <= sh, LO_EINVAL, "fused_experts_fp8: out overlaps shared_output without being it");
   const FewLayout layout = few_layout(M, top_k, H, I);
   const int64_t need = layout.total;
   LO_REQUIRE(workspace_bytes >= need, LO_ENOSPC, "fused_experts_fp8: workspace holds %lld bytes, needs %lld", (long long)workspace_bytes,

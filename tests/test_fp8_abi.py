@@ -154,3 +154,10 @@ def test_gemm_workspace_refuses_what_the_call_refuses(lib, M, N, K, dtype):
     assert lib.lo_per_token_group_quant_fp8(None, 7, 0, 128, 1e-10, None, None, None) < 0  # another operator's error before it
     assert lib.lo_gemm_w8a8_fp8_block_workspace_bytes(M, N, K, dtype) < 0
     assert b"gemm_w8a8_fp8_block" in lib.lo_last_error()
+
+
+@pytest.mark.parametrize("out,sh", [(P + 2, P), (P, P + 2), (P + 1022, P), (P, P + 512)])
+def test_experts_refuse_shared_rows_under_other_outputs(lib, out, sh):
+    """Two rows of 256: an output stored over a shared value that another one still adds."""
+    assert _experts(lib, out=out, sh=sh) < 0
+    assert b"overlaps" in lib.lo_last_error()

@@ -326,3 +326,23 @@ def test_a_refused_batch_takes_no_memory(monkeypatch, M, k):
     refused()
     monkeypatch.setattr(_lib, "_host", _lib._NoHost())
     refused()
+
+
+@pytest.mark.parametrize("M,E,k", [(5, 8, 2), (40, 32, 4)])
+def test_in_place_beside_shared_rows(M, E, k):
+    """The output over the hidden states, which are the shared rows too, or follow them in one buffer; shifted by a row it is refused."""
+    from lightop_amd.moe import fused_experts_decode_fp8
+
+    w1, w2, s1, s2 = _layer(E, 256, 128)
+    x, tw, ids, shared = _tokens(M, 256, E, k, torch.bfloat16)
+    f = lambda x, sh, **o: fused_experts_decode_fp8(x, w1, w2, tw, ids, s1, s2, shared_output=sh, **o)
+    want, own = f(x, shared), f(x, x)
+    y = x.clone()
+    assert torch.equal(f(y, y, inplace=True), own) and torch.equal(y, own)
+    buf = torch.cat([shared, x])
+    assert torch.equal(f(buf[M:], buf[:M], inplace=True), want)
+    assert torch.equal(buf[M:], want) and torch.equal(buf[:M], shared)
+    buf = torch.cat([x, x])
+    with pytest.raises(RuntimeError, match="overlaps"):
+        f(buf[1:M + 1], buf[:M], inplace=True)
+    assert torch.equal(buf, torch.cat([x, x]))

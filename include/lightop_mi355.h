@@ -601,6 +601,8 @@ enum { LO_Q_INT8_ROWS = 0, LO_Q_INT8_GROUPS = 1, LO_Q_FP8_GROUPS = 2 };
  *   q_form  LO_Q_INT8_ROWS: scale [M], the rule of lo_per_token_quant_int8
  *           LO_Q_INT8_GROUPS: scale [M, H/128], the rule of lo_per_token_group_quant_int8 (eps 1e-10)
  *           LO_Q_FP8_GROUPS: scale [M, H/128], e4m3 codes (eps 1e-10)
+ *   A NaN or an infinity in a row: NaN codes in e4m3 and NaNs in normed_out; the int8 rules leave a NaN out of the maximum, and such a row's
+ *   int8 codes (0 and -128, scale 1e-10 / 127) stand for about zero
  */
 int lo_rms_norm_quant(const void *x, int dtype, int64_t x_stride, const void *residual, int64_t residual_stride,
                       const void *weight, int weight_dtype, int64_t M, int64_t H, float eps, int q_form,

@@ -245,3 +245,31 @@ def test_a_sum_that_begins_on_any_value(form, dtype):
         assert got.residual is out and torch.equal(out, want.residual)
         assert torch.equal(got.q.view(torch.int8), want.q.view(torch.int8)) and torch.equal(got.scale, want.scale)
         assert room[0] == 7 and (room[1 + 7 * 384:] == 7).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("M", [4, 800])
+def test_a_row_with_a_nan_or_an_infinity(form, M):
+    """What becomes of the row itself: the codes and scales that the package's own quantisation gives its normed rows."""
+    from lightop_amd.norm import rms_norm_quant
+    from lightop_amd.quant import per_token_group_quant_fp8, per_token_group_quant_int8, per_token_quant_int8
+
+    q, g = FORMS[form]
+    x, _, w = _make(M, 256, torch.bfloat16, False)
+    x[1, 7], x[2, 9] = float("nan"), float("-inf")
+    out = rms_norm_quant(x, w, quant_dtype=q, group_size=g, return_normed=True)
+    assert out.normed[1].isnan().all() and out.normed[2].isnan().sum() == 1 and (out.normed[2, 10:] == 0).all()
+    rows = out.normed[1:3].contiguous()
+    want = (per_token_quant_int8(rows) if form == "int8 rows" else
+            (per_token_group_quant_int8 if form == "int8 groups" else per_token_group_quant_fp8)(rows, 128))
+    assert torch.equal(out.q[1:3].view(torch.int8), want[0].view(torch.int8)) and torch.equal(out.scale[1:3], want[1])
+    assert (out.scale[1:3] < 1e-12).all()
+    if q == torch.int8:
+        assert (out.q[1] == -128).all() and out.q[2, 9] == -128 and (out.q[2] == 0).sum() == 255
+    else:
+        assert out.q[1].float().isnan().all() and out.q[2].float().isnan().sum() == 1
+    clean = x.clone()
+    clean[1:3] = 1
+    rest = rms_norm_quant(clean, w, quant_dtype=q, group_size=g)
+    keep = [0, *range(3, M)]
+    assert torch.equal(out.q[keep].view(torch.int8), rest.q[keep].view(torch.int8)) and torch.equal(out.scale[keep], rest.scale[keep])

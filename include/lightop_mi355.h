@@ -626,6 +626,9 @@ int lo_act_mul_group_quant_fp8(const void *c1, int dtype, int activation, int64_
  *   The query refuses the sizes that the call refuses
  */
 int64_t lo_gemm_w8a8_fp8_block_workspace_bytes(int64_t M, int64_t N, int64_t K, int out_dtype);
+/* Tokens and columns of the tile that such a call takes, and its parts of K (1 without a workspace). */
+int lo_gemm_w8a8_fp8_block_tile_query(int64_t M, int64_t N, int64_t K, int out_dtype, int has_workspace, int32_t *tile_m,
+                                      int32_t *tile_n, int32_t *parts);
 int lo_gemm_w8a8_fp8_block(const void *a, const float *a_scale, const void *b, const float *b_scale, void *c,
                            int out_dtype, int64_t M, int64_t N, int64_t K, void *workspace, int64_t workspace_bytes,
                            lo_stream_t stream);

@@ -111,6 +111,7 @@ SIGNATURES = {
     "lo_act_mul_group_quant_fp8": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "lo_gemm_w8a8_fp8_block": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64,
                                        c_void_p, c_int64, c_void_p]),
+    "lo_gemm_w8a8_fp8_block_tile_query": (c_int, [c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "lo_gemm_w8a8_fp8_block_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int]),
     "lo_fused_experts_fp8_workspace_bytes": (c_int64, [c_int64, c_int32, c_int64, c_int64]),
     "lo_fused_experts_fp8": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p,

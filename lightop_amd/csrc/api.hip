@@ -297,7 +297,7 @@ static int plan_channel_path(int flags, int64_t M, int32_t num_experts, int32_t 
 
 } // namespace lo
 
-extern "C" int lo_version(void) { return 102; }
+extern "C" int lo_version(void) { return 103; }
 
 extern "C" const char *lo_last_error(void) { return lo::g_err; }
 

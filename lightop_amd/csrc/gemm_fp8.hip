@@ -438,9 +438,10 @@ template <int DT, int TM, int TN, int WM, int WN, int ST> static int launch_tile
     return rc ? rc : join_parts<DT>(a, stream);
   }
 }
+constexpr int64_t kFp8FewTokens = 16; // gemm_fp8_few_kernel
 template <int DT> static int launch_gemm_fp8(const Fp8GemmArgs &a, int64_t part_bytes, hipStream_t stream) {
   // us, this / the tiles: 1 x 4096 x 7168 9.1 / 11.5, 16: 11.2 / 12.1, 16 x 7168 x 2048 7.4 / 7.4; 32 tokens in two fragments 15.7 / 12.3
-  if (a.M <= 16) {
+  if (a.M <= kFp8FewTokens) {
     const int waves = a.KB >= 16 ? 16 : a.KB >= 8 ? 8 : 4;
     hipLaunchKernelGGL((gemm_fp8_few_kernel<DT>), dim3(static_cast<unsigned>((a.N + 15) / 16)), dim3(waves * 64), 0, stream, a);
     return LO_OK;
@@ -473,9 +474,23 @@ extern "C" int64_t lo_gemm_w8a8_fp8_block_workspace_bytes(int64_t M, int64_t N, 
   using namespace lo;
   const int rc = check_gemm_fp8_sizes(M, N, K, out_dtype);
   if (rc) return rc;
-  if (M <= 16 || N == 0) return 0;
+  if (M <= kFp8FewTokens || N == 0) return 0;
   const Fp8Plan p = plan_gemm_fp8(M, N, K / kGroup, out_dtype == LO_F32, true);
   return p.parts > 1 ? p.parts * M * part_pitch(N) * 4 : 0;
+}
+
+extern "C" int lo_gemm_w8a8_fp8_block_tile_query(int64_t M, int64_t N, int64_t K, int out_dtype, int has_workspace, int32_t *tile_m, int32_t *tile_n,
+                                                 int32_t *parts) {
+  using namespace lo;
+  const int rc = check_gemm_fp8_sizes(M, N, K, out_dtype);
+  if (rc) return rc;
+  LO_REQUIRE(tile_m && tile_n && parts, LO_EINVAL, "gemm_w8a8_fp8_block_tile_query: null pointer");
+  const bool few = M <= kFp8FewTokens;
+  const Fp8Plan p = few || N == 0 ? Fp8Plan{kT64x32, 1} : plan_gemm_fp8(M, N, K / kGroup, out_dtype == LO_F32, has_workspace != 0);
+  *tile_m = few ? 16 : kFp8Tile[p.tile].tm;
+  *tile_n = few ? 16 : kFp8Tile[p.tile].tn;
+  *parts = p.parts;
+  return LO_OK;
 }
 
 extern "C" int lo_gemm_w8a8_fp8_block(const void *a, const float *a_scale, const void *b, const float *b_scale, void *c, int out_dtype,

@@ -3,6 +3,14 @@ import torch
 
 G = 128
 FP8 = torch.float8_e4m3fn
+# Sizes M, N, K of the dense product by the tile they take with a workspace (tokens, columns, whether K is in parts): rows and columns that end
+# inside a tile, columns in fours and not, numbers of K blocks that are no multiple of four, more than 64 of them.
+TILES = {(64, 32, False): [(17, 21, 384), (100, 700, 1664), (59, 6020, 8320)], (64, 32, True): [(18, 21, 2432), (17, 20, 8320), (130, 300, 7552)],
+         (64, 64, False): [(18, 8285, 896), (157, 4356, 8448)], (64, 64, True): [(17, 1461, 6272), (19, 1380, 8320)],
+         (128, 128, False): [(197, 8199, 384), (262, 7316, 8576)], (128, 128, True): [(66, 2751, 5760), (67, 2052, 8832)],
+         (128, 256, False): [(398, 8273, 384), (409, 8500, 8832)], (128, 256, True): [(18, 5661, 6912), (17, 5780, 8576)],
+         (192, 256, False): [(1025, 7291, 384), (1041, 7320, 8576)], (256, 256, False): [(1553, 7255, 384), (1741, 6740, 8448)]}
+TILE_SIZES = [(tile, size) for tile in TILES for size in TILES[tile]]
 ULP32 = 2.0 ** -24  # one fp32 rounding, relative
 
 

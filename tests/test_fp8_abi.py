@@ -4,6 +4,8 @@ import ctypes
 import pytest
 import torch
 
+import fp8_ref as ref
+
 
 @pytest.fixture(scope="module")
 def lib():
@@ -161,3 +163,32 @@ def test_experts_refuse_shared_rows_under_other_outputs(lib, out, sh):
     """Two rows of 256: an output stored over a shared value that another one still adds."""
     assert _experts(lib, out=out, sh=sh) < 0
     assert b"overlaps" in lib.lo_last_error()
+
+
+def _tile(lib, M, N, K, dtype=0, workspace=1):
+    out = [ctypes.c_int32(-7) for _ in range(3)]
+    rc = lib.lo_gemm_w8a8_fp8_block_tile_query(M, N, K, dtype, workspace, *(ctypes.byref(v) for v in out))
+    return rc if rc else tuple(v.value for v in out)
+
+
+def test_tiles_of_the_product(lib):
+    """The sizes that the GPU tests run by tile take that tile, the list has every tile that there is, and the workspace holds the parts."""
+    seen = {(16, 16, False)}
+    assert _tile(lib, 1, 4096, 7168) == _tile(lib, 16, 30, 128) == (16, 16, 1)
+    for (tm, tn, parts), (M, N, K) in ref.TILE_SIZES:
+        for dtype in (0, 1, 2):
+            m, n, p = _tile(lib, M, N, K, dtype)
+            assert (dtype == 2 and tm * tn > 128 * 128) or ((m, n, p > 1) == (tm, tn, parts)), (M, N, K, dtype)
+            seen.add((m, n, p > 1))
+            need = lib.lo_gemm_w8a8_fp8_block_workspace_bytes(M, N, K, dtype)
+            assert need == (p * M * -(-N // 4) * 16 if p > 1 else 0)
+            assert _tile(lib, M, N, K, dtype, 0)[2] == 1
+    for M in (17, 20, 33, 64, 65, 100, 128, 200, 300, 500, 800, 1400, 3000, 8192):
+        for N in (1, 24, 576, 1000, 2048, 4097, 7168, 16384):
+            for K in (128, 512, 1152, 2048, 7168, 16384):
+                for dtype in (0, 2):
+                    m, n, p = _tile(lib, M, N, K, dtype)
+                    assert (m, n, p > 1) in seen
+    for bad in ((-1, 1, 128), (1, 1, 64), (1, (1 << 24) + 1, 128), (1, 1, 1 << 23), (20, 20, 128, 3)):
+        assert _tile(lib, *bad) < 0 and b"gemm_w8a8_fp8_block" in lib.lo_last_error()
+    assert lib.lo_gemm_w8a8_fp8_block_tile_query(1, 1, 128, 0, 1, None, None, None) < 0

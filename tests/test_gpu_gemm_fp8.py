@@ -1,4 +1,6 @@
 """Dense e4m3 product with block scales against float64."""
+import ctypes
+
 import pytest
 import torch
 
@@ -269,3 +271,43 @@ def test_less_room_than_the_parts_take_is_no_room(dtype, M, N, K):
     out, untouched = run(need)
     assert not untouched
     _check(out, a, b, sa, sb)
+
+
+@pytest.mark.parametrize("tile,size", ref.TILE_SIZES, ids=lambda v: "x".join(map(str, v)))
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+def test_every_tile(dtype, tile, size):
+    """Each tile, whole and in parts, with what ends inside it; without a workspace the tiles that K in one piece takes."""
+    from lightop_amd import _lib
+    from lightop_amd.gemmopt import gemm_w8a8_fp8_block
+
+    M, N, K = size
+    lib, code = _lib.lib(), {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}[dtype]
+    got = [ctypes.c_int32() for _ in range(3)]
+    _lib.check(lib.lo_gemm_w8a8_fp8_block_tile_query(M, N, K, code, 1, *(ctypes.byref(v) for v in got)))
+    m, n, parts = (v.value for v in got)
+    assert dtype == torch.float32 or (m, n, parts > 1) == tile
+    print("[case] gemm", dtype, M, N, K, "tile", m, n, parts, flush=True)
+    a, b, sa, sb = _make(M, N, K)
+    out = gemm_w8a8_fp8_block(a, b, sa, sb, out_dtype=dtype)
+    _check(out, a, b, sa, sb)
+    assert torch.equal(out, gemm_w8a8_fp8_block(a, b, sa, sb, out_dtype=dtype))
+    if parts > 1:
+        whole = torch.empty_like(out)
+        _lib.check(lib.lo_gemm_w8a8_fp8_block(_lib.ptr(a), _lib.ptr(sa), _lib.ptr(b), _lib.ptr(sb), _lib.ptr(whole), code, M, N, K, None, 0,
+                                              _lib.stream_of(a)))
+        _check(whole, a, b, sa, sb)
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 250, 512), (70, 520, 512), (600, 250, 512), (20, 576, 7168), (333, 577, 7168)])
+def test_infinite_scales_stay_in_their_rows_and_columns(M, N, K):
+    from lightop_amd.gemmopt import gemm_w8a8_fp8_block
+
+    a, b, sa, sb = _make(M, N, K)
+    want = gemm_w8a8_fp8_block(a, b, sa, sb)
+    rows, cols = sa.clone(), sb.clone()
+    rows[1, K // 128 - 1] = float("inf")
+    cols[0, 2] = float("nan")
+    got = gemm_w8a8_fp8_block(a, b, rows, sb)
+    assert not got[1].isfinite().any() and torch.equal(got[0], want[0]) and torch.equal(got[2:], want[2:])
+    got = gemm_w8a8_fp8_block(a, b, sa, cols)
+    assert got[:, :128].isnan().all() and torch.equal(got[:, 128:], want[:, 128:])

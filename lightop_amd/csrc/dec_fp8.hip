@@ -8,7 +8,7 @@
 //          then every token's slots are added up in their order, by the experts' halves where two workgroups share them (few_split).  No
 //          atomics on results: the order of every sum is fixed.
 // Both find the experts hit from the ids by themselves.  The first product is the exact one (fp8.h): the matrix cores have time, and an error
-// of 1e-5 moves codes of the second quantisation; behind the second one stands a rounding to 16 bits.
+// of 1e-5 moves codes of the second quantisation.  So is the second one in the four launches; in the two its rounding to 16 bits follows the e4m3 instruction.
 //
 // HBM bounds them once many experts are hit (64 tokens of a DeepSeek-V3 share of 32 experts: 1.23 GB in 245 us, 5.0 TB/s, a copy's rate; of
 // Qwen3-30B-A3B 0.59 GB in 132 us), the two launches' dependent round trips with a few (one token of Qwen3-30B-A3B 18 us: ids, rows and
@@ -424,7 +424,7 @@ __global__ __launch_bounds__(1024) void experts_fp8_down_kernel(const Fp8Experts
         x[at][k] = codes_from_lds(codes + k * R * kGroup, row, q);
         sx[at][k] = scales[k * 16 + row];
       }
-      const v4f d = mfma_e4m3(w[at][k], x[at][k]);
+      const v4f d = mfma_e4m3_as<CODES>(w[at][k], x[at][k]);
       const float s = sx[at][k] * lane_value(b[at], k);
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s, acc[i]);

@@ -39,10 +39,18 @@ __device__ __forceinline__ v4f mfma_e4m3(const v8i a, const v8i b) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0, 0, 0);
 }
 
-// The same with every product and the sum to fp32's precision: e4m3 values are halves, four of the half instructions take them.
-// The e4m3 instruction lines the products up on the largest and drops what lies far below it: measured against 64 bits, normal operands
-// 1.4e-5 of the result, operands of very different sizes 6e-5, whichever of its forms (16x16x32, 16x16x128, 32x32x64); this one 1e-8 to 1e-7.
-// That is below a step of bf16 or fp16 and far above one of fp32, and what is quantised behind it moves codes.
+// What that instruction keeps: eight products that follow each other in K are lined up on the largest of them, by the operands' exponents, and cut
+// off, towards zero, 13 bits below (448 * 448 beside 3.75 * 3.75: 8 of 14.06 are added; the same for 16x16x32 and 32x32x64).  So a K block is off by
+// at most 7 * 2^-13, under 2^-10, of the sum of its eights' largest products: measured against 64 bits, normal operands 1.4e-5 of the
+// result's norm, operands of very different sizes 6e-5, all of one sign up to 4e-4 of a result, and where large products cancel what is left can
+// lose its digits.  bf16's half step is 2^-8, fp16's 2^-11.
+//
+// The same with every product and the sum to fp32's precision (1e-8 to 1e-7): e4m3 values are halves, four of the half instructions take them.
+// It takes four times as long, and so stands where the matrix cores have the time or the digits count: where weights are streamed (up to 16 tokens of
+// the dense product 8.45 -> 8.53 us, 1 x 4096 x 7168; the experts' second product in four launches 132.3 -> 132.4 us, 64 tokens of
+// Qwen3-30B-A3B), for fp32 outputs and for what is quantised again, whose codes 1e-5 would move.  It does not where it was in the way: the
+// tiles of 16-bit outputs (64 x 4096 x 7168 11.9 / 14.3 us, larger ones more) and the experts' second product in two launches, which comes last
+// with nothing to hide it (one token of Qwen3-30B-A3B 18.0 / 18.6 us, of a DeepSeek-V3 share 17.5 / 18.3).
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ v8h e4m3_halves(int lo, int hi) {
@@ -57,9 +65,9 @@ __device__ __forceinline__ v4f mfma_e4m3_exact(const v8i a, const v8i b) {
     d = __builtin_amdgcn_mfma_f32_16x16x32_f16(e4m3_halves(a[i], a[i + 1]), e4m3_halves(b[i], b[i + 1]), d, 0, 0, 0);
   return d;
 }
-// For a result that is kept in DT.
-template <int DT> __device__ __forceinline__ v4f mfma_e4m3_for(const v8i a, const v8i b) {
-  if constexpr (DT == LO_F32) return mfma_e4m3_exact(a, b);
+// Which of the two.
+template <bool EXACT> __device__ __forceinline__ v4f mfma_e4m3_as(const v8i a, const v8i b) {
+  if constexpr (EXACT) return mfma_e4m3_exact(a, b);
   else return mfma_e4m3(a, b);
 }
 

@@ -2,7 +2,7 @@
 //   C[m, n] = sum over kb of (A[m, kb] . B[n, kb]) * As[m, kb] * Bs[n / 128, kb],
 // A [M, K] rows with one scale for 128 values, B [N, K] a weight with one for 128 x 128.  A K block's 128 products are one MFMA
 // (v_mfma_f32_16x16x128_f8f6f4, which starts from zero), its fp32 result is folded into the fp32 sum with the scales' product.
-// (An fp32 output takes the exact form of it, fp8.h.)  Weights are the A operand: a lane holds four neighbouring columns of C for one token,
+// (An fp32 output and up to 16 tokens take the exact form of it, fp8.h.)  Weights are the A operand: a lane holds four neighbouring columns of C for one token,
 // whose scale it carries.
 #include "gemm.h"
 #include "fp8.h"
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(1024) void gemm_fp8_few_kernel(const Fp8GemmArgs a)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (kb0 + u * waves >= KB) break;
-      const v4f d = mfma_e4m3_for<DT>(w[u], x[u]);
+      const v4f d = mfma_e4m3_exact(w[u], x[u]);
       const float sc = s[u] * b[u];
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], sc, acc[i]);
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_fp8_tile_kernel(const Fp8Ge
       v4f d[FN];
 #pragma unroll
       for (int n = 0; n < FN; ++n) {
-        d[n] = mfma_e4m3_for<DT>(w[n], x[cur]);
+        d[n] = mfma_e4m3_as<DT == LO_F32>(w[n], x[cur]);
         if (m + 1 == FM) w[n] = read(sb, n, next);
       }
       fold(m == 0 ? FM - 1 : m - 1);

@@ -346,3 +346,21 @@ def test_in_place_beside_shared_rows(M, E, k):
     with pytest.raises(RuntimeError, match="overlaps"):
         f(buf[1:M + 1], buf[:M], inplace=True)
     assert torch.equal(buf, torch.cat([x, x]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("M,E,k,H,I", [(32, 30, 4, 2048, 768), (16, 26, 8, 4096, 256)])
+def test_many_experts_hit_only_fp32_roundings_are_in_front_of_the_output(dtype, M, E, k, H, I):
+    """The second product of the four launches keeps its sums to fp32's precision."""
+    w1, w2, s1, s2 = w = _layer(E, H, I)
+    x, tw, ids, _ = _tokens(M, H, E, k, dtype)
+    out, h = _run(x, w, tw, ids)
+    want, slack = torch.zeros(M, H, dtype=torch.float64, device="cuda"), torch.zeros(M, H, dtype=torch.float64, device="cuda")
+    for e in range(E):
+        t, j = torch.nonzero(ids == e, as_tuple=True)
+        if not t.numel():
+            continue
+        hd, d2, share = ref.dequant(*_codes32(h[t, j])), ref.dequant_weight(w2[e], s2[e]), tw[t, j].double().unsqueeze(1)
+        want.index_add_(0, t, share * (hd @ d2.T))
+        slack.index_add_(0, t, share * (hd.abs() @ d2.abs().T) * (I // 128 + 150 + k) * ref.ULP32)
+    assert ((out.double() - want).abs() <= slack + ref.half_step(dtype, want.abs() + slack)).all()

@@ -26,7 +26,7 @@ template <int DT> __device__ __forceinline__ void store_c(void *c, int64_t at, f
 // ---- up to 16 tokens ---------------------------------------------------------------------------------------------------------
 // A workgroup takes 16 columns and all tokens; its waves share the K blocks and add their sums up through LDS, in the same order every time.
 // Weights are read once, straight into registers, four K blocks of a wave in flight: HBM and the launch bound it (1 x 4096 x 7168: 29 MB in
-// 8.3 us).  Rows past the tokens are past the extents and read as zeros.
+// 8.5 us), where N is narrow the few workgroups (1 x 576 x 7168, 36 of them, 7.6 us; 16 rows 10.7).  Rows past the tokens are past the extents and read as zeros.
 template <int DT>
 __global__ __launch_bounds__(1024) void gemm_fp8_few_kernel(const Fp8GemmArgs a) {
   __shared__ __attribute__((aligned(16))) float red[16][256]; // [wave][token][column]
@@ -96,7 +96,9 @@ __device__ __forceinline__ bool dense_tile(int bid, int m_tiles, int n_tiles, in
 // loop is bound by the MFMAs with the fold's vector instructions between them, and by the clock, 1.7 GHz under that load.  Freeing the
 // weights' and the tokens' half of a stage apart took it from 217 us; other orders of the copies, s_setprio and groups of 8 token tiles to an
 // XCD gained nothing.  Middle sizes lose to their last round of workgroups, narrow ones to a step's latency: rings of six and eight stages
-// (64 x 64, 64 x 32) and an XCD to each part of K are no faster (333 x 576 x 7168 13.1 / 13.3 us, 48 x 7168 x 2048 8.0 / 8.0).
+// (64 x 64, 64 x 32) and an XCD to each part of K are no faster (each pair of one run, so / as it is: 333 x 576 x 7168 13.1 / 13.3 us, 48 x 7168 x 2048 8.0 / 8.0; by themselves 12.3 and 7.7).
+// An fp32 output's exact products take their time in large sizes: 8192 x 4096 x 7168 510 us, 1531 x 7168 x 2048 59, 333 x 576 x 7168 15.0, 48 x 7168 x
+// 2048 10.0.
 __device__ __forceinline__ void copy16(brsrc r, int8_t *lds, int voff, int soff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 16, voff, soff, 0, 0);
 }
@@ -384,8 +386,9 @@ template <int DT> static int join_parts(const Fp8GemmArgs &a, hipStream_t stream
 
 // Which tile, and how many parts of K: the smallest estimate of the time.  A K block takes a CU t1 us with one workgroup of the tile on it and
 // tn_us with as many as it holds (LDS); a workgroup starts and ends in `start` us; the parts are joined by a launch of kJoinUs that moves
-// them twice at kJoinBytes a us.  The figures are fitted to 67 sizes (17 to 8192 tokens, N 576 to 7168, K 256 to 7168), each timed with
-// every tile and 1 to 8 parts: the choice is 0.1 % off the fastest on average, 2.4 % at the most.  us, by another tile / by the choice: 1531 x
+// them twice at kJoinBytes a us.  The figures are fitted to 16-bit outputs of 67 sizes (17 to 8192 tokens, N 576 to 7168, K 256 to 7168), each timed with
+// every tile and 1 to 8 parts: the choice is 0.1 % off the fastest on average, 2.4 % at the most.  For fp32 outputs, whose products take four times as
+// long, the same figures only order the tiles and parts: they are not fitted, and how far that choice is off is not measured.  us, by another tile / by the choice: 1531 x
 // 7168 x 2048 28.9 (256 x 256) / 25.0 (192 x 256), 726 x 7168 x 2048 22.6 (192 x 256) / 17.9 (128 x 256), 490 x 7168 x 2048 22.1 (192 x
 // 256) / 14.2 (128 x 128), 333 x 576 x 7168 18.9 (64 x 32, whole) / 12.9 (64 x 64, four parts), 48 x 7168 x 2048 9.4 (64 x 64) / 7.6 (64 x 32).
 struct Fp8Tile {

@@ -6,15 +6,16 @@
 //
 // One pass: a row stays in registers between its sum of squares and its codes (and, per token, its maximum), so a value is read once and
 // every output written once.  A workgroup a row: the row's two reductions then meet in LDS, and thousands of rows fill the card; rows that
-// several workgroups shared would need a second launch.  What bounds it is HBM (8192 x 7168 bf16 with a residual, e4m3 codes: 411 MB in 82 us,
-// 5.0 TB/s, what a copy reaches), for a few hundred rows the chain of load, barrier and store (700 x 4096 fp16: 6.2 us), for one row
-// the launch (2.9 us).  The weight asked for in front of the first barrier gained nothing.
+// several workgroups shared would need a second launch.  What bounds it is HBM (with a residual, e4m3 codes: 8192 x 7168 bf16, 413 MB in 79-82 us,
+// 5.0-5.2 TB/s, what a copy reaches; fp32, 765 MB in 140 us, 5.5 TB/s; 4096 x 4096 fp32 42 us), for a few hundred rows the chain of load, barrier and
+// store (700 x 4096 bf16 6.2 us, fp16 with int8 groups and the normed rows 7.3), for one row the launch (2.8 us).  The weight asked for in
+// front of the first barrier gained nothing.  (Times in a captured graph, over inputs of more than the caches hold.)
 #include "fp8.h"
 
 namespace lo {
 
 constexpr int64_t kNormMaxH = 65536;
-// Up to so many rows a thread takes one piece (a row's steps, one behind the other, are what counts), beyond as many as fill 256 threads.  us, so /
+// Up to so many rows a thread takes one piece (a row's steps, one behind the other, are what counts), beyond as many as fill 256 threads.  us (inputs in the caches), so /
 // with 256 threads, bf16 rows with a residual, e4m3: 512 x 7168 7.6 / 8.7, 700 x 4096 6.2 / 6.6, 1000 x 7168 12.6 / 11.8, 2048 x 7168 21.1 / 19.9.
 constexpr int64_t kNormFew = 768;
 

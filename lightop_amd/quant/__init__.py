@@ -68,8 +68,8 @@ def per_token_group_quant_fp8(
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Quantise every ``group_size`` contiguous values of the last dimension to e4m3: ``top = max(|x|.max(), eps); s = top / 448;
     q = e4m3(448 x / top)``, to nearest, ties to even.  Returns ``(x_q, x_s)`` with ``x_s`` of shape
-    ``x.shape[:-1] + (x.shape[-1] // group_size,)`` in fp32.  Built for ``group_size == 128``; ``x`` is bf16, fp16 or fp32.
-    A NaN stays one and is left out of the maximum."""
+    ``x.shape[:-1] + (x.shape[-1] // group_size,)`` in fp32.  Built for ``group_size == 128``; ``x`` is bf16, fp16 or fp32,
+    ``eps`` finite and from 1e-30 up.  A NaN stays one and is left out of the maximum."""
     assert x.shape[-1] % group_size == 0, "the last dimension of `x` must be divisible by `group_size`"
     if dtype != torch.float8_e4m3fn:
         raise RuntimeError("per_token_group_quant_fp8: only torch.float8_e4m3fn output is supported")

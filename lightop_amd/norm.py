@@ -78,16 +78,16 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, res
         return RmsNormQuant(q, scale, total, normed)
     rows, w = _strided_rows(x), _rows16(weight)
     res = None if residual is None else _strided_rows(residual)
-    made = total  # (contiguous rows that begin off 16 bytes take a copy, as inputs do)
+    target = total  # (contiguous rows that begin off 16 bytes take a copy, as inputs do)
     if total is not None and total.data_ptr() % 16:
-        made = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        target = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     with _on_device(x):
         _lib.check(_lib.lib().lo_rms_norm_quant(
             _lib.ptr(rows), dtype, rows.stride(0), _lib.ptr(res), 0 if res is None else res.stride(0), _lib.ptr(w),
-            _float_dtype(w, "weight"), rows.shape[0], H, float(eps), form, _lib.ptr(made), _lib.ptr(normed), _lib.ptr(q),
+            _float_dtype(w, "weight"), rows.shape[0], H, float(eps), form, _lib.ptr(target), _lib.ptr(normed), _lib.ptr(q),
             _lib.ptr(scale), _lib.stream_of(x)))
-        if made is not total:
-            total.detach().copy_(made)
+        if target is not total:
+            total.detach().copy_(target)
     return RmsNormQuant(q, scale, total, normed)
 
 

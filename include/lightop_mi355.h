@@ -653,6 +653,49 @@ int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t H, int64_t
                          int activation, float routed_scaling_factor, const void *shared_output, void *out,
                          void *workspace, int64_t workspace_bytes, lo_stream_t stream);
 
+/* ---- dense blocks around the routed experts ------------------------------------------------------------
+ * The norms behind and in front of a block, its gate and the residual, in one pass; in fp32 between inputs and outputs:
+ *   h = x * (mean(x^2) + eps)^-1/2 * post_weight            (h = x without post_weight)
+ *   z = residual_scale * residual + scale * act(gate) * h   (act: identity, or the sigmoid with gate_sigmoid)
+ *   y = z * (mean(z^2) + eps)^-1/2 * weight                 (nothing of it without weight)
+ *   x, residual [M, H] rows of `dtype` x_stride / residual_stride values apart (multiples of 16 bytes); H <= 65536, a
+ *   multiple of 8 (q_form with groups: of 128)
+ *   gate: NULL, or rows gate_stride values apart, one for gate_rows rows of x: row m takes gate row m / gate_rows, H values
+ *   with gate_channels (16-byte aligned rows), else one value
+ *   weight, post_weight [H], gate: of `dtype` or LO_F32
+ *   residual_out [M, H]: z rounded once; may be x or residual itself where that is contiguous, and must not overlap an input otherwise
+ *   normed_out [M, H]: y rounded once; may be NULL where q_form gives codes
+ *   q_form: LO_Q_NONE, or y's codes q [M, H] and q_scale in the forms of lo_rms_norm_quant
+ * No output but residual_out may overlap an input. */
+enum { LO_Q_NONE = -1 };
+int lo_rms_norm_block(const void *x, int dtype, int64_t x_stride, const void *residual, int64_t residual_stride,
+                      const void *post_weight, int post_weight_dtype, const void *gate, int gate_dtype,
+                      int64_t gate_stride, int64_t gate_rows, int gate_channels, int gate_sigmoid, const void *weight,
+                      int weight_dtype, float scale, float residual_scale, int64_t M, int64_t H, float eps, int q_form,
+                      void *residual_out, void *normed_out, void *q, float *q_scale, lo_stream_t stream);
+
+/*
+ * Dense product with bias, activation and residual in its epilogue; K-major operands, fp32 (int8: int32) sums.
+ *   v[m, n] = sum over k of a[m, k] * b[n, k], times a_scale[m] * b_scale[n] with LO_I8, + bias[n]
+ *   c[m, n] = scale * act(v[m, n]) + residual[m, n], or, gated, scale * act(v[m, n]) * v[m, N + n] + residual[m, n]
+ *   a [M, K], b [N, K] (gated: [2N, K], the gate's rows first) of `dtype` LO_BF16, LO_F16 or LO_I8, rows a_stride / b_stride values
+ *   apart; rows and strides multiples of 16 bytes, as K is; strides at most 4 MiB, an int8 K at most 131056
+ *   a_scale [M], b_scale [N] (gated [2N]) fp32 with LO_I8, else NULL
+ *   bias NULL or [N] (gated [2N]) of out_dtype or LO_F32;  activation LO_ACT_NONE, LO_ACT_SILU or LO_ACT_GELU
+ *   residual NULL or [M, N] of out_dtype, rows residual_stride values apart; c itself, or apart from it
+ *   c [M, N] of out_dtype LO_BF16, LO_F16 or LO_F32: rounded once.  It must not overlap another input
+ *   workspace: NULL, or at least lo_gemm_bias_act_workspace_bytes, 16-byte aligned, one call's at a time: parts of K for sizes
+ *   whose tiles do not fill the GPU.  Without it, or with less, K is not split.  The order of the sum is fixed by the sizes
+ *   and by whether the workspace is there.
+ */
+enum { LO_I8 = 3 };
+enum { LO_ACT_NONE = -1 };
+int64_t lo_gemm_bias_act_workspace_bytes(int dtype, int gated, int64_t M, int64_t N, int64_t K);
+int lo_gemm_bias_act(const void *a, int64_t a_stride, const void *b, int64_t b_stride, int dtype, const float *a_scale,
+                     const float *b_scale, const void *bias, int bias_dtype, int activation, int gated, float scale,
+                     const void *residual, int64_t residual_stride, void *c, int out_dtype, int64_t M, int64_t N,
+                     int64_t K, void *workspace, int64_t workspace_bytes, lo_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,9 +19,10 @@ LO_GEMM_W4 = 32
 LO_FUSED_NO_DECODE_PATH = 64
 LO_FUSED_FORCE_DECODE_PATH = 128
 LO_FUSED_ACT_GELU = 256
-LO_ACT_SILU, LO_ACT_GELU = 0, 1
+LO_ACT_NONE, LO_ACT_SILU, LO_ACT_GELU = -1, 0, 1
 LO_FORM_BLOCK, LO_FORM_CHANNEL, LO_FORM_W4 = 0, 1, 2
-LO_Q_INT8_ROWS, LO_Q_INT8_GROUPS, LO_Q_FP8_GROUPS = 0, 1, 2
+LO_Q_NONE, LO_Q_INT8_ROWS, LO_Q_INT8_GROUPS, LO_Q_FP8_GROUPS = -1, 0, 1, 2
+LO_I8 = 3
 LO_NOALLOC_SCRATCH_BYTES = 32 << 20
 LO_KERNEL_WS, LO_KERNEL_TILE, LO_KERNEL_PC, LO_KERNEL_AS, LO_KERNEL_T128, LO_KERNEL_W4_TILE, LO_KERNEL_DEC = 0, 1, 2, 3, 4, 5, 6
 KERNEL_NAMES = {LO_KERNEL_WS: "moe_gemm_ws_kernel", LO_KERNEL_TILE: "moe_gemm_tile_kernel",
@@ -117,6 +118,12 @@ SIGNATURES = {
     "lo_fused_experts_fp8": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p,
                                      c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_float, c_void_p,
                                      c_void_p, c_void_p, c_int64, c_void_p]),
+    "lo_rms_norm_block": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_int,
+                                  c_int, c_void_p, c_int, c_float, c_float, c_int64, c_int64, c_float, c_int, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_void_p]),
+    "lo_gemm_bias_act_workspace_bytes": (c_int64, [c_int, c_int, c_int64, c_int64, c_int64]),
+    "lo_gemm_bias_act": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float,
+                                 c_void_p, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
 }
 
 _lib = None

@@ -110,16 +110,17 @@ template <int DT> __device__ __forceinline__ void store8(void *x, int64_t at, co
 }
 
 // act(g) * u in fp32, nothing rounded to 16 bits on the way.
-// SiLU: exp(-g) as 2^(-g log2 e) with the product's rounding error and the constant's given back, so that far gates keep their digits.
-__device__ __forceinline__ float silu_f32(float g) {
+// Sigmoid: exp(-g) as 2^(-g log2 e) with the product's rounding error and the constant's given back, so that far gates keep their digits.
+__device__ __forceinline__ float sigmoid_f32(float g) {
   const float n = g * -1.44269502f;
   const float lost = __builtin_fmaf(g, -1.44269502f, -n) + g * -1.92596299e-8f;
   const float e = __builtin_amdgcn_exp2f(n);
   // (past the ends of the exponential there is nothing to correct, and an infinite n has no difference)
   const float e1 = fabsf(n) < 126.0f ? __builtin_fmaf(e, lost * 0.693147182f, e) : e;
   const float d = 1.0f + e1, r = __builtin_amdgcn_rcpf(d);
-  return g * (r > 0.0f ? __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r) : r); // (an infinite d: 0)
+  return r > 0.0f ? __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r) : r; // (an infinite d: 0)
 }
+__device__ __forceinline__ float silu_f32(float g) { return g * sigmoid_f32(g); }
 // GELU in its erf form; the complement keeps the digits that 1 + erf loses left of zero.
 __device__ __forceinline__ float gelu_f32(float g) { return 0.5f * g * erfcf(g * -0.707106769f); }
 template <int ACT> __device__ __forceinline__ float act_mul_f32(float g, float u) {

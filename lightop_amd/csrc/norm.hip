@@ -46,6 +46,44 @@ template <bool MAX> __device__ __forceinline__ float across_waves(float v, float
   return v;
 }
 
+// Codes of a thread's eight values, of a group that it shares with the 15 lanes around it (all of them in the row or none).
+template <int FORM> __device__ __forceinline__ void group_codes(const float (&v)[8], int8_t *q, float *scale) {
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  top = fmaxf(top, 1e-10f);
+  float s;
+  v2i packed;
+  if constexpr (FORM == LO_Q_FP8_GROUPS) {
+    const Fp8Group g = fp8_group(top, s);
+    packed = v2i{fp8_pack4(&v[0], g), fp8_pack4(&v[4], g)};
+  } else {
+    s = top / 127.0f;
+    const float y = 1.0f / s;
+    packed = v2i{static_cast<int>(quant4(&v[0], s, y)), static_cast<int>(quant4(&v[4], s, y))};
+  }
+  *reinterpret_cast<v2i *>(q) = packed;
+  if ((threadIdx.x & 15) == 0) *scale = s;
+}
+// Codes of a row whose largest magnitude is amax.
+template <int CH> __device__ __forceinline__ void row_codes(const float (&v)[CH][8], float amax, int8_t *q, float *scale, int pieces) {
+  amax = fmaxf(amax, 1e-10f);
+  const float inv = 127.0f / amax;
+  if (threadIdx.x == 0) *scale = amax / 127.0f;
+#pragma unroll
+  for (int j = 0; j < CH; ++j) {
+    const int p = threadIdx.x + j * blockDim.x;
+    if (p >= pieces) continue;
+    int b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = rne_i8(v[j][i] * inv);
+    *reinterpret_cast<v2i *>(q + p * 8) =
+        v2i{static_cast<int>(pack4_i8(b[0], b[1], b[2], b[3])), static_cast<int>(pack4_i8(b[4], b[5], b[6], b[7]))};
+  }
+}
+
 // A workgroup a row; CH pieces of eight values a thread.
 template <int DT, int FORM, int CH>
 __global__ __launch_bounds__(1024) void rms_norm_quant_kernel(const NormArgs a) {
@@ -93,56 +131,31 @@ __global__ __launch_bounds__(1024) void rms_norm_quant_kernel(const NormArgs a) 
 #pragma unroll
       for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[j][i]));
     } else if (p < pieces) {
-      float top = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[j][i]));
-#pragma unroll
-      for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor(top, d)); // 16 lanes hold a group, all of them in the row or none
-      top = fmaxf(top, 1e-10f);
-      float s;
-      v2i packed;
-      if constexpr (FORM == LO_Q_FP8_GROUPS) {
-        const Fp8Group g = fp8_group(top, s);
-        packed = v2i{fp8_pack4(&v[j][0], g), fp8_pack4(&v[j][4], g)};
-      } else {
-        s = top / 127.0f;
-        const float y = 1.0f / s;
-        packed = v2i{static_cast<int>(quant4(&v[j][0], s, y)), static_cast<int>(quant4(&v[j][4], s, y))};
-      }
-      *reinterpret_cast<v2i *>(a.q + base + p * 8) = packed;
-      if ((tid & 15) == 0) a.s[(base >> 7) + (p >> 4)] = s;
+      group_codes<FORM>(v[j], a.q + base + p * 8, a.s + (base >> 7) + (p >> 4));
     }
   }
-  if constexpr (FORM == LO_Q_INT8_ROWS) {
-    amax = fmaxf(across_waves<true>(amax, red[1], waves), 1e-10f);
-    const float inv = 127.0f / amax;
-    if (tid == 0) a.s[row] = amax / 127.0f;
-#pragma unroll
-    for (int j = 0; j < CH; ++j) {
-      const int p = tid + j * threads;
-      if (p >= pieces) continue;
-      int b[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) b[i] = rne_i8(v[j][i] * inv);
-      *reinterpret_cast<v2i *>(a.q + base + p * 8) =
-          v2i{static_cast<int>(pack4_i8(b[0], b[1], b[2], b[3])), static_cast<int>(pack4_i8(b[4], b[5], b[6], b[7]))};
-    }
-  }
+  if constexpr (FORM == LO_Q_INT8_ROWS) row_codes<CH>(v, across_waves<true>(amax, red[1], waves), a.q + base, a.s + row, pieces);
 }
 
+struct NormGrid {
+  static constexpr int64_t kRows = 1 << 21; // of one launch: a grid holds fewer than 2^32 threads
+  int threads, ch;
+  NormGrid(int H, int64_t M) {
+    // (a thread holds at most eight pieces; short rows take fewer threads)
+    const int pieces = H / 8;
+    threads = pieces > 8 * 256 || M <= kNormFew ? 1024 : 256;
+    while (threads > 64 && threads / 2 >= pieces) threads /= 2;
+    ch = (pieces + threads - 1) / threads;
+  }
+  dim3 rows(int64_t left) const { return dim3(static_cast<unsigned>(left < kRows ? left : kRows)); }
+};
 template <int DT, int FORM> static void launch_norm(NormArgs a, int64_t M, hipStream_t stream) {
-  const bool few = M <= kNormFew;
-  // (a thread holds at most eight pieces; short rows take fewer threads)
-  const int pieces = a.H / 8;
-  int threads = pieces > 8 * 256 || few ? 1024 : 256;
-  while (threads > 64 && threads / 2 >= pieces) threads /= 2;
-  const int ch = (pieces + threads - 1) / threads;
-  constexpr int64_t kRows = 1 << 21; // of one launch: a grid holds fewer than 2^32 threads
-  for (; a.row0 < M; a.row0 += kRows) {
-    const dim3 grid(static_cast<unsigned>(M - a.row0 < kRows ? M - a.row0 : kRows)), block(static_cast<unsigned>(threads));
-    if (ch <= 1) hipLaunchKernelGGL((rms_norm_quant_kernel<DT, FORM, 1>), grid, block, 0, stream, a);
-    else if (ch <= 2) hipLaunchKernelGGL((rms_norm_quant_kernel<DT, FORM, 2>), grid, block, 0, stream, a);
-    else if (ch <= 4) hipLaunchKernelGGL((rms_norm_quant_kernel<DT, FORM, 4>), grid, block, 0, stream, a);
+  const NormGrid g(a.H, M);
+  for (; a.row0 < M; a.row0 += NormGrid::kRows) {
+    const dim3 grid = g.rows(M - a.row0), block(static_cast<unsigned>(g.threads));
+    if (g.ch <= 1) hipLaunchKernelGGL((rms_norm_quant_kernel<DT, FORM, 1>), grid, block, 0, stream, a);
+    else if (g.ch <= 2) hipLaunchKernelGGL((rms_norm_quant_kernel<DT, FORM, 2>), grid, block, 0, stream, a);
+    else if (g.ch <= 4) hipLaunchKernelGGL((rms_norm_quant_kernel<DT, FORM, 4>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((rms_norm_quant_kernel<DT, FORM, 8>), grid, block, 0, stream, a);
   }
 }
@@ -150,6 +163,126 @@ template <int DT> static void launch_norm_form(int form, const NormArgs &a, int6
   if (form == LO_Q_INT8_ROWS) launch_norm<DT, LO_Q_INT8_ROWS>(a, M, stream);
   else if (form == LO_Q_INT8_GROUPS) launch_norm<DT, LO_Q_INT8_GROUPS>(a, M, stream);
   else launch_norm<DT, LO_Q_FP8_GROUPS>(a, M, stream);
+}
+
+// ---- the norms behind and in front of a block ---------------------------------------------------------------------------------
+//   h = x * (mean(x^2) + eps)^-1/2 * post,  z = residual_scale * r + scale * act(gate) * h,  y = z * (mean(z^2) + eps)^-1/2 * w
+// and y's codes; in fp32 between the inputs and the outputs, as above.
+constexpr int kNoCodes = -1;
+struct NormBlockArgs {
+  const void *x, *r, *post, *w, *gate;
+  void *z, *y;
+  int8_t *q;
+  float *s;
+  int64_t xs, rs, gs; // row strides, in values
+  int64_t row0;       // of the launch's first workgroup
+  uint32_t gate_rows; // rows that share a row of the gate
+  int32_t H;
+  int32_t post_f32, w_f32, gate_f32, gate_channels, gate_sigmoid;
+  float eps, scale, residual_scale;
+};
+
+template <int DT> __device__ __forceinline__ void load8_as(const void *x, int f32, int64_t at, float (&v)[8]) {
+  if (f32) load8<LO_F32>(x, at, v);
+  else load8<DT>(x, at, v);
+}
+
+template <int DT, int FORM, int CH>
+__global__ __launch_bounds__(1024) void rms_norm_block_kernel(const NormBlockArgs a) {
+  __shared__ float red[3][16];
+  const int tid = threadIdx.x, threads = blockDim.x, waves = threads >> 6;
+  const int pieces = a.H / 8;
+  const int64_t row = a.row0 + blockIdx.x, base = row * a.H;
+  float v[CH][8];
+#pragma unroll
+  for (int j = 0; j < CH; ++j) {
+    const int p = tid + j * threads;
+    if (p < pieces) load8<DT>(a.x, row * a.xs + p * 8, v[j]);
+    else
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[j][i] = 0.0f;
+  }
+  const int64_t gate0 = a.gate ? static_cast<uint32_t>(row) / a.gate_rows * a.gs : 0;
+  float token = 1.0f;
+  if (a.gate && !a.gate_channels) {
+    token = a.gate_f32 ? static_cast<const float *>(a.gate)[gate0]
+            : DT == LO_F32 ? static_cast<const float *>(a.gate)[gate0] : to_f32<DT>(static_cast<const uint16_t *>(a.gate)[gate0]);
+    if (a.gate_sigmoid) token = sigmoid_f32(token);
+  }
+  float rstd = 1.0f;
+  if (a.post) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(v[j][i], v[j][i], ss);
+    rstd = 1.0f / sqrtf(across_waves<false>(ss, red[0], waves) / static_cast<float>(a.H) + a.eps);
+  }
+  float ss = 0.0f;
+#pragma unroll
+  for (int j = 0; j < CH; ++j) {
+    const int p = tid + j * threads;
+    if (p < pieces) {
+      float r[8], w[8];
+      load8<DT>(a.r, row * a.rs + p * 8, r);
+      if (a.post) {
+        load8_as<DT>(a.post, a.post_f32, p * 8, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j][i] = v[j][i] * rstd * w[i];
+      }
+      if (a.gate_channels) {
+        load8_as<DT>(a.gate, a.gate_f32, gate0 + p * 8, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j][i] *= a.gate_sigmoid ? sigmoid_f32(w[i]) : w[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j][i] *= token;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[j][i] = __builtin_fmaf(a.scale, v[j][i], a.residual_scale * r[i]);
+      store8<DT>(a.z, base + p * 8, v[j]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(v[j][i], v[j][i], ss);
+  }
+  if (!a.w) return;
+  rstd = 1.0f / sqrtf(across_waves<false>(ss, red[1], waves) / static_cast<float>(a.H) + a.eps);
+  float amax = 0.0f;
+#pragma unroll
+  for (int j = 0; j < CH; ++j) {
+    const int p = tid + j * threads;
+    if (p < pieces) {
+      float w[8];
+      load8_as<DT>(a.w, a.w_f32, p * 8, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[j][i] = v[j][i] * rstd * w[i];
+      if (a.y) store8<DT>(a.y, base + p * 8, v[j]);
+    }
+    if constexpr (FORM == LO_Q_INT8_ROWS) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[j][i]));
+    } else if constexpr (FORM != kNoCodes) {
+      if (p < pieces) group_codes<FORM>(v[j], a.q + base + p * 8, a.s + (base >> 7) + (p >> 4));
+    }
+  }
+  if constexpr (FORM == LO_Q_INT8_ROWS) row_codes<CH>(v, across_waves<true>(amax, red[2], waves), a.q + base, a.s + row, pieces);
+}
+
+template <int DT, int FORM> static void launch_norm_block(NormBlockArgs a, int64_t M, hipStream_t stream) {
+  const NormGrid g(a.H, M);
+  for (; a.row0 < M; a.row0 += NormGrid::kRows) {
+    const dim3 grid = g.rows(M - a.row0), block(static_cast<unsigned>(g.threads));
+    if (g.ch <= 1) hipLaunchKernelGGL((rms_norm_block_kernel<DT, FORM, 1>), grid, block, 0, stream, a);
+    else if (g.ch <= 2) hipLaunchKernelGGL((rms_norm_block_kernel<DT, FORM, 2>), grid, block, 0, stream, a);
+    else if (g.ch <= 4) hipLaunchKernelGGL((rms_norm_block_kernel<DT, FORM, 4>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((rms_norm_block_kernel<DT, FORM, 8>), grid, block, 0, stream, a);
+  }
+}
+template <int DT> static void launch_norm_block_form(int form, const NormBlockArgs &a, int64_t M, hipStream_t stream) {
+  if (form == LO_Q_INT8_ROWS) launch_norm_block<DT, LO_Q_INT8_ROWS>(a, M, stream);
+  else if (form == LO_Q_INT8_GROUPS) launch_norm_block<DT, LO_Q_INT8_GROUPS>(a, M, stream);
+  else if (form == LO_Q_FP8_GROUPS) launch_norm_block<DT, LO_Q_FP8_GROUPS>(a, M, stream);
+  else launch_norm_block<DT, kNoCodes>(a, M, stream);
 }
 
 } // namespace lo
@@ -193,4 +326,59 @@ extern "C" int lo_rms_norm_quant(const void *x, int dtype, int64_t x_stride, con
   else if (dtype == LO_F16) launch_norm_form<LO_F16>(q_form, a, M, s);
   else launch_norm_form<LO_F32>(q_form, a, M, s);
   return check_launch("rms_norm_quant");
+}
+
+extern "C" int lo_rms_norm_block(const void *x, int dtype, int64_t x_stride, const void *residual, int64_t residual_stride, const void *post_weight,
+                                 int post_weight_dtype, const void *gate, int gate_dtype, int64_t gate_stride, int64_t gate_rows, int gate_channels,
+                                 int gate_sigmoid, const void *weight, int weight_dtype, float scale, float residual_scale, int64_t M, int64_t H,
+                                 float eps, int q_form, void *residual_out, void *normed_out, void *q, float *q_scale, lo_stream_t stream) {
+  using namespace lo;
+  LO_REQUIRE(M >= 0, LO_EINVAL, "rms_norm_block: %lld rows", (long long)M);
+  LO_REQUIRE(M <= INT32_MAX, LO_ENOTSUP, "rms_norm_block: %lld rows (at most 2^31 - 1)", (long long)M);
+  LO_REQUIRE(dtype == LO_BF16 || dtype == LO_F16 || dtype == LO_F32, LO_ENOTSUP, "rms_norm_block: rows are bf16, fp16 or fp32");
+  LO_REQUIRE((!weight || weight_dtype == dtype || weight_dtype == LO_F32) && (!post_weight || post_weight_dtype == dtype || post_weight_dtype == LO_F32) &&
+                 (!gate || gate_dtype == dtype || gate_dtype == LO_F32),
+             LO_ENOTSUP, "rms_norm_block: weights and gate have the rows' type or are fp32");
+  LO_REQUIRE(q_form == LO_Q_NONE || q_form == LO_Q_INT8_ROWS || q_form == LO_Q_INT8_GROUPS || q_form == LO_Q_FP8_GROUPS, LO_EINVAL,
+             "rms_norm_block: unknown output form %d", q_form);
+  const bool groups = q_form == LO_Q_INT8_GROUPS || q_form == LO_Q_FP8_GROUPS;
+  LO_REQUIRE(H > 0 && H % (groups ? kGroup : 8) == 0, LO_EINVAL, "rms_norm_block: the hidden size (%lld) must be a multiple of %d", (long long)H,
+             groups ? kGroup : 8);
+  LO_REQUIRE(H <= kNormMaxH, LO_ENOTSUP, "rms_norm_block: rows of %lld values (at most %lld)", (long long)H, (long long)kNormMaxH);
+  LO_REQUIRE(eps >= 0.0f, LO_EINVAL, "rms_norm_block: eps must not be negative");
+  LO_REQUIRE(weight || (q_form == LO_Q_NONE && !normed_out), LO_EINVAL, "rms_norm_block: normed rows and codes need the weight of the norm");
+  LO_REQUIRE(!gate || (gate_rows > 0 && gate_stride >= 0), LO_EINVAL, "rms_norm_block: rows of the gate: stride %lld, each for %lld rows",
+             (long long)gate_stride, (long long)gate_rows);
+  if (M == 0) return LO_OK;
+  LO_REQUIRE(x && residual && residual_out && (q_form == LO_Q_NONE || (q && q_scale)) && (!weight || normed_out || q_form != LO_Q_NONE), LO_EINVAL,
+             "rms_norm_block: null pointer");
+  LO_REQUIRE(M == 1 || (x_stride >= H && residual_stride >= H), LO_EINVAL, "rms_norm_block: rows overlap (stride below %lld)", (long long)H);
+  const int64_t piece = dtype == LO_F32 ? 4 : 8, size = dtype == LO_F32 ? 4 : 2, gate_size = gate_dtype == LO_F32 ? 4 : 2;
+  LO_REQUIRE(x_stride % piece == 0 && residual_stride % piece == 0 && (!gate || !gate_channels || gate_stride * gate_size % 16 == 0), LO_EINVAL,
+             "rms_norm_block: row strides must keep rows 16-byte aligned");
+  const auto off = [](const void *p, unsigned al) { return (reinterpret_cast<uintptr_t>(p) & (al - 1)) != 0; };
+  LO_REQUIRE(!off(x, 16) && !off(residual, 16) && !off(weight, 16) && !off(post_weight, 16) && !off(residual_out, 16) && !off(normed_out, 16) &&
+                 !off(q, 8) && !off(q_scale, 4) && !off(gate, gate_channels ? 16 : static_cast<unsigned>(gate_size)),
+             LO_EINVAL, "rms_norm_block: rows, weights and a gate of channels must be 16-byte, q 8-byte aligned");
+  // the sum may take the place of a whole input, row by row; a row of it over another input row would be read too late
+  const uintptr_t z = reinterpret_cast<uintptr_t>(residual_out), z_end = z + M * H * size;
+  const auto meets = [&](const void *p, int64_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    return p && at < z_end && z < at + bytes;
+  };
+  const auto over = [&](const void *in, int64_t stride) {
+    return !(reinterpret_cast<uintptr_t>(in) == z && (stride == H || M == 1)) && meets(in, ((M - 1) * stride + H) * size);
+  };
+  LO_REQUIRE(!over(x, x_stride) && !over(residual, residual_stride) &&
+                 !meets(gate, (gate ? (M - 1) / gate_rows * gate_stride + (gate_channels ? H : 1) : 0) * gate_size) &&
+                 !meets(weight, H * (weight_dtype == LO_F32 ? 4 : 2)) && !meets(post_weight, H * (post_weight_dtype == LO_F32 ? 4 : 2)),
+             LO_EINVAL, "rms_norm_block: residual_out overlaps an input without being it");
+  const NormBlockArgs a{x, residual, post_weight, weight, gate, residual_out, normed_out, static_cast<int8_t *>(q), q_scale, x_stride, residual_stride,
+                        gate_stride, 0, gate ? static_cast<uint32_t>(gate_rows < M ? gate_rows : M) : 1u, static_cast<int32_t>(H), post_weight_dtype == LO_F32, weight_dtype == LO_F32,
+                        gate_dtype == LO_F32, gate && gate_channels, gate_sigmoid != 0, eps, scale, residual_scale};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == LO_BF16) launch_norm_block_form<LO_BF16>(q_form, a, M, s);
+  else if (dtype == LO_F16) launch_norm_block_form<LO_F16>(q_form, a, M, s);
+  else launch_norm_block_form<LO_F32>(q_form, a, M, s);
+  return check_launch("rms_norm_block");
 }

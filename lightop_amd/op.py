@@ -31,6 +31,16 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _strided_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as [rows, H] whose rows are contiguous and 16-byte aligned: a view where it can be."""
+    t = t.reshape(-1, t.shape[-1])
+    size = t.element_size()
+    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or (t.stride(0) >= t.shape[1]
+                                                                            and t.stride(0) * size % 16 == 0)):
+        return t
+    return _rows16(t)
+
+
 @contextlib.contextmanager
 def _on_device(t: torch.Tensor):
     if torch.cuda.current_device() == t.device.index:

@@ -691,6 +691,9 @@ int lo_rms_norm_block(const void *x, int dtype, int64_t x_stride, const void *re
 enum { LO_I8 = 3 };
 enum { LO_ACT_NONE = -1 };
 int64_t lo_gemm_bias_act_workspace_bytes(int dtype, int gated, int64_t M, int64_t N, int64_t K);
+/* Tokens and weight rows of the tile that such a call takes, and its parts of K (1 without a workspace). */
+int lo_gemm_bias_act_tile_query(int dtype, int gated, int64_t M, int64_t N, int64_t K, int has_workspace, int32_t *tile_m,
+                                int32_t *tile_n, int32_t *parts);
 int lo_gemm_bias_act(const void *a, int64_t a_stride, const void *b, int64_t b_stride, int dtype, const float *a_scale,
                      const float *b_scale, const void *bias, int bias_dtype, int activation, int gated, float scale,
                      const void *residual, int64_t residual_stride, void *c, int out_dtype, int64_t M, int64_t N,

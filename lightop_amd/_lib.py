@@ -122,6 +122,7 @@ SIGNATURES = {
                                   c_int, c_void_p, c_int, c_float, c_float, c_int64, c_int64, c_float, c_int, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_void_p]),
     "lo_gemm_bias_act_workspace_bytes": (c_int64, [c_int, c_int, c_int64, c_int64, c_int64]),
+    "lo_gemm_bias_act_tile_query": (c_int, [c_int, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
     "lo_gemm_bias_act": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float,
                                  c_void_p, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
 }

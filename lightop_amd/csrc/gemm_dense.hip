@@ -1,35 +1,45 @@
-// Entry points of the dense product with an epilogue (gemm_dense.h).
+// Entry points of the dense product with an epilogue (gemm_dense.h), and which of its kernels a call takes.
 #include "gemm_dense.h"
 
 namespace lo {
 
-// A wave takes 16 rows of A and 16 columns of C (gated: of both halves), operands straight from memory.
-template <int DT> __global__ __launch_bounds__(256) void gemm_dense_simple_kernel(const DenseArgs a) {
-  typedef Operand<DT> Op;
-  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, wave = threadIdx.x >> 6;
-  const int columns = static_cast<int>((a.N + 15) / 16);
-  const int64_t m = (static_cast<int64_t>(blockIdx.x / columns) * 4 + wave) * 16 + r, n0 = static_cast<int64_t>(blockIdx.x % columns) * 16;
-  const int64_t ma = m < a.M ? m : a.M - 1, nb = n0 + r < a.N ? n0 + r : a.N - 1;
-  const int8_t *const pa = a.A + ma * a.lda, *const pb = a.B + nb * a.ldb, *const pu = a.B + (nb + a.N) * a.ldb;
-  typename Op::Acc g = {}, u = {};
-  for (int k = 0; k < a.K; k += 64) {
-    const int at = k + q * 16;
-    v4i x = {}, w = {}, y = {};
-    if (at < a.K) {
-      x = *reinterpret_cast<const v4i *>(pa + at);
-      w = *reinterpret_cast<const v4i *>(pb + at);
-      if (a.gated) y = *reinterpret_cast<const v4i *>(pu + at);
+// Which tile, and how many parts of K: the smallest estimate of the time.  A K block takes a CU t1 us with one workgroup of the tile on it and
+// tn_us with as many as it holds (LDS); a workgroup starts and ends in `start` us; the parts are joined by a launch of kJoinUs that moves
+// them twice at kJoinBytes a us.
+struct DenseTile {
+  int tm, tn, held;
+  float t1, tn_us, start;
+};
+constexpr DenseTile kDenseTile[kDenseTiles] = {{256, 256, 1, 1.55f, 1.55f, 3.0f}, {192, 256, 1, 1.30f, 1.30f, 3.0f}, {128, 256, 1, 0.93f, 0.93f, 2.0f},
+                                               {128, 128, 1, 0.60f, 0.60f, 2.0f}, {64, 64, 2, 0.30f, 0.54f, 1.9f},   {64, 32, 3, 0.23f, 0.60f, 1.2f}};
+constexpr float kJoinUs = 3.2f, kJoinBytes = 4.7e6f;
+constexpr int kMostParts = 8, kLeastBlocks = 4; // of K, in a part
+constexpr int64_t kFewTokens = 16;              // gemm_dense_few_kernel
+struct DensePlan {
+  int tile, parts;
+};
+// Values of a row of the parts.
+static int64_t part_pitch(int64_t N, bool gated) { return (N + 3) / 4 * 4 * (gated ? 2 : 1); }
+static DensePlan plan_dense(int64_t M, int64_t N, int64_t KB, bool gated, bool may_split) {
+  if (M <= kFewTokens) return {kDenseFew, 1};
+  DensePlan best{kDenseFew, 1};
+  float least = 0.0f;
+  for (int i = 0; i < kDenseTiles; ++i) {
+    const DenseTile &t = kDenseTile[i];
+    const int64_t width = gated ? t.tn / 2 : t.tn, tiles = ((M + t.tm - 1) / t.tm) * ((N + width - 1) / width);
+    for (int parts = 1; parts <= (may_split && i >= kD128x256 ? kMostParts : 1); parts += parts < 4 ? 1 : 2) {
+      const int64_t bytes = parts * M * part_pitch(N, gated) * 4;
+      if (parts > 1 && KB / parts < kLeastBlocks) break;
+      const int64_t each = (tiles * parts + 255) / 256; // workgroups of a CU
+      const float blocks = static_cast<float>((KB + parts - 1) / parts);
+      const int64_t rounds = each / t.held, rest = each % t.held;
+      float us = static_cast<float>(rounds) * (t.start + blocks * t.tn_us);
+      if (rest) us += t.start + blocks * (t.t1 + (t.held > 1 ? (t.tn_us - t.t1) * static_cast<float>(rest - 1) / static_cast<float>(t.held - 1) : 0.0f));
+      if (parts > 1) us += kJoinUs + 2.0f * static_cast<float>(bytes) / kJoinBytes;
+      if (best.tile < 0 || us < least) best = {i, parts}, least = us;
     }
-    g = Op::mfma(w, x, g);
-    if (a.gated) u = Op::mfma(y, x, u);
   }
-  for (int i = 0; i < 4; ++i) {
-    const int64_t n = n0 + 4 * q + i;
-    if (m >= a.M || n >= a.N) continue;
-    float v = activate(a.act, dense_value(a, g[i], m, n));
-    if (a.gated) v *= dense_value(a, u[i], m, n + a.N);
-    dense_store(a, v, m, n);
-  }
+  return best;
 }
 
 constexpr int64_t kMostStride = 4 << 20; // bytes: 256 rows of a tile stay within 2^30
@@ -42,14 +52,30 @@ static int check_dense_sizes(int dtype, int64_t M, int64_t N, int64_t K) {
   LO_REQUIRE(M <= (1 << 24) && N <= (1 << 23), LO_ENOTSUP, "gemm_bias_act: %lld x %lld outputs (at most 2^24 x 2^23)", (long long)M, (long long)N);
   return LO_OK;
 }
+static int64_t k_blocks(int dtype, int64_t K) { return (K * (dtype == LO_I8 ? 1 : 2) + kBlockK - 1) / kBlockK; }
 
 } // namespace lo
 
 extern "C" int64_t lo_gemm_bias_act_workspace_bytes(int dtype, int gated, int64_t M, int64_t N, int64_t K) {
   using namespace lo;
-  (void)gated;
   const int rc = check_dense_sizes(dtype, M, N, K);
-  return rc;
+  if (rc) return rc;
+  if (N == 0) return 0;
+  const DensePlan p = plan_dense(M, N, k_blocks(dtype, K), gated != 0, true);
+  return p.parts > 1 ? p.parts * M * part_pitch(N, gated != 0) * 4 : 0;
+}
+
+extern "C" int lo_gemm_bias_act_tile_query(int dtype, int gated, int64_t M, int64_t N, int64_t K, int has_workspace, int32_t *tile_m,
+                                           int32_t *tile_n, int32_t *parts) {
+  using namespace lo;
+  const int rc = check_dense_sizes(dtype, M, N, K);
+  if (rc) return rc;
+  LO_REQUIRE(tile_m && tile_n && parts, LO_EINVAL, "gemm_bias_act_tile_query: null pointer");
+  const DensePlan p = plan_dense(M, N, k_blocks(dtype, K), gated != 0, has_workspace != 0);
+  *tile_m = p.tile == kDenseFew ? 16 : kDenseTile[p.tile].tm;
+  *tile_n = p.tile == kDenseFew ? 16 : kDenseTile[p.tile].tn;
+  *parts = p.parts;
+  return LO_OK;
 }
 
 extern "C" int lo_gemm_bias_act(const void *a, int64_t a_stride, const void *b, int64_t b_stride, int dtype, const float *a_scale, const float *b_scale,
@@ -86,15 +112,16 @@ extern "C" int lo_gemm_bias_act(const void *a, int64_t a_stride, const void *b, 
                  !meets(bias, rows * (bias_dtype == LO_F32 ? 4 : out_size)) &&
                  !(meets(residual, ((M - 1) * residual_stride + N) * out_size) && !(residual == c && (M == 1 || residual_stride == N))),
              LO_EINVAL, "gemm_bias_act: the output overlaps an input");
-  DenseArgs args{static_cast<const int8_t *>(a), static_cast<const int8_t *>(b), a_scale, b_scale, bias, residual, c, M, N, M == 1 ? N : residual_stride,
-                 static_cast<int32_t>(lda), static_cast<int32_t>(ldb), static_cast<int32_t>(K * size), activation, gated != 0, bias_dtype == LO_F32,
-                 out_dtype, scale};
+  const DenseArgs args{static_cast<const int8_t *>(a), static_cast<const int8_t *>(b), a_scale, b_scale, bias, residual, c, workspace, M, N,
+                 M == 1 ? N : residual_stride, static_cast<int32_t>(lda), static_cast<int32_t>(ldb), static_cast<int32_t>(K * size), activation,
+                 gated != 0, bias_dtype == LO_F32, out_dtype, scale, static_cast<int32_t>(k_blocks(dtype, K)), 0, 0, 1,
+                 static_cast<int32_t>(part_pitch(N, gated != 0))};
+  // (with less room than the parts take K stays whole: the order of the sum goes by whether there is a workspace, not by its size)
+  DensePlan p = plan_dense(M, N, args.KB, gated != 0, true);
+  if (p.parts > 1 && p.parts * M * args.pitch * 4 > (workspace ? workspace_bytes : 0)) p = plan_dense(M, N, args.KB, gated != 0, false);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t workgroups = (N + 15) / 16 * ((M + 63) / 64);
-  LO_REQUIRE(workgroups < (1 << 24), LO_ENOTSUP, "gemm_bias_act: %lld x %lld outputs", (long long)M, (long long)N);
-  const dim3 grid(static_cast<unsigned>(workgroups));
-  if (dtype == LO_BF16) hipLaunchKernelGGL((gemm_dense_simple_kernel<LO_BF16>), grid, dim3(256), 0, s, args);
-  else if (dtype == LO_F16) hipLaunchKernelGGL((gemm_dense_simple_kernel<LO_F16>), grid, dim3(256), 0, s, args);
-  else hipLaunchKernelGGL((gemm_dense_simple_kernel<LO_I8>), grid, dim3(256), 0, s, args);
-  return check_launch("gemm_bias_act");
+  const int rc = dtype == LO_BF16 ? launch_dense<LO_BF16>(args, p.tile, p.parts, s)
+                 : dtype == LO_F16 ? launch_dense<LO_F16>(args, p.tile, p.parts, s)
+                                   : launch_dense<LO_I8>(args, p.tile, p.parts, s);
+  return rc ? rc : check_launch("gemm_bias_act");
 }

@@ -6,6 +6,7 @@
 // whose scale it carries.
 #include "gemm.h"
 #include "fp8.h"
+#include "tiles.h"
 
 namespace lo {
 
@@ -72,18 +73,6 @@ __global__ __launch_bounds__(1024) void gemm_fp8_few_kernel(const Fp8GemmArgs a)
   store_c<DT>(a.C, m * a.N + n, v);
 }
 
-// Workgroups are dealt round-robin to the 8 XCDs: each takes a range of tiles of its own, in groups of G token tiles by all columns, so that
-// tiles at work at one time share rows and columns in its L2.
-__device__ __forceinline__ bool dense_tile(int bid, int m_tiles, int n_tiles, int G, int &mt, int &nt) {
-  const int total = m_tiles * n_tiles, per = (total + 7) / 8, id = (bid & 7) * per + (bid >> 3);
-  if ((bid >> 3) >= per || id >= total) return false;
-  const int first = id / (G * n_tiles) * G, in = id - first * n_tiles;
-  const int size = m_tiles - first < G ? m_tiles - first : G;
-  nt = in / size;
-  mt = first + in - nt * size;
-  return true;
-}
-
 // ---- tiles -----------------------------------------------------------------------------------------------------------------
 // Both operands go to LDS by direct loads, a K block to a stage of a ring of ST; 16-byte pieces of a row are swizzled by the row.  The rows'
 // scales go there four K blocks at a time (a scale is a line of its own to the texture path, whatever it fetches of it).  A wave keeps its
@@ -99,14 +88,6 @@ __device__ __forceinline__ bool dense_tile(int bid, int m_tiles, int n_tiles, in
 // (64 x 64, 64 x 32) and an XCD to each part of K are no faster (each pair of one run, so / as it is: 333 x 576 x 7168 13.1 / 13.3 us, 48 x 7168 x 2048 8.0 / 8.0; by themselves 12.3 and 7.7).
 // An fp32 output's exact products take their time in large sizes: 8192 x 4096 x 7168 510 us, 1531 x 7168 x 2048 59, 333 x 576 x 7168 15.0, 48 x 7168 x
 // 2048 10.0.
-__device__ __forceinline__ void copy16(brsrc r, int8_t *lds, int voff, int soff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 16, voff, soff, 0, 0);
-}
-// All but this wave's newest N copies have landed and what it has read from LDS is there, and the workgroup meets.
-template <int N> __device__ __forceinline__ void wait_barrier() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
-
 // PART: this workgroup's part of K only, its fp32 sums to a.part.
 template <int DT, int TM, int TN, int WM, int WN, int ST, bool PART>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_fp8_tile_kernel(const Fp8GemmArgs a, int group_m) {

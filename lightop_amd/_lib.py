@@ -165,6 +165,7 @@ class _NoHost:
 
     fused_experts = topk_softmax = fused_gate = _decline
     rms_norm_quant = group_quant_fp8 = gemm_fp8 = experts_fp8 = _decline
+    gemm_dense = rms_norm_block = _decline
 
 
 def host():
@@ -191,7 +192,8 @@ def host():
                                         "lo_fused_experts_workspace_bytes", "lo_topk_softmax", "lo_moe_fused_gate", "lo_last_error")),
                             (mod.bind_fp8, ("lo_rms_norm_quant", "lo_per_token_group_quant_fp8", "lo_act_mul_group_quant_fp8",
                                             "lo_gemm_w8a8_fp8_block", "lo_fused_experts_fp8", "lo_fused_experts_fp8_workspace_bytes",
-                                            "lo_gemm_w8a8_fp8_block_workspace_bytes"))):
+                                            "lo_gemm_w8a8_fp8_block_workspace_bytes")),
+                            (mod.bind_dense, ("lo_rms_norm_block", "lo_gemm_bias_act", "lo_gemm_bias_act_workspace_bytes"))):
             bind(*(ctypes.cast(getattr(handle, n), c_void_p).value for n in names))
         _host = mod
     return _host

@@ -1,5 +1,5 @@
-// Host path of the calls a serving loop makes on every step: the whole fused-experts layer, the two routers and the 8-bit operators
-// beside them.
+// Host path of the calls a serving loop makes on every step: the whole fused-experts layer, the two routers, the 8-bit operators
+// beside them and those of the dense blocks.
 //
 // A one-token layer is two kernel launches, 17 us of GPU time; marshalling the same call through Python (argument
 // checks on fifteen tensors, ctypes conversions, stream and workspace look-ups) took 25-27 us of host time and set
@@ -43,6 +43,9 @@ decltype(&lo_gemm_w8a8_fp8_block) g_gemm_fp8 = nullptr;
 decltype(&lo_gemm_w8a8_fp8_block_workspace_bytes) g_gemm_fp8_bytes = nullptr;
 decltype(&lo_fused_experts_fp8) g_experts_fp8 = nullptr;
 decltype(&lo_fused_experts_fp8_workspace_bytes) g_experts_fp8_bytes = nullptr;
+decltype(&lo_rms_norm_block) g_norm_block = nullptr;
+decltype(&lo_gemm_bias_act) g_gemm_dense = nullptr;
+decltype(&lo_gemm_bias_act_workspace_bytes) g_gemm_dense_bytes = nullptr;
 
 PyObject *s_preshuffled, *s_int4, *s_kmajor; // attribute names of weights in their load-time layout
 
@@ -582,6 +585,159 @@ PyObject *experts_fp8(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// A Python number; false: something else.
+bool number(PyObject *o, double &v) {
+  if (!PyFloat_Check(o) && !PyLong_Check(o)) return false;
+  v = PyFloat_AsDouble(o);
+  return true;
+}
+
+// gemm_dense(a, b, a_scale or None, b_scale or None, bias or None, residual or None, out or None, activation, gated, scale, dtype) -> tensor, or
+// None: not an ordinary call.  activation: LO_ACT_*; dtype: LO_* of the result.
+PyObject *gemm_dense(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  if (nargs != 11) {
+    PyErr_SetString(PyExc_TypeError, "gemm_dense takes 11 arguments");
+    return nullptr;
+  }
+  const at::Tensor *t[7];
+  for (int i = 0; i < 7; ++i) {
+    t[i] = nullptr;
+    if (!(i >= 2 && args[i] == Py_None) && !(t[i] = tensor_of(args[i]))) Py_RETURN_NONE;
+  }
+  double scale;
+  if (!PyLong_Check(args[7]) || !PyLong_Check(args[8]) || !PyLong_Check(args[10]) || !number(args[9], scale)) Py_RETURN_NONE;
+  const long act = PyLong_AsLong(args[7]), gated = PyLong_AsLong(args[8]), result = PyLong_AsLong(args[10]);
+  if (PyErr_Occurred()) return nullptr;
+  HANDLE_TH_ERRORS
+  const at::Tensor &a = *t[0], &b = *t[1], *as = t[2], *bs = t[3], *bias = t[4], *r = t[5], *to = t[6];
+  if (!a.is_cuda() || a.get_device() != device_now() || a.dim() < 1 || b.dim() != 2 || result < 0 || b.scalar_type() != a.scalar_type()) Py_RETURN_NONE;
+  const int dev = a.get_device();
+  const bool i8 = a.scalar_type() == at::kChar;
+  const int dtype = i8 ? LO_I8 : dtype_code(a.scalar_type());
+  if (!(i8 || dtype == LO_BF16 || dtype == LO_F16) || i8 != (as != nullptr) || i8 != (bs != nullptr) || !plain16(a, dev) || !plain16(b, dev))
+    Py_RETURN_NONE;
+  const int64_t K = b.size(1), rows = b.size(0), N = gated ? rows / 2 : rows, M = K ? a.numel() / K : 0;
+  if (K == 0 || K % (i8 ? 16 : 8) || a.size(-1) != K || M == 0 || N == 0 || (gated && rows % 2)) Py_RETURN_NONE;
+  auto sizes = a.sizes().vec();
+  if (i8) {
+    if (!plain(*as, dev) || !plain(*bs, dev) || as->scalar_type() != at::kFloat || bs->scalar_type() != at::kFloat || as->numel() != M ||
+        bs->numel() != rows || (bs->dim() != 1 && !(bs->dim() == 2 && bs->size(1) == 1)))
+      Py_RETURN_NONE;
+    sizes.back() = 1;
+    if (as->sizes() != at::IntArrayRef(sizes) && as->sizes() != at::IntArrayRef(sizes.data(), sizes.size() - 1)) Py_RETURN_NONE;
+  }
+  sizes.back() = N;
+  const at::ScalarType made = result == LO_BF16 ? at::kBFloat16 : result == LO_F16 ? at::kHalf : at::kFloat;
+  if (bias && (!plain(*bias, dev) || bias->dim() != 1 || bias->size(0) != rows || (bias->scalar_type() != made && bias->scalar_type() != at::kFloat)))
+    Py_RETURN_NONE;
+  for (const at::Tensor *v : {r, to})
+    if (v && (!plain(*v, dev) || v->scalar_type() != made || v->sizes() != at::IntArrayRef(sizes))) Py_RETURN_NONE;
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream();
+  const int64_t bytes = g_gemm_dense_bytes(dtype, static_cast<int>(gated), M, N, K);
+  if (bytes < 0) return raise(static_cast<int>(bytes));
+  if (bytes > 0 && capturing(stream)) Py_RETURN_NONE; // (its scratch belongs to the graph)
+  const void *ap = a.data_ptr(), *bp = b.data_ptr(), *biasp = bias ? bias->data_ptr() : nullptr, *rp = r ? r->data_ptr() : nullptr;
+  const float *asp = i8 ? as->data_ptr<float>() : nullptr, *bsp = i8 ? bs->data_ptr<float>() : nullptr;
+  const int bias_type = bias && bias->scalar_type() == at::kFloat ? LO_F32 : static_cast<int>(result);
+  const auto opts = a.options().requires_grad(false).dtype(made);
+  at::Tensor out;
+  if (to) out = *to;
+  int rc;
+  {
+    const NoGil nogil;
+    if (!to) out = at::empty(sizes, opts);
+    const auto call = [&](void *ws) {
+      return g_gemm_dense(ap, K, bp, K, dtype, asp, bsp, biasp, bias_type, static_cast<int>(act), static_cast<int>(gated), static_cast<float>(scale), rp,
+                          N, out.data_ptr(), static_cast<int>(result), M, N, K, ws, bytes, stream);
+    };
+    if (bytes == 0) {
+      rc = call(nullptr);
+    } else {
+      const std::shared_ptr<Scratch> ws = workspace_for(bytes, dev, stream);
+      const std::lock_guard<std::mutex> lock(ws->busy);
+      rc = call(ws->buf.data_ptr());
+    }
+  }
+  if (rc < 0) return raise(rc);
+  if (to) { // the caller's own object
+    Py_INCREF(args[6]);
+    return args[6];
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_block(x, residual, weight or None, post_weight or None, gate or None, residual_out or None, gate_sigmoid, scale, residual_scale, eps,
+//                form, return_normed) -> (residual, normed or None, q or None, scale or None), or None: not an ordinary call.
+PyObject *rms_norm_block(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  if (nargs != 12) {
+    PyErr_SetString(PyExc_TypeError, "rms_norm_block takes 12 arguments");
+    return nullptr;
+  }
+  const at::Tensor *t[6];
+  for (int i = 0; i < 6; ++i) {
+    t[i] = nullptr;
+    if (!(i >= 2 && args[i] == Py_None) && !(t[i] = tensor_of(args[i]))) Py_RETURN_NONE;
+  }
+  double scale, residual_scale, eps;
+  if (!PyLong_Check(args[6]) || !number(args[7], scale) || !number(args[8], residual_scale) || !number(args[9], eps) || !PyLong_Check(args[10]))
+    Py_RETURN_NONE;
+  const long sigmoid = PyLong_AsLong(args[6]), form = PyLong_AsLong(args[10]);
+  int normed = PyObject_IsTrue(args[11]);
+  if (normed < 0 || PyErr_Occurred()) return nullptr;
+  HANDLE_TH_ERRORS
+  const at::Tensor &x = *t[0], &r = *t[1], *w = t[2], *post = t[3], *gate = t[4], *to = t[5];
+  if (!x.is_cuda() || x.get_device() != device_now() || x.dim() < 1) Py_RETURN_NONE;
+  const int dev = x.get_device(), dtype = dtype_code(x.scalar_type());
+  const bool groups = form == LO_Q_INT8_GROUPS || form == LO_Q_FP8_GROUPS;
+  const int64_t H = x.size(-1);
+  if (dtype < 0 || H == 0 || H % (groups ? 128 : 8) || x.numel() == 0 || (!w && (form != LO_Q_NONE || normed))) Py_RETURN_NONE;
+  if (!plain16(x, dev) || !plain16(r, dev) || r.scalar_type() != x.scalar_type() || r.sizes() != x.sizes()) Py_RETURN_NONE;
+  for (const at::Tensor *v : {w, post})
+    if (v && (!plain16(*v, dev) || v->dim() != 1 || v->size(0) != H || (v->scalar_type() != x.scalar_type() && v->scalar_type() != at::kFloat)))
+      Py_RETURN_NONE;
+  if (to && (!plain16(*to, dev) || to->scalar_type() != x.scalar_type() || to->sizes() != x.sizes())) Py_RETURN_NONE;
+  const int64_t rows = x.numel() / H;
+  auto sizes = x.sizes().vec();
+  int64_t gate_stride = 0, gate_rows = rows;
+  bool channels = false;
+  if (gate) { // one row for all, a value or a row for each token; other layouts are sorted out in Python
+    if (!plain16(*gate, dev) || (gate->scalar_type() != x.scalar_type() && gate->scalar_type() != at::kFloat) || gate->dim() < 1) Py_RETURN_NONE;
+    channels = gate->size(-1) == H;
+    sizes.back() = 1;
+    if (channels && gate->sizes() == x.sizes()) gate_stride = H, gate_rows = 1;
+    else if (gate->sizes() == at::IntArrayRef(sizes)) gate_stride = 1, gate_rows = 1;
+    else if (!(channels && gate->dim() == 1)) Py_RETURN_NONE;
+    sizes.back() = H;
+  }
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream();
+  const auto code = [&](const at::Tensor *v) { return v && v->scalar_type() == at::kFloat ? LO_F32 : dtype; };
+  const auto at_of = [](const at::Tensor *v) -> const void * { return v ? v->data_ptr() : nullptr; };
+  const void *xp = x.data_ptr(), *rp = r.data_ptr(), *wp = at_of(w), *pp = at_of(post), *gp = at_of(gate);
+  const int wt = code(w), pt = code(post), gt = code(gate);
+  const auto opts = x.options().requires_grad(false);
+  at::Tensor out[4]; // residual, normed, q, scale
+  if (to) out[0] = *to;
+  int rc;
+  {
+    const NoGil nogil;
+    if (!to) out[0] = at::empty(sizes, opts);
+    if (w && (normed || form == LO_Q_NONE)) out[1] = at::empty(sizes, opts);
+    if (form != LO_Q_NONE) {
+      out[2] = at::empty(sizes, opts.dtype(form == LO_Q_FP8_GROUPS ? at::kFloat8_e4m3fn : at::kChar));
+      sizes.back() = groups ? H / 128 : 1;
+      out[3] = at::empty(sizes, opts.dtype(at::kFloat));
+    }
+    rc = g_norm_block(xp, dtype, H, rp, H, pp, pt, gp, gt, gate_stride, gate_rows, channels, static_cast<int>(sigmoid), wp, wt,
+                      static_cast<float>(scale), static_cast<float>(residual_scale), rows, H, static_cast<float>(eps), static_cast<int>(form),
+                      out[0].data_ptr(), out[1].defined() ? out[1].data_ptr() : nullptr, out[2].defined() ? out[2].data_ptr() : nullptr,
+                      out[3].defined() ? out[3].data_ptr<float>() : nullptr, stream);
+  }
+  if (rc < 0) return raise(rc);
+  return tuple_of(out, 4);
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(lo_fused_experts_block_int8, lo_fused_experts_channel_int8, lo_fused_experts_workspace_bytes, lo_topk_softmax,
 //      lo_moe_fused_gate, lo_last_error): addresses of the library's functions.
 PyObject *bind(PyObject *, PyObject *args) {
@@ -610,9 +766,20 @@ PyObject *bind_fp8(PyObject *, PyObject *args) {
   Py_RETURN_NONE;
 }
 
+// bind_dense(lo_rms_norm_block, lo_gemm_bias_act, lo_gemm_bias_act_workspace_bytes): those of the dense blocks.
+PyObject *bind_dense(PyObject *, PyObject *args) {
+  unsigned long long a[3];
+  if (!PyArg_ParseTuple(args, "KKK", &a[0], &a[1], &a[2])) return nullptr;
+  g_norm_block = reinterpret_cast<decltype(g_norm_block)>(a[0]);
+  g_gemm_dense = reinterpret_cast<decltype(g_gemm_dense)>(a[1]);
+  g_gemm_dense_bytes = reinterpret_cast<decltype(g_gemm_dense_bytes)>(a[2]);
+  Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, nullptr},
     {"bind_fp8", bind_fp8, METH_VARARGS, nullptr},
+    {"bind_dense", bind_dense, METH_VARARGS, nullptr},
     {"fused_experts", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(fused_experts)), METH_FASTCALL, nullptr},
     {"topk_softmax", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(topk_softmax)), METH_FASTCALL, nullptr},
     {"fused_gate", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(fused_gate)), METH_FASTCALL, nullptr},
@@ -620,6 +787,8 @@ PyMethodDef methods[] = {
     {"group_quant_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(group_quant_fp8)), METH_FASTCALL, nullptr},
     {"gemm_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(gemm_fp8)), METH_FASTCALL, nullptr},
     {"experts_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(experts_fp8)), METH_FASTCALL, nullptr},
+    {"gemm_dense", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(gemm_dense)), METH_FASTCALL, nullptr},
+    {"rms_norm_block", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(rms_norm_block)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -112,6 +112,10 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
 def _dense(name: str, a, b, a_scale, b_scale, bias, activation, gated: bool, scale: float, residual, out_dtype, out) -> torch.Tensor:
     if activation not in _ACTIVATIONS or (gated and activation is None):
         raise ValueError(f"{name}: unsupported activation {activation!r}")
+    made = (_lib._host or _lib.host()).gemm_dense(a, b, a_scale, b_scale, bias, residual, out, _ACTIVATIONS[activation], gated, scale,
+                                                  _OUT_DTYPES.get(out_dtype, -1))
+    if made is not None:
+        return made
     _one_device(a, b, a_scale, b_scale, bias, residual, out)
     int8 = a_scale is not None
     if a.dtype != b.dtype or (a.dtype != torch.int8 if int8 else a.dtype not in (torch.bfloat16, torch.float16)):
@@ -130,8 +134,6 @@ def _dense(name: str, a, b, a_scale, b_scale, bias, activation, gated: bool, sca
                  or a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32):
         raise RuntimeError(f"{name}: scales must be float32, one for a row: {tuple(a.shape[:-1])} and ({rows},), got "
                            f"{tuple(a_scale.shape)} {a_scale.dtype} and {tuple(b_scale.shape)} {b_scale.dtype}")
-    if out_dtype is None:
-        out_dtype = torch.bfloat16 if int8 else a.dtype
     if out_dtype not in _OUT_DTYPES:
         raise RuntimeError(f"{name}: out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
     if bias is not None and (bias.shape != (rows,) or bias.dtype not in (out_dtype, torch.float32)):
@@ -181,7 +183,7 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
     of 8; ``bias`` [N] of ``out_dtype`` or float32; ``activation`` None, "silu" or "gelu" (its erf form); ``residual`` [..., N] of
     ``out_dtype``.  Written into ``out`` (contiguous) where the caller brings it, ``residual`` itself to update it in place; any other
     overlap is refused."""
-    return _dense("gemm_bias_act", a, b, None, None, bias, activation, False, scale, residual, out_dtype, out)
+    return _dense("gemm_bias_act", a, b, None, None, bias, activation, False, scale, residual, out_dtype or a.dtype, out)
 
 
 def gemm_act_and_mul(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "silu",
@@ -189,7 +191,7 @@ def gemm_act_and_mul(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tens
     """Both projections of a gated block, activation and product in one: ``out = act(a b[:I]^T + bias[:I]) * (a b[I:]^T + bias[I:])``
     with ``b`` [2I, K], the gate's rows first as in the experts' ``w1``; ``activation`` "silu" or "gelu".  Nothing of it is
     rounded before the result; the rest as in ``gemm_bias_act``."""
-    return _dense("gemm_act_and_mul", a, b, None, None, bias, activation, True, 1.0, None, out_dtype, out)
+    return _dense("gemm_act_and_mul", a, b, None, None, bias, activation, True, 1.0, None, out_dtype or a.dtype, out)
 
 
 def gemm_w8a8_bias_act(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,

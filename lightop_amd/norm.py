@@ -141,6 +141,10 @@ def rms_norm_block(x: torch.Tensor, residual: torch.Tensor, weight: Optional[tor
         raise ValueError(f"rms_norm_block: unsupported gate_activation {gate_activation!r}")
     if weight is None and (form != _lib.LO_Q_NONE or return_normed):
         raise RuntimeError("rms_norm_block: normed rows and codes need the weight of the norm")
+    made = (_lib._host or _lib.host()).rms_norm_block(x, residual, weight, post_weight, gate, residual_out, _GATES[gate_activation], scale,
+                                                      residual_scale, eps, form, return_normed)
+    if made is not None:  # None: not an ordinary call (csrc/host_binding.cpp); checked and converted below
+        return RmsNormBlock(*(made if residual_out is None else (residual_out, *made[1:])))
     _one_device(x, residual, weight, post_weight, gate, residual_out)
     H = x.shape[-1] if x.dim() else 0
     unit = 8 if group_size is None else group_size

@@ -5,6 +5,8 @@
 // 64 values of 16 bits or 128 of int8, two matrix instructions of every 16 x 16 sums.  B (the weight) is the instructions' first
 // operand: a lane holds four neighbouring columns of C for one token.
 #pragma once
+#include <type_traits>
+
 #include "fp8.h"
 #include "gemm.h"
 #include "tiles.h"
@@ -28,9 +30,10 @@ constexpr int kBlockK = 128; // bytes
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
-// The operands' types: sixteen bytes a lane of 16 rows of either operand, 64 bytes of K, into the 16 x 16 sums.
+// The operands' types and the matrix instructions: sixteen bytes a lane of 16 rows of either operand, 64 bytes of K, into the 16 x 16 sums.
 template <int DT> struct Operand {
   typedef v4f Acc;
+  typedef float Sum;
   static __device__ __forceinline__ Acc mfma(const v4i a, const v4i b, const Acc c) {
     if constexpr (DT == LO_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
@@ -38,6 +41,7 @@ template <int DT> struct Operand {
 };
 template <> struct Operand<LO_I8> {
   typedef v4i Acc;
+  typedef int Sum;
   static __device__ __forceinline__ Acc mfma(const v4i a, const v4i b, const Acc c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 };
 
@@ -63,265 +67,233 @@ __device__ __forceinline__ float dense_result(const DenseArgs &a, float v, int64
 }
 
 // ---- up to 16 tokens ---------------------------------------------------------------------------------------------------------
-// A workgroup takes 16 rows of B (gated: eight of either projection) and all tokens; its waves share the K blocks and add their sums up through
-// LDS, in the same order every time.  Weights are read once, straight into registers, four K blocks of a wave in flight.
+// A workgroup takes 16 / C rows of B (gated: half of them of either projection) and all tokens, at most 16 / C; its waves share K and add
+// their sums up through LDS, in the same order every time.  With C > 1 the 16 rows of a matrix instruction's operands are C K blocks of the
+// workgroup's rows, and of the tokens; of its 16 x 16 sums those on the diagonal of C x C squares count, and are added up with the waves'.
+// Weights are read once, straight into registers, U instructions of a wave in flight.
 template <int DT>
-__global__ __launch_bounds__(1024) void gemm_dense_few_kernel(const DenseArgs a) {
+__global__ __launch_bounds__(512) void gemm_dense_few_kernel(const DenseArgs a, int lg) {
   typedef Operand<DT> Op;
-  typedef typename Op::Acc Acc;
-  __shared__ __attribute__((aligned(16))) int red[16][256]; // [wave][token][B's row]
+  __shared__ __attribute__((aligned(16))) int red[8][256]; // [wave][16 of tokens][16 of B's rows]
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (a.gated ? 8 : 16);
-  int64_t nb = n0 + (a.gated ? r & 7 : r);
-  nb = (nb < a.N ? nb : a.N - 1) + (a.gated && r >= 8 ? a.N : 0); // (rows and tokens past the end: the last one again, not stored)
-  const int8_t *const pb = a.B + nb * a.ldb + q * 16;
-  const int8_t *const pa = a.A + (r < a.M ? r : a.M - 1) * a.lda + q * 16;
-  Acc acc = {};
+  const int C = 1 << lg, width = 16 >> lg, half = a.gated ? width >> 1 : width; // rows of B; columns of the result
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * half;
+  const int row = r & (width - 1), block = r >> (4 - lg); // of the workgroup, of the C
+  int64_t nb = n0 + (row < half ? row : row - half);
+  nb = (nb < a.N ? nb : a.N - 1) + (row < half ? 0 : a.N); // (rows and tokens past the end: the last one again, not stored)
+  const int at0 = block * kBlockK + q * 16;
+  const int8_t *const pb = a.B + nb * a.ldb + at0;
+  const int8_t *const pa = a.A + (row < a.M ? row : a.M - 1) * a.lda + at0;
+  typename Op::Acc acc = {};
   constexpr int U = 4;
-  for (int kb0 = wave; kb0 < a.KB; kb0 += waves * U) {
+  const int step = C * kBlockK;
+  for (int k0 = wave * step; k0 < a.K; k0 += waves * U * step) {
     v4i w[U][2], x[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int kb = kb0 + u * waves, kc = (kb < a.KB ? kb : kb0) * kBlockK; // past the end: this one again, left out below
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int at = kc + q * 16 + h * 64 < a.K ? kc + h * 64 : -q * 16; // past the row's end: its first bytes, cleared below
+        const int k = k0 + u * waves * step + h * 64, at = k + at0 < a.K ? k : -at0; // past the row's end: its first bytes, cleared below
         w[u][h] = __builtin_nontemporal_load(reinterpret_cast<const v4i *>(pb + at));
         x[u][h] = *reinterpret_cast<const v4i *>(pa + at);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int kb = kb0 + u * waves;
-      if (kb >= a.KB) break;
+      if (k0 + u * waves * step >= a.K) break;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const bool in = kb * kBlockK + q * 16 + h * 64 < a.K;
+        const bool in = k0 + u * waves * step + h * 64 + at0 < a.K;
         acc = Op::mfma(in ? w[u][h] : v4i{}, in ? x[u][h] : v4i{}, acc);
       }
     }
   }
   *reinterpret_cast<v4i *>(&red[wave][r * 16 + 4 * q]) = __builtin_bit_cast(v4i, acc);
   __syncthreads();
-  if (threadIdx.x >= 256) return;
-  const int64_t m = threadIdx.x >> 4;
-  const int c = threadIdx.x & 15;
-  const int64_t n = n0 + c;
-  if (m >= a.M || n >= a.N || (a.gated && c >= 8)) return;
-  typedef decltype(Acc{}[0] + Acc{}[0]) T;
-  auto sum = [&](int at) __attribute__((always_inline)) {
-    T v = __builtin_bit_cast(T, red[0][at]);
-    for (int i = 1; i < waves; ++i) v += __builtin_bit_cast(T, red[i][at]);
-    return v;
-  };
-  float v = activate(a.act, dense_value(a, sum(threadIdx.x), m, n));
-  if (a.gated) v *= dense_value(a, sum(threadIdx.x + 8), m, n + a.N);
-  store_value(a.C, a.out, m * a.N + n, dense_result(a, v, m, n));
+  for (int i = threadIdx.x; i < static_cast<int>(a.M) * half; i += blockDim.x) {
+    const int m = i / half, c = i % half;
+    const int64_t n = n0 + c;
+    if (n >= a.N) continue;
+    auto sum = [&](int col) __attribute__((always_inline)) {
+      typename Op::Sum v = 0;
+      for (int j = 0; j < waves; ++j)
+        for (int k = 0; k < C; ++k) v += __builtin_bit_cast(typename Op::Sum, red[j][(k * width + m) * 16 + k * width + col]);
+      return v;
+    };
+    float v = activate(a.act, dense_value(a, sum(c), m, n));
+    if (a.gated) v *= dense_value(a, sum(c + half), m, n + a.N);
+    store_value(a.C, a.out, m * a.N + n, dense_result(a, v, m, n));
+  }
 }
 
 // ---- tiles -----------------------------------------------------------------------------------------------------------------
-// Both operands go to LDS by direct loads, a K block to a stage of a ring of ST; 16-byte pieces of a row are swizzled by the row.  A wave keeps its
-// weight fragments of a K block in registers and walks through its token fragments, a step each: the next token fragment is read while this
-// one is multiplied.  The workgroup meets in front of the last step, when nobody reads the K block's stage any more: behind the barrier the
-// next block's first operands are read under the step's products, and the copies of the block that takes the stage over are asked
-// for, a few a step.  A gated product's fragments hold eight weight rows of either projection.
-//
-// PART: this workgroup's part of K only, its sums to a.part.
-constexpr int dense_staging(int tn, int wm, int wn, int round) { return wm * wn * round * 16 * (tn / wn * 4 + 16); } // bytes
-// Token fragments of a wave that the epilogue turns around at a time: all of them, or half where they do not fit.
-constexpr int dense_round(int tm, int tn, int wm, int wn) { return dense_staging(tn, wm, wn, tm / wm / 16) <= 160 * 1024 ? tm / wm / 16 : tm / wm / 32; }
-constexpr int dense_lds(int tm, int tn, int wm, int wn, int st, bool part) {
-  const int ring = st * (tm + tn) * kBlockK, staging = part ? 0 : dense_staging(tn, wm, wn, dense_round(tm, tn, wm, wn));
+// Both operands go to LDS by direct loads, S K blocks to a stage of a ring; 16-byte pieces of a row are swizzled by the row.  A gated
+// product's fragments of 16 rows hold eight of either projection.
+constexpr int dense_staging(int tn, int wm, int wn, int rows) { return wm * wn * rows * (tn / wn * 4 + 16); } // bytes
+// Token fragments of a wave that the epilogue turns around at a time: all of them, or half where they do not fit into the ring.
+constexpr int dense_round(int tm, int tn, int wm, int wn, int ring) {
+  return (dense_staging(tn, wm, wn, tm / wm) <= ring || tm / wm / 16 % 2 ? tm : tm / 2) / wm / 16;
+}
+constexpr int dense_lds(int tm, int tn, int wm, int wn, int ring, bool part) {
+  const int staging = part ? 0 : dense_staging(tn, wm, wn, dense_round(tm, tn, wm, wn, ring) * 16);
   return ring > staging ? ring : staging;
 }
-template <int DT, int TM, int TN, int WM, int WN, int ST, bool PART>
-__global__ __launch_bounds__(WM * WN * 64) void gemm_dense_tile_kernel(const DenseArgs a, int group_m) {
-  typedef Operand<DT> Op;
-  typedef typename Op::Acc Acc;
-  constexpr int kWaves = WM * WN;
-  constexpr int FM = TM / WM / 16, FN = TN / WN / 16;            // fragments of a wave: tokens, weights
-  constexpr int kA = TM / 8 / kWaves, kB = TN / 8 / kWaves, kCopies = kA + kB; // 1 KB copies of a stage, of a wave
-  constexpr int kStep = (kCopies + FM - 1) / FM;                               // copies of a step
-  constexpr int kStage = (TM + TN) * kBlockK;
-  // Two stages leave a copy little time.  The weights' part of a stage is free long before the tokens', once every wave has its fragments:
-  // the workgroup meets in front of step kMid too, and from there on the next but one K block's weights are asked for, its tokens
-  // behind the last step's barrier.
-  constexpr bool kApart = ST == 2;
-  constexpr int kMid = kA - 1;
-  static_assert(!kApart || (kA >= 2 && kMid < FM - 1), "steps for the copies");
-  static_assert(TM / 8 % kWaves == 0 && TN / 8 % kWaves == 0 && (TM / WM) % 16 == 0 && (TN / WN) % 16 == 0 && FM % 2 == 0, "tile");
-  extern __shared__ __attribute__((aligned(16))) int8_t smem[];
-  int mt, nt;
-  const int split = PART ? blockIdx.y : 0;
-  if (!dense_tile(blockIdx.x, a.m_tiles, a.n_tiles, group_m, mt, nt)) return;
-  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
-  const int first = PART ? static_cast<int>(static_cast<int64_t>(a.KB) * split / a.splits) : 0;
-  const int KB = (PART ? static_cast<int>(static_cast<int64_t>(a.KB) * (split + 1) / a.splits) : a.KB) - first;
-  const bool gated = a.gated;
-  const int width = gated ? TN / 2 : TN; // columns of C
-  const int64_t m0 = static_cast<int64_t>(mt) * TM, n0 = static_cast<int64_t>(nt) * width;
-  const int rows = static_cast<int>(a.M - m0 < TM ? a.M - m0 : TM), cols = static_cast<int>(a.N - n0 < width ? a.N - n0 : width);
-  const int8_t *const pa = a.A + m0 * a.lda + first * kBlockK;
-  const int8_t *pb[kB]; // of the projection that a copy's eight rows belong to
-  const uint32_t endA = static_cast<uint32_t>((rows - 1) * a.lda + a.K - first * kBlockK), endB = static_cast<uint32_t>((cols - 1) * a.ldb + a.K - first * kBlockK);
+
+// What a workgroup multiplies, and how its waves' copies find it.
+template <int TM, int TN, int WM, int WN, bool PART> struct DenseTileOf {
+  static constexpr int kWaves = WM * WN, kA = TM / 8 / kWaves, kB = TN / 8 / kWaves; // 1 KB copies of a K block, of a wave
+  static_assert(TM / 8 % kWaves == 0 && TN / 8 % kWaves == 0 && TM / WM % 16 == 0 && TN / WN % 16 == 0, "tile");
+  int lane, r, q, wave, wm, wn, split, rows, cols, KB, tail;
+  int64_t m0, n0;
+  brsrc A, B[2]; // B's rows; gated: of the two projections
   int voff[kA + kB];
-  const int piece = ((lane & 7) ^ (lane >> 3)) * 16;
+  int lds[2]; // the lane's pieces of a fragment
+  __device__ __forceinline__ bool start(const DenseArgs &a, int group_m) {
+    int mt, nt;
+    split = PART ? blockIdx.y : 0;
+    if (!dense_tile(blockIdx.x, a.m_tiles, a.n_tiles, group_m, mt, nt)) return false;
+    mt = __builtin_amdgcn_readfirstlane(mt), nt = __builtin_amdgcn_readfirstlane(nt); // (a division's results: the descriptors go to scalar registers)
+    lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+    const int first = PART ? static_cast<int>(static_cast<int64_t>(a.KB) * split / a.splits) : 0;
+    KB = (PART ? static_cast<int>(static_cast<int64_t>(a.KB) * (split + 1) / a.splits) : a.KB) - first;
+    const int width = a.gated ? TN / 2 : TN; // columns of C
+    m0 = static_cast<int64_t>(mt) * TM, n0 = static_cast<int64_t>(nt) * width;
+    rows = static_cast<int>(a.M - m0 < TM ? a.M - m0 : TM), cols = static_cast<int>(a.N - n0 < width ? a.N - n0 : width);
+    const int left = a.K - first * kBlockK; // bytes of a row from this part on
+    A = make_rsrc(a.A + m0 * a.lda + first * kBlockK, static_cast<uint32_t>((rows - 1) * a.lda + left));
 #pragma unroll
-  for (int j = 0; j < kA; ++j) voff[j] = ((wave * kA + j) * 8 + (lane >> 3)) * a.lda + piece;
+    for (int p = 0; p < 2; ++p) B[p] = make_rsrc(a.B + (n0 + (a.gated && p ? a.N : 0)) * a.ldb + first * kBlockK, static_cast<uint32_t>((cols - 1) * a.ldb + left));
+    const int piece = ((lane & 7) ^ (lane >> 3)) * 16;
 #pragma unroll
-  for (int j = 0; j < kB; ++j) {
-    const int g = wave * kB + j; // eight rows; a fragment is two of them
-    pb[j] = a.B + (n0 + (gated && (g & 1) ? a.N : 0)) * a.ldb + first * kBlockK;
-    voff[kA + j] = ((gated ? g >> 1 : g) * 8 + (lane >> 3)) * a.ldb + piece;
-  }
-  // Past a row's end (in its last K block, where K is no multiple of 128 bytes) a piece's offset is past the extents, which end below 2^30.
-  const int last = a.KB - 1 - first, tail = last * kBlockK + piece < a.K - first * kBlockK ? 0 : 1 << 30;
-  // Copy c of K block kb.  What lies past the extents is written as zero: rows past the end, and past the last K block, where the extents are
-  // empty, all of it (the copies, which the waits count, fetch nothing).
-  auto copy = [&](int c, int kb, int stage) __attribute__((always_inline)) {
-    const bool in = kb < KB;
-    const int at = voff[c] + (kb == last ? tail : 0), soff = in ? kb * kBlockK : 0;
-    if (c < kA) copy16(make_rsrc(pa, in ? endA : 0u), smem + stage * kStage + (wave * kA + c) * 1024, at, soff);
-    else copy16(make_rsrc(pb[c - kA], in ? endB : 0u), smem + stage * kStage + TM * kBlockK + (wave * kB + c - kA) * 1024, at, soff);
-  };
-  const int lds[2] = {r * kBlockK + ((q ^ (r & 7)) * 16), r * kBlockK + (((q + 4) ^ (r & 7)) * 16)};
-  const int8_t *const sa = smem + wm * (TM / WM) * kBlockK, *const sb = smem + (TM + wn * (TN / WN)) * kBlockK;
-  auto read = [&](const int8_t *base, int f, int h, int stage) __attribute__((always_inline)) {
-    return *reinterpret_cast<const v4i *>(base + stage * kStage + f * 2048 + lds[h]);
-  };
-  Acc acc[FM][FN];
+    for (int j = 0; j < kA; ++j) voff[j] = ((wave * kA + j) * 8 + (lane >> 3)) * a.lda + piece;
 #pragma unroll
-  for (int m = 0; m < FM; ++m)
-#pragma unroll
-    for (int n = 0; n < FN; ++n) acc[m][n] = Acc{};
-
-  if constexpr (kApart) {
-#pragma unroll
-    for (int c = 0; c < kCopies; ++c) copy(c, 0, 0);
-#pragma unroll
-    for (int c = kA; c < kCopies; ++c) copy(c, 1, 1);
-    copy(0, 1, 1);
-    wait_barrier<kB + 1>();
-  } else {
-#pragma unroll
-    for (int i = 0; i < ST; ++i)
-#pragma unroll
-      for (int c = 0; c < (i < ST - 1 ? kCopies : kStep); ++c) copy(c, i, i);
-    wait_barrier<(ST - 2) * kCopies + kStep>();
-  }
-  v4i w[2][FN], x[2][2]; // [half of the K block][fragment], [step][half]
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int n = 0; n < FN; ++n) w[h][n] = read(sb, n, h, 0);
-    x[0][h] = read(sa, 0, h, 0);
-  }
-  int stage = 0;
-  for (int kb = 0; kb < KB; ++kb) {
-    const int next = stage == ST - 1 ? 0 : stage + 1, prev = stage == 0 ? ST - 1 : stage - 1;
-#pragma unroll
-    for (int m = 0; m < FM; ++m) {
-      const int cur = m & 1;
-      if (m + 1 < FM) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) x[cur ^ 1][h] = read(sa, m + 1, h, stage);
-      } else {
-        wait_barrier<kApart ? kB : (ST - 2) * kCopies>();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) x[cur ^ 1][h] = read(sa, 0, h, next);
-      }
-      if constexpr (kApart) {
-        if (m == kMid) asm volatile("s_barrier" ::: "memory"); // (every wave has used its weights: they are in registers)
-        if (m + 1 == FM) {
-          copy(0, kb + 2, stage);
-        } else if (m < kMid) {
-          copy(m + 1, kb + 1, next);
-        } else {
-#pragma unroll
-          for (int c = 0; c < kB; ++c)
-            if (c * (FM - 1 - kMid) / kB == m - kMid) copy(kA + c, kb + 2, stage);
-        }
-      } else { // the stage that the last barrier freed
-#pragma unroll
-        for (int c = 0; c < kStep; ++c) {
-          const int at = (m + 1 == FM ? 0 : m + 1) * kStep + c;
-          if (at < kCopies) copy(at, m + 1 == FM ? kb + ST : kb + ST - 1, m + 1 == FM ? stage : prev);
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int n = 0; n < FN; ++n) {
-          acc[m][n] = Op::mfma(w[h][n], x[cur][h], acc[m][n]);
-          if (m + 1 == FM) w[h][n] = read(sb, n, h, next);
-        }
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-#pragma unroll
-      for (int n = 0; n < 2 * FN; ++n) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        if (n < 2) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-        if (m + 1 == FM) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+    for (int j = 0; j < kB; ++j) {
+      const int g = wave * kB + j; // eight rows; a fragment is two of them
+      voff[kA + j] = ((a.gated ? g >> 1 : g) * 8 + (lane >> 3)) * a.ldb + piece;
     }
-    stage = next;
+    // Past a row's end (in its last K block, where K is no multiple of 128 bytes) a piece's offset is past the extents, which end at 2^30 at the most.
+    tail = (KB - 1) * kBlockK + piece < left ? 0 : 1 << 30;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) lds[h] = r * kBlockK + (((h * 4 + q) ^ (r & 7)) * 16);
+    return true;
   }
-  wait_barrier<0>(); // no copy lands in what the epilogue uses, or outlives the workgroup
+  // Copy c of K block kb.  What lies past the extents is written as zero: rows past the end, and past the last K block all of it (the copies,
+  // which the waits count, fetch nothing).
+  __device__ __forceinline__ void copy(int c, int kb, int8_t *to_a, int8_t *to_b) const {
+    const int at = voff[c] + (kb < KB - 1 ? 0 : kb == KB - 1 ? tail : 1 << 30), soff = kb < KB ? kb * kBlockK : 0;
+    if (c < kA) copy16(A, to_a + (wave * kA + c) * 1024, at, soff);
+    else copy16((wave * kB + c - kA) & 1 ? B[1] : B[0], to_b + (wave * kB + c - kA) * 1024, at, soff);
+  }
+};
 
+// Rows of COLS fp32 values in a wave's LDS, COLS * 4 + 16 bytes apart.  Gated: eights of either projection in turn.
+// Activates them where they lie (gated: the gate's, times the other's).
+template <int ROWS, int COLS, bool GATED> __device__ __forceinline__ void dense_activate(int act, int8_t *stg, int lane) {
+  constexpr int kFours = COLS / (GATED ? 8 : 4); // of a row
+#pragma unroll 2
+  for (int i = lane; i < ROWS * kFours; i += 64) {
+    const int k = i % kFours, slot = GATED ? (k >> 1) * 16 + (k & 1) * 4 : k * 4;
+    v4f *const p = reinterpret_cast<v4f *>(stg + i / kFours * (COLS * 4 + 16) + slot * 4);
+    v4f v = *p;
+    if (act == LO_ACT_SILU) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = silu_f32(v[j]);
+    } else if (act == LO_ACT_GELU) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = gelu_f32(v[j]);
+    }
+    if constexpr (GATED) v = v * p[2];
+    *p = v;
+  }
+  lds_order();
+}
+// Stores them, scaled and the residual added, in whole pieces of 16 bytes: `in` rows of C from value c0 on (of R from r0), `left` columns.
+template <int ROWS, int COLS, bool GATED, int OUT>
+__device__ __forceinline__ void dense_rows(const DenseArgs &a, const int8_t *stg, int lane, int64_t c0, int64_t r0, int in, int left) {
+  constexpr int V = OUT == LO_F32 ? 4 : 8, kLanes = (GATED ? COLS / 2 : COLS) / V, kTurns = (ROWS * kLanes + 63) / 64, U = kTurns < 4 ? kTurns : 4;
+  typedef std::conditional_t<OUT == LO_F32, v4f, v8u16> Piece;
+  typedef std::conditional_t<OUT == LO_F32, float, uint16_t> Value;
+#pragma unroll 1
+  for (int first = 0; first < kTurns; first += U) {
+    Piece add[U] = {};
+    if (a.R) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = (first + u) * 64 + lane, row = i / kLanes, c = i % kLanes * V;
+        if (row < in && c < left) add[u] = *reinterpret_cast<const Piece *>(static_cast<const Value *>(a.R) + r0 + row * a.rs + c);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = (first + u) * 64 + lane, row = i / kLanes, c = i % kLanes * V;
+      if (row >= in || c >= left) continue;
+      const v4f *const p = reinterpret_cast<const v4f *>(stg + row * (COLS * 4 + 16) + (GATED ? (c >> 3) * 16 + (c & 7) : c) * 4);
+      Piece o;
+#pragma unroll
+      for (int j = 0; j < V; j += 4) {
+        const v4f v = p[j / 4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (OUT == LO_F32) o[j + k] = a.R ? __builtin_fmaf(a.scale, v[k], add[u][j + k]) : a.scale * v[k];
+          else o[j + k] = from_f32<OUT>(a.R ? __builtin_fmaf(a.scale, v[k], to_f32<OUT>(add[u][j + k])) : a.scale * v[k]);
+        }
+      }
+      *reinterpret_cast<Piece *>(static_cast<Value *>(a.C) + c0 + row * a.N + c) = o;
+    }
+  }
+}
+
+// What becomes of a workgroup's sums.  PART: they go to a.part.  RING: bytes of LDS that are free by now.
+template <int DT, int TM, int TN, int WM, int WN, bool PART, int RING, int FM, int FN>
+__device__ __forceinline__ void dense_finish(const DenseArgs &a, const DenseTileOf<TM, TN, WM, WN, PART> &t, typename Operand<DT>::Acc (&acc)[FM][FN],
+                                             int8_t *smem) {
   constexpr int kCols = TN / WN; // B's rows of a wave
   if constexpr (PART) {
 #pragma unroll
     for (int m = 0; m < FM; ++m) {
-      const int mr = wm * (TM / WM) + m * 16 + r;
-      int *const row = static_cast<int *>(a.part) + (split * a.M + m0 + mr) * a.pitch + n0;
+      const int mr = t.wm * (TM / WM) + m * 16 + t.r;
+      int *const row = static_cast<int *>(a.part) + (t.split * a.M + t.m0 + mr) * a.pitch + t.n0;
 #pragma unroll
       for (int n = 0; n < FN; ++n) {
-        const int c = gated ? (wn * kCols + n * 16) / 2 + 4 * (q & 1) : wn * kCols + n * 16 + 4 * q;
-        if (mr < rows && c < cols) *reinterpret_cast<v4i *>(row + c + (gated && q >= 2 ? a.pitch / 2 : 0)) = __builtin_bit_cast(v4i, acc[m][n]);
+        const int c = a.gated ? (t.wn * kCols + n * 16) / 2 + 4 * (t.q & 1) : t.wn * kCols + n * 16 + 4 * t.q;
+        if (mr < t.rows && c < t.cols) *reinterpret_cast<v4i *>(row + c + (a.gated && t.q >= 2 ? a.pitch / 2 : 0)) = __builtin_bit_cast(v4i, acc[m][n]);
       }
     }
   } else {
     // A wave turns its tokens around in LDS, kRound fragments of them at a time, in fp32 (its own part; LDS operations of a wave execute in
     // order), and stores whole pieces of rows, activated and the residual added: 16 bytes a lane, or, where rows of either do not begin on 16
     // bytes, a value a lane.
-    constexpr int kPitch = kCols * 4 + 16, kRound = dense_round(TM, TN, WM, WN), kRows = kRound * 16;
-    int8_t *const stg = smem + wave * kRows * kPitch;
+    constexpr int kPitch = kCols * 4 + 16, kRound = dense_round(TM, TN, WM, WN, RING), kRows = kRound * 16;
+    int8_t *const stg = smem + t.wave * kRows * kPitch;
     const int size = a.out == LO_F32 ? 4 : 2;
     const bool whole = ((a.N * size | (a.R ? a.rs * size : 0) | static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.C) | reinterpret_cast<uintptr_t>(a.R))) & 15) == 0;
-    const int out_cols = gated ? kCols / 2 : kCols; // of C, of this wave
-    const int64_t nw = n0 + wn * out_cols;
-    const int left = cols - wn * out_cols; // of them in C
+    const int of_c = t.wn * (a.gated ? kCols / 2 : kCols); // this wave's first column of C
+    const int64_t nw = t.n0 + of_c;
+    const int left = t.cols - of_c;
     float bs[FN][4], bias[FN][4], as[FM];
 #pragma unroll
     for (int n = 0; n < FN; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int64_t c = nw + (gated ? n * 8 + 4 * (q & 1) : n * 16 + 4 * q) + i;
-        const int64_t at = (c < a.N ? c : a.N - 1) + (gated && q >= 2 ? a.N : 0);
+        const int64_t c = nw + (a.gated ? n * 8 + 4 * (t.q & 1) : n * 16 + 4 * t.q) + i;
+        const int64_t at = (c < a.N ? c : a.N - 1) + (a.gated && t.q >= 2 ? a.N : 0);
         if constexpr (DT == LO_I8) bs[n][i] = a.Bs[at];
         bias[n][i] = a.bias ? load_value(a.bias, a.bias_f32 ? LO_F32 : a.out, at) : 0.0f;
       }
 #pragma unroll
     for (int m = 0; m < FM; ++m) {
-      const int row = wm * (TM / WM) + m * 16 + r;
-      if constexpr (DT == LO_I8) as[m] = a.As[m0 + (row < rows ? row : rows - 1)];
+      const int row = t.wm * (TM / WM) + m * 16 + t.r;
+      if constexpr (DT == LO_I8) as[m] = a.As[t.m0 + (row < t.rows ? row : t.rows - 1)];
     }
-    // a row's values from column c: of the gate (or of C), and of the other projection
-    auto place = [&](int row, int c) __attribute__((always_inline)) {
-      return reinterpret_cast<const float *>(stg + row * kPitch) + (gated ? (c >> 3) * 16 + (c & 7) : c);
+    const auto each = [&](auto gated, auto type, int64_t c0, int64_t r0, int in) __attribute__((always_inline)) {
+      dense_rows<kRows, kCols, decltype(gated)::value, decltype(type)::value>(a, stg, t.lane, c0, r0, in, left);
     };
-    auto four = [&](int row, int c, float *v) __attribute__((always_inline)) {
-      const float *const p = place(row, c);
-      const v4f g = *reinterpret_cast<const v4f *>(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = activate(a.act, g[i]);
-      if (gated) {
-        const v4f u = *reinterpret_cast<const v4f *>(p + 8);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] *= u[i];
-      }
+    const auto of_type = [&](auto gated, int64_t c0, int64_t r0, int in) __attribute__((always_inline)) {
+      if (a.out == LO_BF16) each(gated, std::integral_constant<int, LO_BF16>{}, c0, r0, in);
+      else if (a.out == LO_F16) each(gated, std::integral_constant<int, LO_F16>{}, c0, r0, in);
+      else each(gated, std::integral_constant<int, LO_F32>{}, c0, r0, in);
     };
 #pragma unroll
     for (int round = 0; round < FM / kRound; ++round) {
@@ -337,52 +309,25 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_dense_tile_kernel(const Den
             if constexpr (DT == LO_I8) o[i] = o[i] * as[m] * bs[n][i];
             if (a.bias) o[i] += bias[n][i];
           }
-          *reinterpret_cast<v4f *>(stg + (m % kRound * 16 + r) * kPitch + (n * 16 + 4 * q) * 4) = o;
+          *reinterpret_cast<v4f *>(stg + (m % kRound * 16 + t.r) * kPitch + (n * 16 + 4 * t.q) * 4) = o;
         }
       }
       lds_order();
-      const int row0 = wm * (TM / WM) + round * kRows, in = rows - row0 < kRows ? rows - row0 : kRows;
-      const int64_t c0 = (m0 + row0) * a.N + nw, r0 = (m0 + row0) * a.rs + nw;
-      if (whole && a.out != LO_F32) {
-        const int lanes = out_cols / 8; // of a row
-#pragma unroll 1
-        for (int i = lane; i < kRows * lanes; i += 64) {
-          const int row = i / lanes, c = i % lanes * 8;
-          if (row >= in || c >= left) continue;
-          v8u16 o, add = {};
-          if (a.R) add = *reinterpret_cast<const v8u16 *>(static_cast<const uint16_t *>(a.R) + r0 + row * a.rs + c);
-          float v[8];
-          four(row, c, v);
-          four(row, c + 4, v + 4);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v[i] = a.R ? __builtin_fmaf(a.scale, v[i], a.out == LO_BF16 ? bf16_to_f32(add[i]) : f16_to_f32(add[i])) : a.scale * v[i];
-            o[i] = to_half(a.out, v[i]);
-          }
-          *reinterpret_cast<v8u16 *>(static_cast<uint16_t *>(a.C) + c0 + row * a.N + c) = o;
-        }
+      const int row0 = t.wm * (TM / WM) + round * kRows, in = t.rows - row0 < kRows ? t.rows - row0 : kRows;
+      const int64_t c0 = (t.m0 + row0) * a.N + nw, r0 = (t.m0 + row0) * a.rs + nw;
+      if (a.gated) dense_activate<kRows, kCols, true>(a.act, stg, t.lane);
+      else if (a.act != LO_ACT_NONE) dense_activate<kRows, kCols, false>(a.act, stg, t.lane);
+      if (whole && a.gated) {
+        of_type(std::true_type{}, c0, r0, in);
       } else if (whole) {
-        const int lanes = out_cols / 4;
-#pragma unroll 1
-        for (int i = lane; i < kRows * lanes; i += 64) {
-          const int row = i / lanes, c = i % lanes * 4;
-          if (row >= in || c >= left) continue;
-          v4f add = {0.0f, 0.0f, 0.0f, 0.0f}, o;
-          if (a.R) add = *reinterpret_cast<const v4f *>(static_cast<const float *>(a.R) + r0 + row * a.rs + c);
-          float v[4];
-          four(row, c, v);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = a.R ? __builtin_fmaf(a.scale, v[i], add[i]) : a.scale * v[i];
-          *reinterpret_cast<v4f *>(static_cast<float *>(a.C) + c0 + row * a.N + c) = o;
-        }
+        of_type(std::false_type{}, c0, r0, in);
       } else {
 #pragma unroll 1
-        for (int i = lane; i < kRows * out_cols; i += 64) {
-          const int row = i / out_cols, c = i % out_cols;
-          if (row >= in || c >= left) continue;
-          const float *const p = place(row, c);
-          const float v = activate(a.act, p[0]) * (gated ? p[8] : 1.0f);
-          store_value(a.C, a.out, c0 + row * a.N + c, dense_result(a, v, m0 + row0 + row, nw + c));
+        for (int i = t.lane; i < kRows * kCols; i += 64) {
+          const int row = i / kCols, slot = i % kCols, c = a.gated ? (slot >> 4) * 8 + (slot & 7) : slot;
+          if (row >= in || c >= left || (a.gated && (slot & 8))) continue;
+          const float v = *reinterpret_cast<const float *>(stg + row * kPitch + slot * 4);
+          store_value(a.C, a.out, c0 + row * a.N + c, dense_result(a, v, t.m0 + row0 + row, nw + c));
         }
       }
       lds_order();
@@ -390,9 +335,163 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_dense_tile_kernel(const Den
   }
 }
 
+// A wave holds its fragments of a whole stage in registers, and the next stage's are read while they are multiplied: the workgroup meets once a
+// stage, when the next one has landed and everybody's reads of this one are done, so that the ring is refilled from there on and an LDS
+// round trip lies under a stage's products.
+template <int DT, int TM, int TN, int WM, int WN, int S, int ST, bool PART>
+__global__ __launch_bounds__(WM * WN * 64) void gemm_dense_ring_kernel(const DenseArgs a, int group_m) {
+  typedef Operand<DT> Op;
+  constexpr int FM = TM / WM / 16, FN = TN / WN / 16; // fragments of a wave: tokens, weights
+  constexpr int kBlock = (TM + TN) * kBlockK, kStage = S * kBlock;
+  DenseTileOf<TM, TN, WM, WN, PART> t;
+  constexpr int kPer = t.kA + t.kB, kCopies = S * kPer; // of a K block, of a stage
+  static_assert(ST >= 2, "ring");
+  extern __shared__ __attribute__((aligned(16))) int8_t smem[];
+  if (!t.start(a, group_m)) return;
+  auto copy = [&](int i, int st, int stage) __attribute__((always_inline)) {
+    int8_t *const to = smem + stage * kStage + i / kPer * kBlock;
+    t.copy(i % kPer, st * S + i / kPer, to, to + TM * kBlockK);
+  };
+  const int8_t *const sa = smem + t.wm * (TM / WM) * kBlockK, *const sb = smem + (TM + t.wn * (TN / WN)) * kBlockK;
+  struct Fragments {
+    v4i x[S][2][FM], w[S][2][FN];
+  };
+  auto read = [&](Fragments &f, int stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int m = 0; m < FM; ++m) f.x[s][h][m] = *reinterpret_cast<const v4i *>(sa + stage * kStage + s * kBlock + m * 2048 + t.lds[h]);
+#pragma unroll
+        for (int n = 0; n < FN; ++n) f.w[s][h][n] = *reinterpret_cast<const v4i *>(sb + stage * kStage + s * kBlock + n * 2048 + t.lds[h]);
+      }
+  };
+  typename Op::Acc acc[FM][FN];
+#pragma unroll
+  for (int m = 0; m < FM; ++m)
+#pragma unroll
+    for (int n = 0; n < FN; ++n) acc[m][n] = typename Op::Acc{};
+#pragma unroll
+  for (int i = 0; i < ST; ++i)
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) copy(c, i, i);
+  Fragments f[2];
+  wait_barrier<(ST - 1) * kCopies>();
+  read(f[0], 0);
+  const int stages = (t.KB + S - 1) / S;
+  int stage = 0;
+  auto step = [&](Fragments &now, Fragments &then, int st) __attribute__((always_inline)) {
+    const int next = stage == ST - 1 ? 0 : stage + 1;
+    wait_barrier<(ST - 2) * kCopies>();
+    read(then, next);
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) copy(c, st + ST, stage);
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int m = 0; m < FM; ++m)
+#pragma unroll
+          for (int n = 0; n < FN; ++n) acc[m][n] = Op::mfma(now.w[s][h][n], now.x[s][h][m], acc[m][n]);
+    constexpr int kProducts = S * 2 * FM * FN, kReads = S * 2 * (FM + FN);
+#pragma unroll
+    for (int i = 0; i < kProducts; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (i < kReads) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      if (i < kCopies) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+    }
+    if constexpr (kReads > kProducts) __builtin_amdgcn_sched_group_barrier(0x100, kReads - kProducts, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    stage = next;
+  };
+  for (int st = 0; st < stages; st += 2) {
+    step(f[0], f[1], st);
+    if (st + 1 < stages) step(f[1], f[0], st + 1);
+  }
+  wait_barrier<0>(); // no copy lands in what the epilogue uses, or outlives the workgroup
+  dense_finish<DT, TM, TN, WM, WN, PART, ST * kStage>(a, t, acc, smem);
+}
+
+// The largest tiles, whose fragments of a K block do not fit into the registers twice.  A wave keeps its weight fragments of a K block in registers and
+// walks through its token fragments, a step each: the next token fragment is read while this one is multiplied.  The workgroup meets in front of
+// the last step, when nobody reads the K block's place any more and the next one has landed: behind the barrier its first operands are read under
+// the step's products.  The weights' half of a place is free long before the tokens', once every wave has its fragments: the workgroup
+// meets in front of step kMid too, and from there on the next but one K block's weights are asked for, its tokens behind the last barrier.
+template <int DT, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64) void gemm_dense_step_kernel(const DenseArgs a, int group_m) {
+  typedef Operand<DT> Op;
+  constexpr int FM = TM / WM / 16, FN = TN / WN / 16; // fragments of a wave: tokens, weights
+  constexpr int kStage = (TM + TN) * kBlockK;
+  DenseTileOf<TM, TN, WM, WN, false> t;
+  constexpr int kA = t.kA, kB = t.kB, kMid = kA - 1;
+  static_assert(kMid >= 1 && kMid < FM - 1 && FM % 2 == 0, "steps for the copies");
+  extern __shared__ __attribute__((aligned(16))) int8_t smem[];
+  if (!t.start(a, group_m)) return;
+  const int8_t *const sa = smem + t.wm * (TM / WM) * kBlockK, *const sb = smem + (TM + t.wn * (TN / WN)) * kBlockK;
+  auto copy = [&](int c, int kb, int place) __attribute__((always_inline)) { t.copy(c, kb, smem + place * kStage, smem + place * kStage + TM * kBlockK); };
+  auto read = [&](const int8_t *base, int f, int h, int place) __attribute__((always_inline)) {
+    return *reinterpret_cast<const v4i *>(base + place * kStage + f * 2048 + t.lds[h]);
+  };
+  typename Op::Acc acc[FM][FN];
+#pragma unroll
+  for (int m = 0; m < FM; ++m)
+#pragma unroll
+    for (int n = 0; n < FN; ++n) acc[m][n] = typename Op::Acc{};
+#pragma unroll
+  for (int c = 0; c < kA + kB; ++c) copy(c, 0, 0);
+#pragma unroll
+  for (int c = kA; c < kA + kB; ++c) copy(c, 1, 1);
+  copy(0, 1, 1);
+  wait_barrier<kB + 1>();
+  v4i w[2][FN], x[2][2]; // [half of the K block][fragment], [step][half]
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int n = 0; n < FN; ++n) w[h][n] = read(sb, n, h, 0);
+    x[0][h] = read(sa, 0, h, 0);
+  }
+  int place = 0;
+  for (int kb = 0; kb < t.KB; ++kb) {
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
+      const int cur = m & 1;
+      const bool over = m + 1 == FM;
+      if (over) wait_barrier<kB>();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) x[cur ^ 1][h] = read(sa, over ? 0 : m + 1, h, over ? place ^ 1 : place);
+      if (m == kMid) asm volatile("s_barrier" ::: "memory"); // (every wave has used its weights: they are in registers)
+      if (over) copy(0, kb + 2, place);
+      else if (m < kMid) copy(m + 1, kb + 1, place ^ 1);
+#pragma unroll
+      for (int c = 0; c < kB; ++c)
+        if (!over && kMid + c * (FM - 1 - kMid) / kB == m) copy(kA + c, kb + 2, place);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < FN; ++n) {
+          acc[m][n] = Op::mfma(w[h][n], x[cur][h], acc[m][n]);
+          if (over) w[h][n] = read(sb, n, h, place ^ 1);
+        }
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+      for (int n = 0; n < 2 * FN; ++n) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (n < 2) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        if (over) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    place ^= 1;
+  }
+  wait_barrier<0>(); // no copy lands in what the epilogue uses, or outlives the workgroup
+  dense_finish<DT, TM, TN, WM, WN, false, 2 * kStage>(a, t, acc, smem);
+}
+
 // The parts of K added up in their order, and the epilogue.
 template <int DT> __global__ __launch_bounds__(256) void gemm_dense_join_kernel(const DenseArgs a) {
-  typedef decltype(typename Operand<DT>::Acc{}[0] + typename Operand<DT>::Acc{}[0]) T;
+  typedef typename Operand<DT>::Sum T;
   const int half = a.gated ? a.pitch / 2 : a.pitch;
   const int64_t quads = a.M * (half / 4), step = a.M * a.pitch;
   // whole quads are stored where rows begin on a quad: c may begin on any value
@@ -433,60 +532,70 @@ template <int DT> __global__ __launch_bounds__(256) void gemm_dense_join_kernel(
   }
 }
 
-template <int DT, int TM, int TN, int WM, int WN, int ST, bool PART> static int launch_dense_parts(const DenseArgs &a, hipStream_t stream) {
-  constexpr int lds = dense_lds(TM, TN, WM, WN, ST, PART);
-  static_assert(lds <= 160 * 1024, "LDS");
-  const auto kernel = gemm_dense_tile_kernel<DT, TM, TN, WM, WN, ST, PART>;
-  static unsigned long long done = 0;
-  const int rc = reserve_lds_once(reinterpret_cast<const void *>(kernel), lds, &done);
+template <class K> static int launch_dense_kernel(const DenseArgs &a, K kernel, int lds, int threads, unsigned long long *done, hipStream_t stream) {
+  const int rc = reserve_lds_once(reinterpret_cast<const void *>(kernel), lds, done);
   if (rc) return rc;
   const int group_m = a.m_tiles < 4 ? a.m_tiles : 4;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((a.m_tiles * a.n_tiles + 7) / 8 * 8), PART ? a.splits : 1), dim3(WM * WN * 64), lds,
-                     stream, a, group_m);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((a.m_tiles * a.n_tiles + 7) / 8 * 8), a.splits), dim3(threads), lds, stream, a, group_m);
   return LO_OK;
 }
-template <int DT, int TM, int TN, int WM, int WN, int ST, bool SPLIT> static int launch_dense_tile(DenseArgs a, int parts, hipStream_t stream) {
-  const int64_t width = a.gated ? TN / 2 : TN, m_tiles = (a.M + TM - 1) / TM, n_tiles = (a.N + width - 1) / width;
+static int set_dense_tiles(DenseArgs &a, int tm, int tn) {
+  const int64_t width = a.gated ? tn / 2 : tn, m_tiles = (a.M + tm - 1) / tm, n_tiles = (a.N + width - 1) / width;
   LO_REQUIRE(m_tiles * n_tiles < (1 << 22), LO_ENOTSUP, "gemm_bias_act: %lld x %lld outputs", (long long)a.M, (long long)a.N);
   a.m_tiles = static_cast<int32_t>(m_tiles);
   a.n_tiles = static_cast<int32_t>(n_tiles);
-  if constexpr (SPLIT) {
-    if (parts > 1) {
-      a.splits = parts;
-      const int rc = launch_dense_parts<DT, TM, TN, WM, WN, ST, true>(a, stream);
-      if (rc) return rc;
-      const int64_t blocks = (a.M * ((a.gated ? a.pitch / 2 : a.pitch) / 4) + 255) / 256;
-      hipLaunchKernelGGL((gemm_dense_join_kernel<DT>), dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, a);
-      return LO_OK;
-    }
-  }
-  return launch_dense_parts<DT, TM, TN, WM, WN, ST, false>(a, stream);
+  return LO_OK;
+}
+template <int DT, int TM, int TN, int WM, int WN> static int launch_dense_step(DenseArgs a, hipStream_t stream) {
+  constexpr int ring = 2 * (TM + TN) * kBlockK, lds = dense_lds(TM, TN, WM, WN, ring, false);
+  static_assert(lds <= 160 * 1024, "LDS");
+  static unsigned long long done = 0;
+  const int rc = set_dense_tiles(a, TM, TN);
+  return rc ? rc : launch_dense_kernel(a, gemm_dense_step_kernel<DT, TM, TN, WM, WN>, lds, WM * WN * 64, &done, stream);
+}
+template <int DT, int TM, int TN, int WM, int WN, int S, int ST> static int launch_dense_ring(DenseArgs a, int parts, hipStream_t stream) {
+  constexpr int ring = ST * S * (TM + TN) * kBlockK, lds = dense_lds(TM, TN, WM, WN, ring, false);
+  static_assert(lds <= 160 * 1024, "LDS");
+  static unsigned long long done[2] = {0, 0};
+  int rc = set_dense_tiles(a, TM, TN);
+  if (rc) return rc;
+  if (parts <= 1) return launch_dense_kernel(a, gemm_dense_ring_kernel<DT, TM, TN, WM, WN, S, ST, false>, lds, WM * WN * 64, &done[0], stream);
+  a.splits = parts;
+  rc = launch_dense_kernel(a, gemm_dense_ring_kernel<DT, TM, TN, WM, WN, S, ST, true>, ring, WM * WN * 64, &done[1], stream);
+  if (rc) return rc;
+  const int64_t blocks = (a.M * ((a.gated ? a.pitch / 2 : a.pitch) / 4) + 255) / 256;
+  hipLaunchKernelGGL((gemm_dense_join_kernel<DT>), dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, a);
+  return LO_OK;
+}
+// C (as a power of two) and the waves: see the kernel.
+template <int DT> static int launch_dense_few(const DenseArgs &a, int lg, int waves, hipStream_t stream) {
+  const int64_t width = (16 >> lg) / (a.gated ? 2 : 1);
+  hipLaunchKernelGGL((gemm_dense_few_kernel<DT>), dim3(static_cast<unsigned>((a.N + width - 1) / width)), dim3(waves * 64), 0, stream, a, lg);
+  return LO_OK;
 }
 
-enum { kD256, kD192, kD128x256, kD128, kD64, kD64x32, kDenseTiles };
+enum { kD256, kD192, kD128x256, kD128x192, kD128, kD96, kD64x128, kD64, kD64x32, kD32, kDenseTiles };
 constexpr int kDenseFew = -1; // in a tile's place: up to 16 tokens, gemm_dense_few_kernel
-// One operand type's kernels (gemm_dense_*.hip).
+// One operand type's kernels (gemm_dense_*.hip).  parts: of K; of the kernel of few tokens lg + 8 * waves.
 template <int DT> int launch_dense(const DenseArgs &a, int tile, int parts, hipStream_t stream);
 template <> int launch_dense<LO_BF16>(const DenseArgs &a, int tile, int parts, hipStream_t stream);
 template <> int launch_dense<LO_F16>(const DenseArgs &a, int tile, int parts, hipStream_t stream);
 template <> int launch_dense<LO_I8>(const DenseArgs &a, int tile, int parts, hipStream_t stream);
-#define LO_DENSE_LAUNCHERS(DT)                                                                                                    \
-  template <> int launch_dense<DT>(const DenseArgs &a, int tile, int parts, hipStream_t stream) {                                  \
-    switch (tile) {                                                                                                                \
-    case kD256: return launch_dense_tile<DT, 256, 256, 2, 4, 2, false>(a, parts, stream);                                          \
-    case kD192: return launch_dense_tile<DT, 192, 256, 2, 4, 2, false>(a, parts, stream);                                          \
-    case kD128x256: return launch_dense_tile<DT, 128, 256, 2, 4, 3, true>(a, parts, stream);                                       \
-    case kD128: return launch_dense_tile<DT, 128, 128, 2, 4, 4, true>(a, parts, stream);                                           \
-    case kD64: return launch_dense_tile<DT, 64, 64, 2, 2, 4, true>(a, parts, stream);                                              \
-    case kD64x32: return launch_dense_tile<DT, 64, 32, 2, 2, 4, true>(a, parts, stream);                                           \
-    default: {                                                                                                                     \
-      const int waves = a.KB >= 16 ? 16 : a.KB >= 8 ? 8 : 4;                                                                       \
-      const int64_t width = a.gated ? 8 : 16;                                                                                      \
-      hipLaunchKernelGGL((gemm_dense_few_kernel<DT>), dim3(static_cast<unsigned>((a.N + width - 1) / width)), dim3(waves * 64), 0, \
-                         stream, a);                                                                                               \
-      return LO_OK;                                                                                                                \
-    }                                                                                                                              \
-    }                                                                                                                              \
+#define LO_DENSE_LAUNCHERS(DT)                                                                   \
+  template <> int launch_dense<DT>(const DenseArgs &a, int tile, int parts, hipStream_t stream) { \
+    switch (tile) {                                                                               \
+    case kD256: return launch_dense_step<DT, 256, 256, 2, 4>(a, stream);                          \
+    case kD192: return launch_dense_step<DT, 192, 256, 2, 4>(a, stream);                          \
+    case kD128x256: return launch_dense_ring<DT, 128, 256, 2, 4, 1, 3>(a, parts, stream);         \
+    case kD128x192: return launch_dense_ring<DT, 128, 192, 2, 4, 1, 3>(a, parts, stream);         \
+    case kD128: return launch_dense_ring<DT, 128, 128, 2, 4, 1, 4>(a, parts, stream);             \
+    case kD96: return launch_dense_ring<DT, 96, 96, 2, 2, 1, 3>(a, parts, stream);                \
+    case kD64x128: return launch_dense_ring<DT, 64, 128, 2, 4, 1, 4>(a, parts, stream);           \
+    case kD64: return launch_dense_ring<DT, 64, 64, 2, 2, 1, 4>(a, parts, stream);                \
+    case kD64x32: return launch_dense_ring<DT, 64, 32, 2, 2, 1, 6>(a, parts, stream);             \
+    case kD32: return launch_dense_ring<DT, 32, 32, 1, 2, 2, 4>(a, parts, stream);                \
+    default: return launch_dense_few<DT>(a, parts & 7, parts >> 3, stream);                       \
+    }                                                                                             \
   }
 
 } // namespace lo

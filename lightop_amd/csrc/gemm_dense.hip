@@ -3,6 +3,8 @@
 
 namespace lo {
 
+static int64_t k_blocks(int dtype, int64_t K) { return (K * (dtype == LO_I8 ? 1 : 2) + kBlockK - 1) / kBlockK; }
+
 // Which tile, and how many parts of K: the smallest estimate of the time.  A K block takes a CU t1 us with one workgroup of the tile on it and
 // tn_us with as many as it holds (LDS); a workgroup starts and ends in `start` us; the parts are joined by a launch of kJoinUs that moves
 // them twice at kJoinBytes a us.
@@ -10,19 +12,34 @@ struct DenseTile {
   int tm, tn, held;
   float t1, tn_us, start;
 };
-constexpr DenseTile kDenseTile[kDenseTiles] = {{256, 256, 1, 1.55f, 1.55f, 3.0f}, {192, 256, 1, 1.30f, 1.30f, 3.0f}, {128, 256, 1, 0.93f, 0.93f, 2.0f},
-                                               {128, 128, 1, 0.60f, 0.60f, 2.0f}, {64, 64, 2, 0.30f, 0.54f, 1.9f},   {64, 32, 3, 0.23f, 0.60f, 1.2f}};
-constexpr float kJoinUs = 3.2f, kJoinBytes = 4.7e6f;
+constexpr DenseTile kDenseTile[kDenseTiles] = {{256, 256, 1, 1.24f, 1.24f, 17.8f}, {192, 256, 1, 0.95f, 0.95f, 14.8f}, {128, 256, 1, 0.80f, 0.80f, 8.8f},
+                                               {128, 192, 1, 0.60f, 0.60f, 7.8f},  {128, 128, 1, 0.49f, 0.49f, 6.4f},  {96, 96, 2, 0.41f, 0.68f, 5.4f},
+                                               {64, 128, 1, 0.37f, 0.37f, 4.7f},   {64, 64, 2, 0.25f, 0.47f, 4.2f},    {64, 32, 2, 0.19f, 0.33f, 3.9f},
+                                               {32, 32, 2, 0.11f, 0.25f, 3.7f}};
+constexpr float kJoinUs = 3.2f, kJoinBytes = 5.0e6f;
 constexpr int kMostParts = 8, kLeastBlocks = 4; // of K, in a part
-constexpr int64_t kFewTokens = 16;              // gemm_dense_few_kernel
 struct DensePlan {
-  int tile, parts;
+  int tile, parts; // of K
+  int few;         // gemm_dense_few_kernel: C, as a power of two, + 8 * waves
 };
 // Values of a row of the parts.
 static int64_t part_pitch(int64_t N, bool gated) { return (N + 3) / 4 * 4 * (gated ? 2 : 1); }
-static DensePlan plan_dense(int64_t M, int64_t N, int64_t KB, bool gated, bool may_split) {
-  if (M <= kFewTokens) return {kDenseFew, 1};
-  DensePlan best{kDenseFew, 1};
+// Whether gemm_dense_few_kernel takes a call.  us, it / the best tile: bf16, 8 tokens 4096 x 7168 16.1 / 16.1, 576 x 7168 10.2 / 9.8, 12: 17.3 / 16.0,
+// 16.1 / 9.9; int8, 12 tokens 4096 x 7168 10.4 / 12.4, 16: 11.2 / 12.3, gated 2048 x 7168 12.0 / 12.6, 576 x 7168 10.2 / 8.5.
+static bool few_tokens(int dtype, int64_t M, int64_t rows) { return M <= 8 || (dtype == LO_I8 && M <= 16 && rows >= 1024); }
+static DensePlan plan_dense(int dtype, int64_t M, int64_t N, int64_t K, bool gated, bool may_split) {
+  const int64_t KB = k_blocks(dtype, K);
+  if (few_tokens(dtype, M, gated ? 2 * N : N)) {
+    const int most = gated ? 3 : 4;
+    const int64_t rows = gated ? 2 * N : N;
+    int lg = 0, waves = 1;
+    while (lg < 3 && M <= 4 >> lg) ++lg;
+    while (lg < most && M <= 8 >> lg && (rows << lg) < 16 * 256) ++lg;
+    const int64_t workgroups = ((rows << lg) + 15) / 16, steps = (KB + (1 << lg) - 1) >> lg;
+    while (waves < 8 && workgroups * waves <= 1024 && steps >= 3 * waves) waves *= 2;
+    return {kDenseFew, 1, lg + 8 * waves};
+  }
+  DensePlan best{kDenseFew, 1, 0};
   float least = 0.0f;
   for (int i = 0; i < kDenseTiles; ++i) {
     const DenseTile &t = kDenseTile[i];
@@ -36,7 +53,7 @@ static DensePlan plan_dense(int64_t M, int64_t N, int64_t KB, bool gated, bool m
       float us = static_cast<float>(rounds) * (t.start + blocks * t.tn_us);
       if (rest) us += t.start + blocks * (t.t1 + (t.held > 1 ? (t.tn_us - t.t1) * static_cast<float>(rest - 1) / static_cast<float>(t.held - 1) : 0.0f));
       if (parts > 1) us += kJoinUs + 2.0f * static_cast<float>(bytes) / kJoinBytes;
-      if (best.tile < 0 || us < least) best = {i, parts}, least = us;
+      if (best.tile < 0 || us < least) best = {i, parts, 0}, least = us;
     }
   }
   return best;
@@ -52,7 +69,6 @@ static int check_dense_sizes(int dtype, int64_t M, int64_t N, int64_t K) {
   LO_REQUIRE(M <= (1 << 24) && N <= (1 << 23), LO_ENOTSUP, "gemm_bias_act: %lld x %lld outputs (at most 2^24 x 2^23)", (long long)M, (long long)N);
   return LO_OK;
 }
-static int64_t k_blocks(int dtype, int64_t K) { return (K * (dtype == LO_I8 ? 1 : 2) + kBlockK - 1) / kBlockK; }
 
 } // namespace lo
 
@@ -61,7 +77,7 @@ extern "C" int64_t lo_gemm_bias_act_workspace_bytes(int dtype, int gated, int64_
   const int rc = check_dense_sizes(dtype, M, N, K);
   if (rc) return rc;
   if (N == 0) return 0;
-  const DensePlan p = plan_dense(M, N, k_blocks(dtype, K), gated != 0, true);
+  const DensePlan p = plan_dense(dtype, M, N, K, gated != 0, true);
   return p.parts > 1 ? p.parts * M * part_pitch(N, gated != 0) * 4 : 0;
 }
 
@@ -71,7 +87,7 @@ extern "C" int lo_gemm_bias_act_tile_query(int dtype, int gated, int64_t M, int6
   const int rc = check_dense_sizes(dtype, M, N, K);
   if (rc) return rc;
   LO_REQUIRE(tile_m && tile_n && parts, LO_EINVAL, "gemm_bias_act_tile_query: null pointer");
-  const DensePlan p = plan_dense(M, N, k_blocks(dtype, K), gated != 0, has_workspace != 0);
+  const DensePlan p = plan_dense(dtype, M, N, K, gated != 0, has_workspace != 0);
   *tile_m = p.tile == kDenseFew ? 16 : kDenseTile[p.tile].tm;
   *tile_n = p.tile == kDenseFew ? 16 : kDenseTile[p.tile].tn;
   *parts = p.parts;
@@ -117,11 +133,12 @@ extern "C" int lo_gemm_bias_act(const void *a, int64_t a_stride, const void *b, 
                  gated != 0, bias_dtype == LO_F32, out_dtype, scale, static_cast<int32_t>(k_blocks(dtype, K)), 0, 0, 1,
                  static_cast<int32_t>(part_pitch(N, gated != 0))};
   // (with less room than the parts take K stays whole: the order of the sum goes by whether there is a workspace, not by its size)
-  DensePlan p = plan_dense(M, N, args.KB, gated != 0, true);
-  if (p.parts > 1 && p.parts * M * args.pitch * 4 > (workspace ? workspace_bytes : 0)) p = plan_dense(M, N, args.KB, gated != 0, false);
+  DensePlan p = plan_dense(dtype, M, N, K, gated != 0, true);
+  if (p.parts > 1 && p.parts * M * args.pitch * 4 > (workspace ? workspace_bytes : 0)) p = plan_dense(dtype, M, N, K, gated != 0, false);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int rc = dtype == LO_BF16 ? launch_dense<LO_BF16>(args, p.tile, p.parts, s)
-                 : dtype == LO_F16 ? launch_dense<LO_F16>(args, p.tile, p.parts, s)
-                                   : launch_dense<LO_I8>(args, p.tile, p.parts, s);
+  const int parts = p.tile == kDenseFew ? p.few : p.parts;
+  const int rc = dtype == LO_BF16 ? launch_dense<LO_BF16>(args, p.tile, parts, s)
+                 : dtype == LO_F16 ? launch_dense<LO_F16>(args, p.tile, parts, s)
+                                   : launch_dense<LO_I8>(args, p.tile, parts, s);
   return rc ? rc : check_launch("gemm_bias_act");
 }

@@ -1,6 +1,10 @@
 """What the dense blocks' operators refuse, before any GPU call: through the C entry points, and through Python on CPU tensors."""
+import ctypes
+
 import pytest
 import torch
+
+import dense_ref as ref
 
 
 @pytest.fixture(scope="module")
@@ -106,3 +110,39 @@ def test_names_are_reachable():
     assert lightop.norm.rms_norm_block is lightop_amd.norm.rms_norm_block
     for name in ("gemm_bias_act", "gemm_act_and_mul", "gemm_w8a8_bias_act", "gemm_w8a8_act_and_mul"):
         assert getattr(lightop.gemmopt, name) is getattr(lightop_amd.gemmopt, name) and name in lightop_amd.gemmopt.__all__
+
+
+def _tile(lib, dtype, gated, M, N, K, workspace):
+    a = [ctypes.c_int32() for _ in range(3)]
+    assert lib.lo_gemm_bias_act_tile_query(dtype, gated, M, N, K, workspace, *(ctypes.byref(v) for v in a)) == 0
+    return tuple(v.value for v in a)
+
+
+@pytest.mark.parametrize("tile,size", ref.TILE_SIZES, ids=str)
+def test_tile_of_the_sizes_that_the_gpu_tests_take(lib, tile, size):
+    M, N, K = size
+    tm, tn, split, gated = tile
+    for dtype, k in ((BF16, K), (F16, K), (I8, 2 * K)):
+        assert _tile(lib, dtype, gated, M, N, k, 1)[:2] == (tm, tn) and (_tile(lib, dtype, gated, M, N, k, 1)[2] > 1) == split
+        assert (lib.lo_gemm_bias_act_workspace_bytes(dtype, gated, M, N, k) > 0) == split
+        assert _tile(lib, dtype, gated, M, N, k, 0)[2] == 1
+
+
+def test_every_tile_has_sizes(lib):
+    """Over many sizes no call takes a tile, whole or in parts, that the list above leaves out, but for 128 x 256 in parts."""
+    seen = set()
+    for M in (9, 17, 33, 65, 100, 200, 400, 800, 1600, 3200, 8000):
+        for N in (16, 40, 130, 300, 577, 1000, 2000, 4100, 8000):
+            for K in (16, 200, 504, 1000, 2000, 4000, 8000):
+                for gated in (0, 1):
+                    tm, tn, parts = _tile(lib, BF16, gated, M, N, K, 1)
+                    seen.add((tm, tn, parts > 1, bool(gated)))
+    assert seen <= set(ref.TILES) | {(128, 256, True, False), (128, 256, True, True)}
+    assert all(_tile(lib, I8 if M > 8 else BF16, 0, M, 2048, 256, 1) == (16, 16, 1) for M in (1, 8, 16))
+
+
+def test_tile_query_refuses(lib):
+    v = ctypes.byref(ctypes.c_int32())
+    assert lib.lo_gemm_bias_act_tile_query(BF16, 0, 4, 32, 60, 1, v, v, v) < 0 and lib.lo_gemm_bias_act_tile_query(BF16, 0, 4, 32, 64, 1, v, None, v) < 0
+    assert b"gemm_bias_act" in lib.lo_last_error()
+    assert lib.lo_gemm_bias_act_tile_query(BF16, 0, 0, 0, 64, 1, v, v, v) == 0

@@ -85,6 +85,21 @@ def test_full_sizes(kind, M, N, K, gated):
     assert torch.equal(out, _call(*ops, gated, **k))  # one order of the sum
 
 
+@pytest.mark.parametrize("tile,size", ref.TILE_SIZES, ids=str)
+def test_ragged_sizes_of_every_tile(tile, size):
+    """Each tile, whole and in parts, plain and gated, every operand type, every way out of its epilogue."""
+    M, N, K = size
+    gated = tile[3]
+    for kind, out, k in ((torch.bfloat16, None, K), (torch.float16, torch.float32, K), (torch.int8, torch.float16, 2 * K), (torch.int8, torch.float32, 2 * K)):
+        print("[case] dense", tile, kind, M, N, k, flush=True)
+        g, ops = _case(kind, M, 2 * N if gated else N, k, 2)
+        dtype = _out(kind, out)
+        more = dict(bias=_normal(g, 2 * N if gated else N).to(dtype), activation="silu" if gated else None)
+        if not gated:
+            more.update(residual=_normal(g, M, N).to(dtype), scale=0.75)
+        ref.check(_call(*ops, gated, out_dtype=out, **more), ref.dense(*ops, gated=gated, **more))
+
+
 def test_int8_sums_are_exact():
     """All products of one sign and largest: K * 2^14, just under 2^31."""
     for M in (1, 20, 200):

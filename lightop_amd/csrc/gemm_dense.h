@@ -70,7 +70,9 @@ __device__ __forceinline__ float dense_result(const DenseArgs &a, float v, int64
 // A workgroup takes 16 / C rows of B (gated: half of them of either projection) and all tokens, at most 16 / C; its waves share K and add
 // their sums up through LDS, in the same order every time.  With C > 1 the 16 rows of a matrix instruction's operands are C K blocks of the
 // workgroup's rows, and of the tokens; of its 16 x 16 sums those on the diagonal of C x C squares count, and are added up with the waves'.
-// Weights are read once, straight into registers, U instructions of a wave in flight.
+// Weights are read once, straight into registers, U K blocks of a wave in flight (twice as many, asked for before the last ones are multiplied: 10 to 20 % slower, but
+// for the shortest K).  HBM bounds it where there are rows enough (one token, gated 2048 x 7168 bf16: 59 MB in 14.2 us; int8 29 MB in 9.0; 16384 x 7168 bf16
+// 4.45 TB/s), else the launch and one round trip (256 x 7168 bf16 5.0 us, 128 x 2048 3.4).
 template <int DT>
 __global__ __launch_bounds__(512) void gemm_dense_few_kernel(const DenseArgs a, int lg) {
   typedef Operand<DT> Op;
@@ -128,8 +130,15 @@ __global__ __launch_bounds__(512) void gemm_dense_few_kernel(const DenseArgs a, 
 }
 
 // ---- tiles -----------------------------------------------------------------------------------------------------------------
-// Both operands go to LDS by direct loads, S K blocks to a stage of a ring; 16-byte pieces of a row are swizzled by the row.  A gated
-// product's fragments of 16 rows hold eight of either projection.
+// Both operands go to LDS by direct loads, a K block to a stage of a ring; 16-byte pieces of a row are swizzled by the row.  A gated
+// product's fragments of 16 rows hold eight of either projection, so that the epilogue finds both values of a column in one wave.
+//
+// What bounds them: the largest sizes the matrix cores and the clock under their load (8192 x 4096 x 7168 bf16 with bias and residual 348 us, 1.38 PFLOP/s; the
+// library's plain product 365; int8 4096 x 4096 x 7168 87 us, 2.76 POP/s, library 105); all others the copies, which bring a CU 65 to 70 bytes a ns
+// whatever the ring's depth (the products or the LDS reads taken away, a K block of 128 x 128 takes 0.45 to 0.50 us in place of 0.53), since operands come into
+// each XCD's L2 once and several CUs wait for the same lines: copies of lines that are there run at 130.  Larger tiles copy less and fill
+// fewer CUs; K in another order for each tile gained nothing.  32 x 32 instructions (400 / 364 us for the largest size), waves of 128 x 128 (438) and a third
+// place for the tokens' part (379) were slower.
 constexpr int dense_staging(int tn, int wm, int wn, int rows) { return wm * wn * rows * (tn / wn * 4 + 16); } // bytes
 // Token fragments of a wave that the epilogue turns around at a time: all of them, or half where they do not fit into the ring.
 constexpr int dense_round(int tm, int tn, int wm, int wn, int ring) {
@@ -335,37 +344,32 @@ __device__ __forceinline__ void dense_finish(const DenseArgs &a, const DenseTile
   }
 }
 
-// A wave holds its fragments of a whole stage in registers, and the next stage's are read while they are multiplied: the workgroup meets once a
-// stage, when the next one has landed and everybody's reads of this one are done, so that the ring is refilled from there on and an LDS
-// round trip lies under a stage's products.
-template <int DT, int TM, int TN, int WM, int WN, int S, int ST, bool PART>
+// A wave holds its fragments of a whole K block in registers, and the next one's are read while they are multiplied: the workgroup meets once a
+// K block, when the next one has landed and everybody's reads of this one are done, so that the ring is refilled from there on and an LDS
+// round trip lies under a K block's products.
+template <int DT, int TM, int TN, int WM, int WN, int ST, bool PART>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_dense_ring_kernel(const DenseArgs a, int group_m) {
   typedef Operand<DT> Op;
   constexpr int FM = TM / WM / 16, FN = TN / WN / 16; // fragments of a wave: tokens, weights
-  constexpr int kBlock = (TM + TN) * kBlockK, kStage = S * kBlock;
+  constexpr int kStage = (TM + TN) * kBlockK;
   DenseTileOf<TM, TN, WM, WN, PART> t;
-  constexpr int kPer = t.kA + t.kB, kCopies = S * kPer; // of a K block, of a stage
+  constexpr int kCopies = t.kA + t.kB; // of a stage
   static_assert(ST >= 2, "ring");
   extern __shared__ __attribute__((aligned(16))) int8_t smem[];
   if (!t.start(a, group_m)) return;
-  auto copy = [&](int i, int st, int stage) __attribute__((always_inline)) {
-    int8_t *const to = smem + stage * kStage + i / kPer * kBlock;
-    t.copy(i % kPer, st * S + i / kPer, to, to + TM * kBlockK);
-  };
+  auto copy = [&](int c, int kb, int stage) __attribute__((always_inline)) { t.copy(c, kb, smem + stage * kStage, smem + stage * kStage + TM * kBlockK); };
   const int8_t *const sa = smem + t.wm * (TM / WM) * kBlockK, *const sb = smem + (TM + t.wn * (TN / WN)) * kBlockK;
   struct Fragments {
-    v4i x[S][2][FM], w[S][2][FN];
+    v4i x[2][FM], w[2][FN]; // [half of the K block]
   };
   auto read = [&](Fragments &f, int stage) __attribute__((always_inline)) {
 #pragma unroll
-    for (int s = 0; s < S; ++s)
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int m = 0; m < FM; ++m) f.x[h][m] = *reinterpret_cast<const v4i *>(sa + stage * kStage + m * 2048 + t.lds[h]);
 #pragma unroll
-        for (int m = 0; m < FM; ++m) f.x[s][h][m] = *reinterpret_cast<const v4i *>(sa + stage * kStage + s * kBlock + m * 2048 + t.lds[h]);
-#pragma unroll
-        for (int n = 0; n < FN; ++n) f.w[s][h][n] = *reinterpret_cast<const v4i *>(sb + stage * kStage + s * kBlock + n * 2048 + t.lds[h]);
-      }
+      for (int n = 0; n < FN; ++n) f.w[h][n] = *reinterpret_cast<const v4i *>(sb + stage * kStage + n * 2048 + t.lds[h]);
+    }
   };
   typename Op::Acc acc[FM][FN];
 #pragma unroll
@@ -379,23 +383,20 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_dense_ring_kernel(const Den
   Fragments f[2];
   wait_barrier<(ST - 1) * kCopies>();
   read(f[0], 0);
-  const int stages = (t.KB + S - 1) / S;
   int stage = 0;
-  auto step = [&](Fragments &now, Fragments &then, int st) __attribute__((always_inline)) {
+  auto step = [&](const Fragments &now, Fragments &then, int kb) __attribute__((always_inline)) {
     const int next = stage == ST - 1 ? 0 : stage + 1;
     wait_barrier<(ST - 2) * kCopies>();
     read(then, next);
 #pragma unroll
-    for (int c = 0; c < kCopies; ++c) copy(c, st + ST, stage);
+    for (int c = 0; c < kCopies; ++c) copy(c, kb + ST, stage);
 #pragma unroll
-    for (int s = 0; s < S; ++s)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int m = 0; m < FM; ++m)
 #pragma unroll
-        for (int m = 0; m < FM; ++m)
-#pragma unroll
-          for (int n = 0; n < FN; ++n) acc[m][n] = Op::mfma(now.w[s][h][n], now.x[s][h][m], acc[m][n]);
-    constexpr int kProducts = S * 2 * FM * FN, kReads = S * 2 * (FM + FN);
+        for (int n = 0; n < FN; ++n) acc[m][n] = Op::mfma(now.w[h][n], now.x[h][m], acc[m][n]);
+    constexpr int kProducts = 2 * FM * FN, kReads = 2 * (FM + FN);
 #pragma unroll
     for (int i = 0; i < kProducts; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -406,9 +407,9 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_dense_ring_kernel(const Den
     __builtin_amdgcn_sched_barrier(0);
     stage = next;
   };
-  for (int st = 0; st < stages; st += 2) {
-    step(f[0], f[1], st);
-    if (st + 1 < stages) step(f[1], f[0], st + 1);
+  for (int kb = 0; kb < t.KB; kb += 2) {
+    step(f[0], f[1], kb);
+    if (kb + 1 < t.KB) step(f[1], f[0], kb + 1);
   }
   wait_barrier<0>(); // no copy lands in what the epilogue uses, or outlives the workgroup
   dense_finish<DT, TM, TN, WM, WN, PART, ST * kStage>(a, t, acc, smem);
@@ -553,15 +554,15 @@ template <int DT, int TM, int TN, int WM, int WN> static int launch_dense_step(D
   const int rc = set_dense_tiles(a, TM, TN);
   return rc ? rc : launch_dense_kernel(a, gemm_dense_step_kernel<DT, TM, TN, WM, WN>, lds, WM * WN * 64, &done, stream);
 }
-template <int DT, int TM, int TN, int WM, int WN, int S, int ST> static int launch_dense_ring(DenseArgs a, int parts, hipStream_t stream) {
-  constexpr int ring = ST * S * (TM + TN) * kBlockK, lds = dense_lds(TM, TN, WM, WN, ring, false);
+template <int DT, int TM, int TN, int WM, int WN, int ST> static int launch_dense_ring(DenseArgs a, int parts, hipStream_t stream) {
+  constexpr int ring = ST * (TM + TN) * kBlockK, lds = dense_lds(TM, TN, WM, WN, ring, false);
   static_assert(lds <= 160 * 1024, "LDS");
   static unsigned long long done[2] = {0, 0};
   int rc = set_dense_tiles(a, TM, TN);
   if (rc) return rc;
-  if (parts <= 1) return launch_dense_kernel(a, gemm_dense_ring_kernel<DT, TM, TN, WM, WN, S, ST, false>, lds, WM * WN * 64, &done[0], stream);
+  if (parts <= 1) return launch_dense_kernel(a, gemm_dense_ring_kernel<DT, TM, TN, WM, WN, ST, false>, lds, WM * WN * 64, &done[0], stream);
   a.splits = parts;
-  rc = launch_dense_kernel(a, gemm_dense_ring_kernel<DT, TM, TN, WM, WN, S, ST, true>, ring, WM * WN * 64, &done[1], stream);
+  rc = launch_dense_kernel(a, gemm_dense_ring_kernel<DT, TM, TN, WM, WN, ST, true>, ring, WM * WN * 64, &done[1], stream);
   if (rc) return rc;
   const int64_t blocks = (a.M * ((a.gated ? a.pitch / 2 : a.pitch) / 4) + 255) / 256;
   hipLaunchKernelGGL((gemm_dense_join_kernel<DT>), dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, a);
@@ -586,14 +587,14 @@ template <> int launch_dense<LO_I8>(const DenseArgs &a, int tile, int parts, hip
     switch (tile) {                                                                               \
     case kD256: return launch_dense_step<DT, 256, 256, 2, 4>(a, stream);                          \
     case kD192: return launch_dense_step<DT, 192, 256, 2, 4>(a, stream);                          \
-    case kD128x256: return launch_dense_ring<DT, 128, 256, 2, 4, 1, 3>(a, parts, stream);         \
-    case kD128x192: return launch_dense_ring<DT, 128, 192, 2, 4, 1, 3>(a, parts, stream);         \
-    case kD128: return launch_dense_ring<DT, 128, 128, 2, 4, 1, 4>(a, parts, stream);             \
-    case kD96: return launch_dense_ring<DT, 96, 96, 2, 2, 1, 3>(a, parts, stream);                \
-    case kD64x128: return launch_dense_ring<DT, 64, 128, 2, 4, 1, 4>(a, parts, stream);           \
-    case kD64: return launch_dense_ring<DT, 64, 64, 2, 2, 1, 4>(a, parts, stream);                \
-    case kD64x32: return launch_dense_ring<DT, 64, 32, 2, 2, 1, 6>(a, parts, stream);             \
-    case kD32: return launch_dense_ring<DT, 32, 32, 1, 2, 2, 4>(a, parts, stream);                \
+    case kD128x256: return launch_dense_ring<DT, 128, 256, 2, 4, 3>(a, parts, stream);            \
+    case kD128x192: return launch_dense_ring<DT, 128, 192, 2, 4, 3>(a, parts, stream);            \
+    case kD128: return launch_dense_ring<DT, 128, 128, 2, 4, 4>(a, parts, stream);                \
+    case kD96: return launch_dense_ring<DT, 96, 96, 2, 2, 3>(a, parts, stream);                   \
+    case kD64x128: return launch_dense_ring<DT, 64, 128, 2, 4, 4>(a, parts, stream);              \
+    case kD64: return launch_dense_ring<DT, 64, 64, 2, 2, 4>(a, parts, stream);                   \
+    case kD64x32: return launch_dense_ring<DT, 64, 32, 2, 2, 6>(a, parts, stream);                \
+    case kD32: return launch_dense_ring<DT, 32, 32, 1, 2, 8>(a, parts, stream);                   \
     default: return launch_dense_few<DT>(a, parts & 7, parts >> 3, stream);                       \
     }                                                                                             \
   }

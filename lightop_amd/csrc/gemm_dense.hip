@@ -7,7 +7,10 @@ static int64_t k_blocks(int dtype, int64_t K) { return (K * (dtype == LO_I8 ? 1 
 
 // Which tile, and how many parts of K: the smallest estimate of the time.  A K block takes a CU t1 us with one workgroup of the tile on it and
 // tn_us with as many as it holds (LDS); a workgroup starts and ends in `start` us; the parts are joined by a launch of kJoinUs that moves
-// them twice at kJoinBytes a us.
+// them twice at kJoinBytes a us.  The figures are fitted to bf16 and int8 products of 163 sizes (17 to 8192 tokens, N 64 to 7168, K 128 to 14336 bytes, plain
+// and gated), each timed with every tile and 1 to 8 parts: the choice is 0.5 % off the fastest on average, 16 % at the most (127 x 128 x 7168, gated: eight parts
+// where four are faster).  us, by another tile / by the choice: 2003 x 1536 x 4096 int8, gated 37.2 (128 x 256) / 32.4 (128 x 192), 1531 x 768 x 2048 bf16, gated 23.4
+// (128 x 128) / 20.6 (96 x 96), 700 x 2048 x 2048 bf16 22.0 (128 x 128) / 17.2 (64 x 128), 24 x 7168 x 2048 int8 9.8 (64 x 64) / 7.3 (32 x 32).
 struct DenseTile {
   int tm, tn, held;
   float t1, tn_us, start;
@@ -24,16 +27,23 @@ struct DensePlan {
 };
 // Values of a row of the parts.
 static int64_t part_pitch(int64_t N, bool gated) { return (N + 3) / 4 * 4 * (gated ? 2 : 1); }
-// Whether gemm_dense_few_kernel takes a call.  us, it / the best tile: bf16, 8 tokens 4096 x 7168 16.1 / 16.1, 576 x 7168 10.2 / 9.8, 12: 17.3 / 16.0,
-// 16.1 / 9.9; int8, 12 tokens 4096 x 7168 10.4 / 12.4, 16: 11.2 / 12.3, gated 2048 x 7168 12.0 / 12.6, 576 x 7168 10.2 / 8.5.
-static bool few_tokens(int dtype, int64_t M, int64_t rows) { return M <= 8 || (dtype == LO_I8 && M <= 16 && rows >= 1024); }
+// Whether gemm_dense_few_kernel takes a call.  us, it / the best tile: bf16, 8 tokens 4096 x 7168 16.1 / 16.1, 7168 x 2048 10.8 / 9.1, 12 tokens 4096 x
+// 7168 17.3 / 16.2, 576 x 7168 16.1 / 9.5; int8, 12 tokens 4096 x 7168 10.3 / 12.0, 16: 11.2 / 12.2, gated 2048 x 7168 12.1 / 12.6, but 7168 x 7168 17.8 / 13.3,
+// 576 x 7168 10.2 / 8.6.
+static bool few_tokens(int dtype, int64_t M, int64_t rows) {
+  return M <= 4 || (M <= 8 && rows <= 4096) || (dtype == LO_I8 && M <= 16 && rows >= 1024 && rows <= 4096);
+}
 static DensePlan plan_dense(int dtype, int64_t M, int64_t N, int64_t K, bool gated, bool may_split) {
   const int64_t KB = k_blocks(dtype, K);
   if (few_tokens(dtype, M, gated ? 2 * N : N)) {
+    // Many small workgroups fill the card best: C as large as the tokens' copies of K leave worth it, unless too few steps are left to a wave (us,
+    // C = 8 / 4 / 2 / 1: bf16, 1 token gated 2048 x 7168 14.2 / 14.8 / 15.2 / 15.3, 7168 x 2048 10.2 / 8.8 / 9.2 / 9.7; 4 tokens 2048 x 7168 gated C = 4 17.4, 2 16.6, 1
+    // 16.1), larger where the rows alone are no 256 workgroups (1 token 256 x 7168 C = 16 5.0, 1 13.6).  Waves until a CU has eight, each
+    // with a step and a half at the least.
     const int most = gated ? 3 : 4;
     const int64_t rows = gated ? 2 * N : N;
     int lg = 0, waves = 1;
-    while (lg < 3 && M <= 4 >> lg) ++lg;
+    while (lg < 3 && M <= 4 >> lg && (KB >> (lg + 1)) >= 6) ++lg;
     while (lg < most && M <= 8 >> lg && (rows << lg) < 16 * 256) ++lg;
     const int64_t workgroups = ((rows << lg) + 15) / 16, steps = (KB + (1 << lg) - 1) >> lg;
     while (waves < 8 && workgroups * waves <= 1024 && steps >= 3 * waves) waves *= 2;

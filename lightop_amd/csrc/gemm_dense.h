@@ -72,7 +72,7 @@ __device__ __forceinline__ float dense_result(const DenseArgs &a, float v, int64
 // workgroup's rows, and of the tokens; of its 16 x 16 sums those on the diagonal of C x C squares count, and are added up with the waves'.
 // Weights are read once, straight into registers, U K blocks of a wave in flight (twice as many, asked for before the last ones are multiplied: 10 to 20 % slower, but
 // for the shortest K).  HBM bounds it where there are rows enough (one token, gated 2048 x 7168 bf16: 59 MB in 14.2 us; int8 29 MB in 9.0; 16384 x 7168 bf16
-// 4.45 TB/s), else the launch and one round trip (256 x 7168 bf16 5.0 us, 128 x 2048 3.4).
+// 4.9 TB/s), else the launch and one round trip (256 x 7168 bf16 5.0 us, 128 x 2048 3.4).
 template <int DT>
 __global__ __launch_bounds__(512) void gemm_dense_few_kernel(const DenseArgs a, int lg) {
   typedef Operand<DT> Op;

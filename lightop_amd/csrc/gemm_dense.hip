@@ -36,14 +36,14 @@ static bool few_tokens(int dtype, int64_t M, int64_t rows) {
 static DensePlan plan_dense(int dtype, int64_t M, int64_t N, int64_t K, bool gated, bool may_split) {
   const int64_t KB = k_blocks(dtype, K);
   if (few_tokens(dtype, M, gated ? 2 * N : N)) {
-    // Many small workgroups fill the card best: C as large as the tokens' copies of K leave worth it, unless too few steps are left to a wave (us,
-    // C = 8 / 4 / 2 / 1: bf16, 1 token gated 2048 x 7168 14.2 / 14.8 / 15.2 / 15.3, 7168 x 2048 10.2 / 8.8 / 9.2 / 9.7; 4 tokens 2048 x 7168 gated C = 4 17.4, 2 16.6, 1
-    // 16.1), larger where the rows alone are no 256 workgroups (1 token 256 x 7168 C = 16 5.0, 1 13.6).  Waves until a CU has eight, each
-    // with a step and a half at the least.
+    // About 2048 small workgroups fill the card best: C as large as the tokens' copies of K leave worth it, unless too few steps are left to a wave (us,
+    // C = 8 / 4 / 2 / 1: bf16, 1 token gated 2048 x 7168 14.2 / 14.8 / 15.2 / 15.3, 7168 x 2048 10.2 / 8.8 / 9.2 / 9.7, 16384 x 7168 52.8 / 48.9 / 47.8 / 48.3; 4 tokens gated 2048 x
+    // 7168 C = 4 17.4, 2 16.6, 1 16.1), larger where the rows alone are no 256 workgroups (1 token 256 x 7168 C = 16 5.0, 1 13.6).  Waves until a CU
+    // has eight, each with a step and a half at the least.
     const int most = gated ? 3 : 4;
     const int64_t rows = gated ? 2 * N : N;
     int lg = 0, waves = 1;
-    while (lg < 3 && M <= 4 >> lg && (KB >> (lg + 1)) >= 6) ++lg;
+    while (lg < 3 && M <= 4 >> lg && (KB >> (lg + 1)) >= 6 && (rows << lg) <= 16 * 1024) ++lg;
     while (lg < most && M <= 8 >> lg && (rows << lg) < 16 * 256) ++lg;
     const int64_t workgroups = ((rows << lg) + 15) / 16, steps = (KB + (1 << lg) - 1) >> lg;
     while (waves < 8 && workgroups * waves <= 1024 && steps >= 3 * waves) waves *= 2;

@@ -6,20 +6,21 @@ namespace lo {
 static int64_t k_blocks(int dtype, int64_t K) { return (K * (dtype == LO_I8 ? 1 : 2) + kBlockK - 1) / kBlockK; }
 
 // Which tile, and how many parts of K: the smallest estimate of the time.  A K block takes a CU t1 us with one workgroup of the tile on it and
-// tn_us with as many as it holds (LDS); a workgroup starts and ends in `start` us; the parts are joined by a launch of kJoinUs that moves
-// them twice at kJoinBytes a us.  The figures are fitted to bf16 and int8 products of 163 sizes (17 to 8192 tokens, N 64 to 7168, K 128 to 14336 bytes, plain
-// and gated), each timed with every tile and 1 to 8 parts: the choice is 0.5 % off the fastest on average, 16 % at the most (127 x 128 x 7168, gated: eight parts
-// where four are faster).  us, by another tile / by the choice: 2003 x 1536 x 4096 int8, gated 37.2 (128 x 256) / 32.4 (128 x 192), 1531 x 768 x 2048 bf16, gated 23.4
-// (128 x 128) / 20.6 (96 x 96), 700 x 2048 x 2048 bf16 22.0 (128 x 128) / 17.2 (64 x 128), 24 x 7168 x 2048 int8 9.8 (64 x 64) / 7.3 (32 x 32).
+// tn_us with as many as it holds (LDS); workgroups start and end in `start` us, those of each further round in `again`; the parts are joined by a launch
+// of kJoinUs, and kPartUs for each, that moves them twice at kJoinBytes a us.  The figures are fitted to bf16 and int8 products of 968 sizes (5 to 16384
+// tokens, N 20 to 160000, K 128 to 16384 bytes, plain and gated), each timed with every tile and 1 to 8 parts: the choice is 0.5 % off the fastest on average, 27 % at
+// the most (52 x 2652 x 6656 bf16, gated; three sizes are over 20 %); fits without 200 of the sizes are 0.8 to 1.2 % off for these.  us, by another tile / by the
+// choice: 2003 x 1536 x 4096 int8, gated 37.2 (128 x 256) / 32.4 (128 x 192), 1531 x 768 x 2048 bf16, gated 23.4 (128 x 128) / 20.6 (96 x 96), 700 x 2048 x 2048 bf16 22.0
+// (128 x 128) / 17.2 (64 x 128), 24 x 7168 x 2048 int8 9.8 (64 x 64) / 7.3 (32 x 32).
 struct DenseTile {
   int tm, tn, held;
-  float t1, tn_us, start;
+  float t1, tn_us, start, again;
 };
-constexpr DenseTile kDenseTile[kDenseTiles] = {{256, 256, 1, 1.24f, 1.24f, 17.8f}, {192, 256, 1, 0.95f, 0.95f, 14.8f}, {128, 256, 1, 0.80f, 0.80f, 8.8f},
-                                               {128, 192, 1, 0.60f, 0.60f, 7.8f},  {128, 128, 1, 0.49f, 0.49f, 6.4f},  {96, 96, 2, 0.41f, 0.68f, 5.4f},
-                                               {64, 128, 1, 0.37f, 0.37f, 4.7f},   {64, 64, 2, 0.25f, 0.47f, 4.2f},    {64, 32, 2, 0.19f, 0.33f, 3.9f},
-                                               {32, 32, 2, 0.11f, 0.25f, 3.7f}};
-constexpr float kJoinUs = 3.2f, kJoinBytes = 5.0e6f;
+constexpr DenseTile kDenseTile[kDenseTiles] = {{256, 256, 1, 1.532f, 1.532f, 3.14f, 10.00f}, {192, 256, 1, 1.254f, 1.254f, 3.69f, 7.57f}, {128, 256, 1, 1.012f, 1.012f, 2.70f, 4.97f},
+                                               {128, 192, 1, 0.743f, 0.743f, 3.26f, 7.65f}, {128, 128, 1, 0.587f, 0.587f, 2.21f, 2.84f}, {96, 96, 2, 0.574f, 0.912f, 1.29f, 0.47f},
+                                               {64, 128, 1, 0.540f, 0.540f, 0.83f, 0.38f}, {64, 64, 2, 0.370f, 0.648f, 0.69f, 0.12f}, {64, 32, 2, 0.277f, 0.496f, 0.01f, 0.32f},
+                                               {32, 32, 2, 0.179f, 0.347f, 0.55f, 2.20f}};
+constexpr float kJoinUs = 3.02f, kPartUs = 0.48f, kJoinBytes = 2.48e6f;
 constexpr int kMostParts = 8, kLeastBlocks = 4; // of K, in a part
 struct DensePlan {
   int tile, parts; // of K
@@ -39,14 +40,15 @@ static DensePlan plan_dense(int dtype, int64_t M, int64_t N, int64_t K, bool gat
     // About 2048 small workgroups fill the card best: C as large as the tokens' copies of K leave worth it, unless too few steps are left to a wave (us,
     // C = 8 / 4 / 2 / 1: bf16, 1 token gated 2048 x 7168 14.2 / 14.8 / 15.2 / 15.3, 7168 x 2048 10.2 / 8.8 / 9.2 / 9.7, 16384 x 7168 52.8 / 48.9 / 47.8 / 48.3; 4 tokens gated 2048 x
     // 7168 C = 4 17.4, 2 16.6, 1 16.1), larger where the rows alone are no 256 workgroups (1 token 256 x 7168 C = 16 5.0, 1 13.6).  Waves until a CU
-    // has eight, each with a step and a half at the least.
+    // has eight, four where there are more workgroups than it holds at a time (1 token 151936 x 2048 C = 2, four waves 113, C = 1, one 139), each with a step
+    // and a half at the least.
     const int most = gated ? 3 : 4;
     const int64_t rows = gated ? 2 * N : N;
     int lg = 0, waves = 1;
-    while (lg < 3 && M <= 4 >> lg && (KB >> (lg + 1)) >= 6 && (rows << lg) <= 16 * 1024) ++lg;
+    while (lg < 3 && M <= 4 >> lg && (KB >> (lg + 1)) >= 6 && (lg == 0 || (rows << lg) <= 16 * 1024)) ++lg;
     while (lg < most && M <= 8 >> lg && (rows << lg) < 16 * 256) ++lg;
     const int64_t workgroups = ((rows << lg) + 15) / 16, steps = (KB + (1 << lg) - 1) >> lg;
-    while (waves < 8 && workgroups * waves <= 1024 && steps >= 3 * waves) waves *= 2;
+    while (waves < 8 && (workgroups * waves <= 1024 || (workgroups > 2048 && waves < 4)) && steps >= 3 * waves) waves *= 2;
     return {kDenseFew, 1, lg + 8 * waves};
   }
   DensePlan best{kDenseFew, 1, 0};
@@ -60,9 +62,9 @@ static DensePlan plan_dense(int dtype, int64_t M, int64_t N, int64_t K, bool gat
       const int64_t each = (tiles * parts + 255) / 256; // workgroups of a CU
       const float blocks = static_cast<float>((KB + parts - 1) / parts);
       const int64_t rounds = each / t.held, rest = each % t.held;
-      float us = static_cast<float>(rounds) * (t.start + blocks * t.tn_us);
-      if (rest) us += t.start + blocks * (t.t1 + (t.held > 1 ? (t.tn_us - t.t1) * static_cast<float>(rest - 1) / static_cast<float>(t.held - 1) : 0.0f));
-      if (parts > 1) us += kJoinUs + 2.0f * static_cast<float>(bytes) / kJoinBytes;
+      float us = static_cast<float>(rounds) * blocks * t.tn_us + t.start + t.again * static_cast<float>(rounds + (rest > 0) - 1);
+      if (rest) us += blocks * (t.t1 + (t.held > 1 ? (t.tn_us - t.t1) * static_cast<float>(rest - 1) / static_cast<float>(t.held - 1) : 0.0f));
+      if (parts > 1) us += kJoinUs + kPartUs * static_cast<float>(parts) + 2.0f * static_cast<float>(bytes) / kJoinBytes;
       if (best.tile < 0 || us < least) best = {i, parts, 0}, least = us;
     }
   }

@@ -72,39 +72,40 @@ def check(out, want):
 # Sizes M, N, K (16-bit operands; int8 ones of twice the K take the same) by the tile they take with a workspace: (tokens, weight rows, whether K is in parts, gated).
 # Rows and columns end inside a tile, K inside a K block; the first N is a multiple of eight, the second odd.
 TILES = {
-    (32, 32, False, False): [(12, 16, 208), (9, 21, 224)],
-    (32, 32, False, True): [(9, 24, 232), (11, 17, 224)],
-    (32, 32, True, False): [(9, 16, 2216), (9, 17, 2256)],
-    (32, 32, True, True): [(9, 24, 2456), (9, 17, 2336)],
-    (64, 32, False, False): [(1652, 136, 232), (34, 4497, 264)],
-    (64, 32, False, True): [(45, 2248, 208), (33, 2147, 224)],
-    (64, 32, True, False): [(2084, 16, 5216), (1083, 33, 4912)],
-    (64, 32, True, True): [(1046, 40, 4568), (1059, 17, 5200)],
-    (64, 64, False, False): [(69, 5704, 200), (35, 8633, 264)],
-    (64, 64, False, True): [(18, 8584, 248), (19, 8377, 224)],
-    (64, 64, True, False): [(34, 1512, 3984), (1361, 33, 3680)],
-    (64, 64, True, True): [(35, 696, 4208), (34, 677, 3472)],
-    (64, 128, False, False): [(268, 3760, 264), (77, 8677, 280)],
-    (64, 128, False, True): [(21, 8560, 432), (19, 8193, 296)],
-    (64, 128, True, False): [(17, 8248, 2480), (17, 8363, 2664)],
-    (64, 128, True, True): [(17, 4184, 2824), (18, 4383, 2600)],
-    (96, 96, False, False): [(1491, 1456, 200), (399, 5099, 200)],
+    (32, 32, False, False): [(11, 16, 408), (10, 17, 360)],
+    (32, 32, False, True): [(10, 24, 328), (10, 19, 352)],
+    (32, 32, True, False): [(9, 16, 2488), (9, 17, 2504)],
+    (32, 32, True, True): [(9, 24, 2456), (9, 17, 2416)],
+    (64, 32, False, False): [(12, 16, 208), (9, 21, 224)],
+    (64, 32, False, True): [(9, 24, 232), (11, 17, 224)],
+    (64, 32, True, False): [(1356, 40, 3040), (1381, 33, 3104)],
+    (64, 32, True, True): [(35, 696, 3064), (1370, 17, 3040)],
+    (64, 64, False, False): [(47, 8520, 328), (33, 8695, 328)],
+    (64, 64, False, True): [(67, 3280, 360), (39, 4285, 376)],
+    (64, 64, True, False): [(33, 4256, 2776), (33, 4207, 2784)],
+    (64, 64, True, True): [(34, 2120, 2832), (35, 2119, 2776)],
+    (64, 128, False, False): [(153, 6328, 216), (149, 6139, 200)],
+    (64, 128, False, True): [(12, 8568, 288), (9, 8545, 224)],
+    (64, 128, True, False): [(9, 8416, 2792), (9, 8307, 2376)],
+    (64, 128, True, True): [(9, 2088, 5280), (9, 4243, 2336)],
+    (96, 96, False, False): [(1491, 1456, 200), (602, 3363, 208)],
     (96, 96, False, True): [(68, 8336, 208), (93, 8371, 216)],
-    (96, 96, True, False): [(68, 3216, 4216), (68, 2769, 3344)],
-    (96, 96, True, True): [(71, 1520, 3624), (65, 1401, 3352)],
-    (128, 128, False, False): [(473, 5080, 336), (208, 8581, 368)],
-    (128, 128, False, True): [(130, 7608, 360), (102, 8621, 368)],
-    (128, 128, True, False): [(65, 8392, 3336), (69, 8297, 2872)],
-    (128, 128, True, True): [(67, 4272, 3480), (66, 4329, 3112)],
+    (96, 96, True, False): [(68, 3216, 4216), (65, 2757, 4704)],
+    (96, 96, True, True): [(77, 1376, 4408), (65, 1491, 4184)],
+    (128, 128, False, False): [(223, 8256, 248), (399, 5099, 200)],
+    (128, 128, False, True): [(203, 4144, 232), (199, 4685, 208)],
+    (128, 128, True, False): [(67, 4424, 4920), (66, 8217, 2408)],
+    (128, 128, True, True): [(65, 3168, 4336), (65, 4327, 2096)],
     (128, 192, False, False): [(542, 8376, 208), (1155, 3917, 200)],
     (128, 192, False, True): [(220, 8936, 200), (484, 4247, 216)],
-    (128, 192, True, False): [(397, 2768, 4656), (291, 3591, 4040)],
-    (128, 192, True, True): [(98, 5624, 4072), (100, 5555, 4024)],
+    (128, 192, True, False): [(141, 5992, 5512), (133, 5549, 4856)],
+    (128, 192, True, True): [(10, 5488, 4144), (9, 5917, 3728)],
     (128, 256, False, False): [(819, 7056, 208), (702, 8209, 208)],
     (128, 256, False, True): [(676, 4184, 208), (521, 4919, 200)],
-    (192, 256, False, False): [(1029, 8984, 280), (1088, 8509, 200)],
-    (192, 256, False, True): [(1184, 3984, 200), (1860, 2489, 200)],
+    (128, 256, True, True): [(9, 8200, 4176), (10, 8275, 4056)],
+    (192, 256, False, False): [(1045, 7456, 208), (946, 8195, 200)],
+    (192, 256, False, True): [(1184, 3984, 200), (391, 8271, 208)],
     (256, 256, False, False): [(2325, 5104, 216), (1617, 7551, 200)],
-    (256, 256, False, True): [(1439, 4464, 208), (2309, 2603, 200)],
+    (256, 256, False, True): [(1009, 5552, 208), (2309, 2603, 200)],
 }
 TILE_SIZES = [(tile, size) for tile in TILES for size in TILES[tile]]

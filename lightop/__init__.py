@@ -6,7 +6,7 @@ python/lightop/moe/__init__.py:57-78).  This package makes those names resolve t
 ``lightop_amd`` themselves - the same module objects, so the lazily resolved entry points
 (``lightop.moe.fused_experts_impl_int8`` and friends) are the same functions and module state (caches,
 flags) exists once.  Only the operators of the block-INT8 fused-MoE path, its per-channel and W4A8 forms and
-the two routers, and the 8-bit operators beside them, exist; every other name of the reference package raises AttributeError / ImportError.
+the two routers, the 8-bit operators beside them and those of the dense blocks exist; every other name of the reference package raises AttributeError / ImportError.
 
 Importing it touches neither the GPU nor the HIP library.
 """

@@ -16,6 +16,10 @@ Public surface (same names, argument order and defaults as the reference package
     lightop_amd.quant.per_token_group_quant_fp8, lightop_amd.moe.act_and_mul_group_quant_fp8
     lightop_amd.gemmopt.gemm_w8a8_fp8_block, lightop_amd.moe.fused_experts_decode_fp8
                                                  (e4m3 with 128 blocks: shared experts, projections, decode batches)
+    lightop_amd.norm.rms_norm_block              (norms behind and in front of a block, its gate and residual scale; 8-bit rows out)
+    lightop_amd.gemmopt.gemm_bias_act, gemm_act_and_mul, gemm_w8a8_bias_act, gemm_w8a8_act_and_mul
+                                                 (dense products of 16-bit and int8 operands: bias, activation and residual in the
+                                                 epilogue, both projections of a gated block in one)
     lightop_amd.op                               (lightop.op: moe_align_block_size, moe_sum)
     lightop_amd.envs                             (lightop.envs: LMSLIM_* flags, read lazily)
 

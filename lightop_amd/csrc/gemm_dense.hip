@@ -24,36 +24,53 @@ constexpr float kJoinUs = 3.02f, kPartUs = 0.48f, kJoinBytes = 2.48e6f;
 constexpr int kMostParts = 8, kLeastBlocks = 4; // of K, in a part
 struct DensePlan {
   int tile, parts; // of K
-  int few;         // gemm_dense_few_kernel: C, as a power of two, + 8 * waves
+  int few;         // gemm_dense_few_kernel: C, as a power of two, + 8 * waves + 128 * U
 };
 // Values of a row of the parts.
 static int64_t part_pitch(int64_t N, bool gated) { return (N + 3) / 4 * 4 * (gated ? 2 : 1); }
-// Whether gemm_dense_few_kernel takes a call.  us, it / the best tile: bf16, 8 tokens 4096 x 7168 16.1 / 16.1, 7168 x 2048 10.8 / 9.1, 12 tokens 4096 x
-// 7168 17.3 / 16.2, 576 x 7168 16.1 / 9.5; int8, 12 tokens 4096 x 7168 10.3 / 12.0, 16: 11.2 / 12.2, gated 2048 x 7168 12.1 / 12.6, but 7168 x 7168 17.8 / 13.3,
-// 576 x 7168 10.2 / 8.6.
-static bool few_tokens(int dtype, int64_t M, int64_t rows) {
-  return M <= 4 || (M <= 8 && rows <= 4096) || (dtype == LO_I8 && M <= 16 && rows >= 1024 && rows <= 4096);
+// Whether gemm_dense_few_kernel takes a call: up to 16 tokens, where K is short enough for them.  It reads weights as they are needed and is through sooner, the tiles'
+// copies run ahead of the products and stream long rows faster.  us, it / the best tile: bf16, 1 token 2048 x 7168 9.1 / 11.2, 7168 x 2048 8.6 / 9.0, but 16384 x
+// 7168 45.9 / 41.7 and 65536 x 14336 358 / 307; 8 tokens 4096 x 2048 6.8 / 8.6, but x 7168 16.0 / 15.9, 7168 x 7168 28.5 / 20.1; 16 tokens 2048 x 2048 7.1 / 7.9, but
+// x 7168 17.9 / 12.0; int8, 8 tokens 4096 x 7168 9.5 / 11.7, 16 11.1 / 12.0.
+static bool few_tokens(int64_t M, int64_t rows, int64_t KB) {
+  return M <= 16 && (rows <= 4096 ? M * KB <= (rows <= 2560 ? 600 : 900) : (M + 2) * KB <= 150);
 }
 static DensePlan plan_dense(int dtype, int64_t M, int64_t N, int64_t K, bool gated, bool may_split) {
   const int64_t KB = k_blocks(dtype, K);
-  if (few_tokens(dtype, M, gated ? 2 * N : N)) {
-    // About 2048 small workgroups fill the card best: C as large as the tokens' copies of K leave worth it, unless too few steps are left to a wave (us,
-    // C = 8 / 4 / 2 / 1: bf16, 1 token gated 2048 x 7168 14.2 / 14.8 / 15.2 / 15.3, 7168 x 2048 10.2 / 8.8 / 9.2 / 9.7, 16384 x 7168 52.8 / 48.9 / 47.8 / 48.3; 4 tokens gated 2048 x
-    // 7168 C = 4 17.4, 2 16.6, 1 16.1), larger where the rows alone are no 256 workgroups (1 token 256 x 7168 C = 16 5.0, 1 13.6).  Waves until a CU
-    // has eight, four where there are more workgroups than it holds at a time (1 token 151936 x 2048 C = 2, four waves 113, C = 1, one 139), each with a step
-    // and a half at the least.
+  if (few_tokens(M, gated ? 2 * N : N, KB)) {
+    // C: the fewest rounds of 256 workgroups, a larger C where that takes a twenty-fifth off (tokens are read C times), and four steps at the least.
+    // Waves, and K blocks in flight of each (U): below 512 workgroups all steps at once on as many waves as that takes, from 36 steps on eight waves, one each; between,
+    // as many as fit on the card at a time and share its bandwidth evenly, less than 4096 of both; beyond, all steps at once again.  More waves for the results of
+    // many tokens.  U divides a wave's steps evenly.  Over 2900 sizes (1 to 16 tokens, 100 to 60000 rows, K 512 to 14336) that were timed with every C, waves and U:
+    // 3.1 % over the fastest on average.  us, by this / one K block in flight: bf16, 1 token 256 x 7168 4.3 / 5.0, 7168 x 2048 8.6 / 9.2, gated 2048 x 7168 14.4 / 14.8.
     const int most = gated ? 3 : 4;
     const int64_t rows = gated ? 2 * N : N;
     int lg = 0, waves = 1;
-    while (lg < 3 && M <= 4 >> lg && (KB >> (lg + 1)) >= 6 && (lg == 0 || (rows << lg) <= 16 * 1024)) ++lg;
-    while (lg < most && M <= 8 >> lg && (rows << lg) < 16 * 256) ++lg;
-    const int64_t workgroups = ((rows << lg) + 15) / 16, steps = (KB + (1 << lg) - 1) >> lg;
-    while (waves < 8 && (workgroups * waves <= 1024 || (workgroups > 2048 && waves < 4)) && steps >= 3 * waves) waves *= 2;
-    return {kDenseFew, 1, lg + 8 * waves};
+    float least = 0.0f;
+    for (int i = 0; i <= most && (i == 0 || (M <= 16 >> i && KB >> i >= 4)); ++i) {
+      const int64_t workgroups = ((rows << i) + 15) / 16, rounds = (workgroups + 255) / 256;
+      const float time = static_cast<float>(rounds) / static_cast<float>(workgroups) * (1.0f + 0.04f * static_cast<float>(i));
+      if (i == 0 || time < least) lg = i, least = time;
+    }
+    const int64_t workgroups = ((rows << lg) + 15) / 16, steps = (KB + (1 << lg) - 1) >> lg, results = M * (16 >> lg) / (gated ? 2 : 1);
+    int64_t flight = 8;
+    if (workgroups < 512) {
+      waves = steps < 8 ? 1 : steps < 20 ? 2 : steps < 36 ? 4 : 8;
+      flight = steps < 36 ? 8 : 1;
+      while (waves < 8 && results > 64 * waves && steps >= 2 * waves) waves *= 2;
+    } else if (workgroups >= 2600) {
+      waves = steps < 10 ? 1 : steps < 20 ? 2 : 4;
+    } else if (workgroups >= 1024 || steps >= 10) {
+      waves = workgroups < 1536 ? 2 : 1;
+      flight = workgroups < 1024 || (workgroups >= 1536 && workgroups < 2048) ? 2 : 1;
+    }
+    while (waves > steps) waves /= 2;
+    const int64_t each = (steps + waves - 1) / waves, passes = (each + flight - 1) / flight;
+    return {kDenseFew, 1, lg + 8 * waves + 128 * static_cast<int>((each + passes - 1) / passes)};
   }
   DensePlan best{kDenseFew, 1, 0};
   float least = 0.0f;
-  for (int i = 0; i < kDenseTiles; ++i) {
+  for (int i = M <= 16 ? kD32 : 0; i < kDenseTiles; ++i) { // (up to 16 tokens the smallest: 2.7 % over the fastest tile, 29 % at the most; by the estimate of all 2.9 and 76)
     const DenseTile &t = kDenseTile[i];
     const int64_t width = gated ? t.tn / 2 : t.tn, tiles = ((M + t.tm - 1) / t.tm) * ((N + width - 1) / width);
     for (int parts = 1; parts <= (may_split && i >= kD128x256 ? kMostParts : 1); parts += parts < 4 ? 1 : 2) {

@@ -129,7 +129,7 @@ def test_tile_of_the_sizes_that_the_gpu_tests_take(lib, tile, size):
 
 
 def test_every_tile_has_sizes(lib):
-    """Over many sizes no call takes a tile, whole or in parts, that the list above leaves out, but for 128 x 256 in parts."""
+    """Over many sizes no call takes a tile, whole or in parts, that the list above leaves out, but for 128 x 256 in parts and the kernel of few tokens."""
     seen = set()
     for M in (9, 17, 33, 65, 100, 200, 400, 800, 1600, 3200, 8000):
         for N in (16, 40, 130, 300, 577, 1000, 2000, 4100, 8000):
@@ -137,7 +137,8 @@ def test_every_tile_has_sizes(lib):
                 for gated in (0, 1):
                     tm, tn, parts = _tile(lib, BF16, gated, M, N, K, 1)
                     seen.add((tm, tn, parts > 1, bool(gated)))
-    assert seen <= set(ref.TILES) | {(128, 256, True, False), (128, 256, True, True)}
+    assert seen <= set(ref.TILES) | {(128, 256, True, False), (128, 256, True, True), (16, 16, False, False), (16, 16, False, True)}
+    assert all(_tile(lib, BF16, gated, M, N, K, 1) == (16, 16, 1) for M, N, K, gated in ref.FEW)
     assert all(_tile(lib, I8 if M > 8 else BF16, 0, M, 2048, 256, 1) == (16, 16, 1) for M in (1, 8, 16))
 
 

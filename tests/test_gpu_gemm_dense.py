@@ -100,6 +100,18 @@ def test_ragged_sizes_of_every_tile(tile, size):
         ref.check(_call(*ops, gated, out_dtype=out, **more), ref.dense(*ops, gated=gated, **more))
 
 
+@pytest.mark.parametrize("size", ref.FEW, ids=str)
+def test_every_form_of_few_tokens(size):
+    M, N, K, gated = size
+    print("[case] few", *size, flush=True)
+    for kind, k in ((torch.bfloat16, K), (torch.float16, K), (torch.int8, 2 * K)):
+        g, ops = _case(kind, M, 2 * N if gated else N, k, 3)
+        bias = _normal(g, 2 * N if gated else N)
+        r = None if gated else _normal(g, M, N).to(_out(kind, None))
+        got = _call(*ops, gated, bias=bias, activation="silu" if gated else None, **({} if gated else {"residual": r}))
+        ref.check(got, ref.dense(*ops, bias, "silu" if gated else None, gated, r))
+
+
 def test_int8_sums_are_exact():
     """All products of one sign and largest: K * 2^14, just under 2^31."""
     for M in (1, 20, 200):

@@ -163,11 +163,12 @@ __global__ __launch_bounds__(512) void gemm_dense_few_kernel(const DenseArgs a, 
 // Both operands go to LDS by direct loads, a K block to a stage of a ring; 16-byte pieces of a row are swizzled by the row.  A gated
 // product's fragments of 16 rows hold eight of either projection, so that the epilogue finds both values of a column in one wave.
 //
-// What bounds them: the largest sizes the matrix cores and the clock under their load (8192 x 4096 x 7168 bf16 with bias and residual 348 us, 1.38 PFLOP/s; the
-// library's plain product 365; int8 4096 x 4096 x 7168 87 us, 2.76 POP/s, library 105); all others the copies, which bring a CU 65 to 70 bytes a ns
+// What bounds them: the largest sizes the matrix cores and the clock under their load (8192 x 4096 x 7168 bf16 with bias and residual 348 to 367 us, 1.31 to
+// 1.38 PFLOP/s; the library's plain product 365; int8 4096 x 4096 x 7168 87 to 91 us, 2.7 POP/s, library 105); all others the copies, which bring a CU 65 to 70 bytes a ns
 // whatever the ring's depth (the products or the LDS reads taken away, a K block of 128 x 128 takes 0.45 to 0.50 us in place of 0.53), since operands come into
 // each XCD's L2 once and several CUs wait for the same lines: copies of lines that are there run at 130.  Larger tiles copy less and fill
-// fewer CUs; K in another order for each tile gained nothing.  32 x 32 instructions (400 / 364 us for the largest size), waves of 128 x 128 (438) and a third
+// fewer CUs; K in another order for each tile gained nothing, nor did one sharer's reading ahead into L2 (96 x 96: a K block 0.40 us, with all
+// operands there 0.33, which is the LDS's).  32 x 32 instructions (400 / 364 us for the largest size), waves of 128 x 128 (438) and a third
 // place for the tokens' part (379) were slower.
 constexpr int dense_staging(int tn, int wm, int wn, int rows) { return wm * wn * rows * (tn / wn * 4 + 16); } // bytes
 // Token fragments of a wave that the epilogue turns around at a time: all of them, or half where they do not fit into the ring.

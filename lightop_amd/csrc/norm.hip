@@ -170,7 +170,8 @@ template <int DT> static void launch_norm_form(int form, const NormArgs &a, int6
 // and y's codes; in fp32 between the inputs and the outputs, as above.  A workgroup a row, x and r read once and both asked for in front of
 // the first sum, where the registers hold them (fp32 rows 205 -> 188 us).  HBM bounds it: 8192 x 7168 bf16, norms on both sides with a gate of channels, 470 MB in
 // 91 to 94 us (5.0 to 5.2 TB/s, a copy's rate), without the norm behind 84.5 (5.6); a sigmoid of channels or 8-bit codes add vector work a value (int8 rows 86 us for
-// 411 MB, with both 103); for one row the launch and two sums across the workgroup (2048 values 4.1 us).
+// 411 MB, with both 103); for one row the launch and two sums across the workgroup (2048 values 4.0 us).  Two rows a workgroup, so that the weights and the gate serve both,
+// were slower (100 / 91).
 constexpr int kNoCodes = -1;
 struct NormBlockArgs {
   const void *x, *r, *post, *w, *gate;
@@ -292,9 +293,9 @@ __global__ __launch_bounds__(1024) void rms_norm_block_kernel(const NormBlockArg
 }
 
 template <int DT, int FORM> static void launch_norm_block(NormBlockArgs a, int64_t M, hipStream_t stream) {
-  // us, 256 threads / 512, many rows of 7168 bf16: without codes 96.5 / 93.1 (a gate of channels), 86.8 / 84.3 (of tokens, no norm behind); with int8
-  // rows 85.5 / 87.0, 4096 x 4096 with int8 groups 33.5 / 36.5
-  const NormGrid g(a.H, M, FORM == kNoCodes ? 512 : 256);
+  // us, 256 threads / 512, 8192 rows bf16: without codes 7168 89.8 / 87.7 (a gate of channels 93.9 / 90.3), 5120 64.6 / 65.7, 4096 45.3 / 51.7, 2560 32.6 / 41.8; with
+  // e4m3 codes 7168 85.8 / 87.3, 4096 46.7 / 54.8.  128 / 256: rows of 2048 with int8 codes, 8192 26.6 / 28.8, 4096 14.9 / 17.0, 1000 7.1 / 6.9
+  const NormGrid g(a.H, M, FORM == kNoCodes && a.H > 5120 ? 512 : a.H <= 2048 && M >= 2048 ? 128 : 256);
   for (; a.row0 < M; a.row0 += NormGrid::kRows) {
     const dim3 grid = g.rows(M - a.row0), block(static_cast<unsigned>(g.threads));
     if (g.ch <= 1) hipLaunchKernelGGL((rms_norm_block_kernel<DT, FORM, 1>), grid, block, 0, stream, a);

@@ -102,6 +102,19 @@ def test_sizes(dtype, form, M, H):
             _check_codes(got, form, want[2], want[3])
 
 
+@pytest.mark.parametrize("form", FORMS, ids=str)
+@pytest.mark.parametrize("M,H", [(2047, 2048), (2048, 2048), (2301, 1152), (3001, 128), (2050, 2176), (1100, 5248)])
+def test_many_rows(form, M, H):
+    print("[case] norm block", form, M, H, flush=True)
+    for dtype, gate in ((torch.bfloat16, "channel"), (torch.float32, "token")):
+        args = _make(M, H, dtype, gate, True)
+        want = _exact(*args, True, 0.5, 1.0, 1e-6)
+        got = _call(args, form, True, 0.5, return_normed=True)
+        _check(got, want, dtype)
+        if form is not None:
+            _check_codes(got, form, want[2], want[3])
+
+
 @pytest.mark.parametrize("H", [8, 24, 40, 520, 2056, 16392])
 @pytest.mark.parametrize("form", [None, (torch.int8, None)], ids=str)
 def test_odd_rows(H, form):

@@ -679,7 +679,8 @@ int lo_rms_norm_block(const void *x, int dtype, int64_t x_stride, const void *re
  *   v[m, n] = sum over k of a[m, k] * b[n, k], times a_scale[m] * b_scale[n] with LO_I8, + bias[n]
  *   c[m, n] = scale * act(v[m, n]) + residual[m, n], or, gated, scale * act(v[m, n]) * v[m, N + n] + residual[m, n]
  *   a [M, K], b [N, K] (gated: [2N, K], the gate's rows first) of `dtype` LO_BF16, LO_F16 or LO_I8, rows a_stride / b_stride values
- *   apart; rows and strides multiples of 16 bytes, as K is; strides at most 4 MiB, an int8 K at most 131056
+ *   apart; rows and strides multiples of 16 bytes, as K is; strides at most 4 MiB, an int8 K at most 131056, another one 2097152
+ *   M <= 2^24, N <= 2^23, and c fewer than 2^22 tiles of 256 x 256 (gated: 256 x 128); more is LO_ENOTSUP, from the queries too
  *   a_scale [M], b_scale [N] (gated [2N]) fp32 with LO_I8, else NULL
  *   bias NULL or [N] (gated [2N]) of out_dtype or LO_F32;  activation LO_ACT_NONE, LO_ACT_SILU or LO_ACT_GELU
  *   residual NULL or [M, N] of out_dtype, rows residual_stride values apart; c itself, or apart from it

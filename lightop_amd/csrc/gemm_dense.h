@@ -634,9 +634,14 @@ template <class K> static int launch_dense_kernel(const DenseArgs &a, K kernel, 
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((a.m_tiles * a.n_tiles + 7) / 8 * 8), a.splits), dim3(threads), lds, stream, a, group_m);
   return LO_OK;
 }
+constexpr int64_t kMostTiles = 1 << 22; // (512 threads of each are below a grid's 2^32)
+static int64_t dense_tiles(int64_t M, int64_t N, int tm, int tn, bool gated) {
+  const int64_t width = gated ? tn / 2 : tn;
+  return (M + tm - 1) / tm * ((N + width - 1) / width);
+}
 static int set_dense_tiles(DenseArgs &a, int tm, int tn) {
   const int64_t width = a.gated ? tn / 2 : tn, m_tiles = (a.M + tm - 1) / tm, n_tiles = (a.N + width - 1) / width;
-  LO_REQUIRE(m_tiles * n_tiles < (1 << 22), LO_ENOTSUP, "gemm_bias_act: %lld x %lld outputs", (long long)a.M, (long long)a.N);
+  LO_REQUIRE(m_tiles * n_tiles < kMostTiles, LO_ENOTSUP, "gemm_bias_act: %lld x %lld outputs", (long long)a.M, (long long)a.N);
   a.m_tiles = static_cast<int32_t>(m_tiles);
   a.n_tiles = static_cast<int32_t>(n_tiles);
   return LO_OK;

@@ -72,7 +72,8 @@ static DensePlan plan_dense(int dtype, int64_t M, int64_t N, int64_t K, bool gat
   float least = 0.0f;
   for (int i = M <= 16 ? kD32 : 0; i < kDenseTiles; ++i) { // (up to 16 tokens the smallest: 2.7 % over the fastest tile, 29 % at the most; by the estimate of all 2.9 and 76)
     const DenseTile &t = kDenseTile[i];
-    const int64_t width = gated ? t.tn / 2 : t.tn, tiles = ((M + t.tm - 1) / t.tm) * ((N + width - 1) / width);
+    const int64_t tiles = dense_tiles(M, N, t.tm, t.tn, gated);
+    if (tiles >= kMostTiles) continue; // (never the largest tile: see check_dense_sizes)
     for (int parts = 1; parts <= (may_split && i >= kD128x256 ? kMostParts : 1); parts += parts < 4 ? 1 : 2) {
       const int64_t bytes = parts * M * part_pitch(N, gated) * 4;
       if (parts > 1 && KB / parts < kLeastBlocks) break;
@@ -89,13 +90,15 @@ static DensePlan plan_dense(int dtype, int64_t M, int64_t N, int64_t K, bool gat
 }
 
 constexpr int64_t kMostStride = 4 << 20; // bytes: 256 rows of a tile stay within 2^30
-static int check_dense_sizes(int dtype, int64_t M, int64_t N, int64_t K) {
+static int check_dense_sizes(int dtype, int gated, int64_t M, int64_t N, int64_t K) {
   LO_REQUIRE(dtype == LO_BF16 || dtype == LO_F16 || dtype == LO_I8, LO_ENOTSUP, "gemm_bias_act: operands are bf16, fp16 or int8");
   LO_REQUIRE(M >= 0 && N >= 0, LO_EINVAL, "gemm_bias_act: bad sizes %lld x %lld", (long long)M, (long long)N);
   const int64_t unit = dtype == LO_I8 ? 16 : 8, most = dtype == LO_I8 ? 131056 : kMostStride / 2; // (sums of int8 products stay below 2^31)
   LO_REQUIRE(K > 0 && K % unit == 0, LO_EINVAL, "gemm_bias_act: K (%lld) must be a multiple of %lld", (long long)K, (long long)unit);
   LO_REQUIRE(K <= most, LO_ENOTSUP, "gemm_bias_act: K (%lld) is at most %lld", (long long)K, (long long)most);
   LO_REQUIRE(M <= (1 << 24) && N <= (1 << 23), LO_ENOTSUP, "gemm_bias_act: %lld x %lld outputs (at most 2^24 x 2^23)", (long long)M, (long long)N);
+  LO_REQUIRE(dense_tiles(M, N, kDenseTile[kD256].tm, kDenseTile[kD256].tn, gated != 0) < kMostTiles, LO_ENOTSUP,
+             "gemm_bias_act: %lld x %lld outputs (fewer than 2^22 tiles of 256 x %d)", (long long)M, (long long)N, gated ? 128 : 256);
   return LO_OK;
 }
 
@@ -103,7 +106,7 @@ static int check_dense_sizes(int dtype, int64_t M, int64_t N, int64_t K) {
 
 extern "C" int64_t lo_gemm_bias_act_workspace_bytes(int dtype, int gated, int64_t M, int64_t N, int64_t K) {
   using namespace lo;
-  const int rc = check_dense_sizes(dtype, M, N, K);
+  const int rc = check_dense_sizes(dtype, gated, M, N, K);
   if (rc) return rc;
   if (N == 0) return 0;
   const DensePlan p = plan_dense(dtype, M, N, K, gated != 0, true);
@@ -113,7 +116,7 @@ extern "C" int64_t lo_gemm_bias_act_workspace_bytes(int dtype, int gated, int64_
 extern "C" int lo_gemm_bias_act_tile_query(int dtype, int gated, int64_t M, int64_t N, int64_t K, int has_workspace, int32_t *tile_m,
                                            int32_t *tile_n, int32_t *parts) {
   using namespace lo;
-  const int rc = check_dense_sizes(dtype, M, N, K);
+  const int rc = check_dense_sizes(dtype, gated, M, N, K);
   if (rc) return rc;
   LO_REQUIRE(tile_m && tile_n && parts, LO_EINVAL, "gemm_bias_act_tile_query: null pointer");
   const DensePlan p = plan_dense(dtype, M, N, K, gated != 0, has_workspace != 0);
@@ -127,7 +130,7 @@ extern "C" int lo_gemm_bias_act(const void *a, int64_t a_stride, const void *b, 
                                 const void *bias, int bias_dtype, int activation, int gated, float scale, const void *residual, int64_t residual_stride,
                                 void *c, int out_dtype, int64_t M, int64_t N, int64_t K, void *workspace, int64_t workspace_bytes, lo_stream_t stream) {
   using namespace lo;
-  const int bad = check_dense_sizes(dtype, M, N, K);
+  const int bad = check_dense_sizes(dtype, gated, M, N, K);
   if (bad) return bad;
   LO_REQUIRE(out_dtype == LO_BF16 || out_dtype == LO_F16 || out_dtype == LO_F32, LO_ENOTSUP, "gemm_bias_act: the output is bf16, fp16 or fp32");
   LO_REQUIRE(activation == LO_ACT_NONE || activation == LO_ACT_SILU || activation == LO_ACT_GELU, LO_EINVAL, "gemm_bias_act: unknown activation %d",

@@ -179,8 +179,8 @@ def gemm_bias_act(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor]
     vocabulary's): ``out = scale * act(a b^T + bias) + residual``, summed and finished in fp32 and rounded once to ``out_dtype``
     (bfloat16, float16 or float32; a's type by default).
 
-    ``a`` [..., K] and ``b`` [N, K] both bfloat16 or both float16, row-major (rows may be strided), any number of rows, any N, K a multiple
-    of 8; ``bias`` [N] of ``out_dtype`` or float32; ``activation`` None, "silu" or "gelu" (its erf form); ``residual`` [..., N] of
+    ``a`` [..., K] and ``b`` [N, K] both bfloat16 or both float16, row-major (rows may be strided), any number of rows and any N up to
+    2^24 and 2^23 (and 2^22 tiles of 256 x 256 results), K a multiple of 8 up to 2097152; ``bias`` [N] of ``out_dtype`` or float32; ``activation`` None, "silu" or "gelu" (its erf form); ``residual`` [..., N] of
     ``out_dtype``.  Written into ``out`` (contiguous) where the caller brings it, ``residual`` itself to update it in place; any other
     overlap is refused."""
     return _dense("gemm_bias_act", a, b, None, None, bias, activation, False, scale, residual, out_dtype or a.dtype, out)
@@ -190,7 +190,7 @@ def gemm_act_and_mul(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tens
                      out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Both projections of a gated block, activation and product in one: ``out = act(a b[:I]^T + bias[:I]) * (a b[I:]^T + bias[I:])``
     with ``b`` [2I, K], the gate's rows first as in the experts' ``w1``; ``activation`` "silu" or "gelu".  Nothing of it is
-    rounded before the result; the rest as in ``gemm_bias_act``."""
+    rounded before the result; the rest as in ``gemm_bias_act`` (tiles of 256 x 128 results)."""
     return _dense("gemm_act_and_mul", a, b, None, None, bias, activation, True, 1.0, None, out_dtype or a.dtype, out)
 
 

@@ -24,3 +24,6 @@ def needs(kind, M, N, K, gated):
     _, _, parts, need = plan(kind, M, N, K, gated)
     assert parts > 1 and need > 0, (kind, M, N, K, gated)
     return need
+
+# Sizes M, N, K (16-bit operands; int8 ones of twice the K take the same) of plain products on tiles of 128 x 256 in parts; columns and K end inside a tile and a K block.
+WIDE = [(18, 18024, 4392), (17, 16969, 5360), (175, 9125, 10984)]

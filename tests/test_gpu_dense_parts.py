@@ -182,3 +182,14 @@ def test_threads():
     assert len(made) == 3
     for outs in made.values():
         assert len(outs) == 60 and all(torch.equal(o, want[i]) for i, o in outs)
+
+
+@pytest.mark.parametrize("M,N,K", parts.WIDE)
+def test_wide_tiles_in_parts(M, N, K):
+    """Tiles of 128 x 256, plain, in parts: ragged tokens, columns and K."""
+    for kind, out, k in ((torch.bfloat16, torch.bfloat16, K), (torch.float16, torch.float32, K), (torch.int8, torch.float16, 2 * K), (torch.int8, torch.float32, 2 * K)):
+        g, ops = _case((kind, M, N, k, False), 6)
+        more = dict(bias=_normal(g, N).to(out), activation="silu", residual=_normal(g, M, N).to(out), scale=0.75)
+        got = _call(*ops, False, out_dtype=out, **more)
+        ref.check(got, ref.dense(*ops, gated=False, **more))
+        assert torch.equal(got, _call(*ops, False, out_dtype=out, **more))

@@ -193,3 +193,26 @@ def test_wide_tiles_in_parts(M, N, K):
         got = _call(*ops, False, out_dtype=out, **more)
         ref.check(got, ref.dense(*ops, gated=False, **more))
         assert torch.equal(got, _call(*ops, False, out_dtype=out, **more))
+
+
+PLAIN_TILES = [(tile, size) for tile, sizes in ref.TILES.items() if not tile[3] for size in sizes[:1]] + [((128, 256, True, False), parts.WIDE[0])]
+
+
+@pytest.mark.parametrize("tile,size", PLAIN_TILES, ids=str)
+def test_strided_residuals_of_every_tile(tile, size):
+    """Residual rows further apart than the result's: on 16 bytes, where they are added in whole pieces, and off them, beside a result whose rows are on
+    them; with values around the residual that would show."""
+    M, N, K = size
+    assert N % 8 == 0
+    for kind, out, k in ((torch.bfloat16, torch.bfloat16, K), (torch.float16, torch.float32, K), (torch.int8, torch.float16, 2 * K)):
+        print("[case] strided residual", tile, kind, M, N, k, flush=True)
+        assert parts.plan(kind, M, N, k, False)[:2] == tile[:2]
+        g = torch.Generator(device="cuda").manual_seed(M + N + k)
+        ops = ref.operands(kind, M, N, k, g)
+        r = _normal(g, M, N).to(out)
+        want = _call(*ops, False, residual=r, scale=-0.5, out_dtype=out)
+        ref.check(want, ref.dense(*ops, residual=r, scale=-0.5))
+        for left, more in ((8, 24), (16, 16), (5, 24), (8, 27)):
+            wide = torch.full((M, N + more), float("nan"), dtype=out, device="cuda")
+            view = wide[:, left:left + N].copy_(r)
+            assert torch.equal(_call(*ops, False, residual=view, scale=-0.5, out_dtype=out), want)

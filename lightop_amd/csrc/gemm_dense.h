@@ -78,7 +78,7 @@ __device__ __forceinline__ float dense_result(const DenseArgs &a, float v, int64
 // their sums up through LDS, in the same order every time.  With C > 1 the 16 rows of a matrix instruction's operands are C K blocks of the
 // workgroup's rows, and of the tokens; of its 16 x 16 sums those on the diagonal of C x C squares count, and are added up with the waves'.
 // Weights are read once, straight into registers, U K blocks of a wave in flight.  HBM bounds it where there are rows enough (one token, gated 2048 x 7168 bf16:
-// 59 MB in 14.4 us; int8 29 MB in 8.8; 16384 x 7168 bf16 5.1 TB/s), else the launch and one round trip (256 x 7168 bf16 4.3 us, 128 x 2048 3.5).
+// 59 MB in 14.4 us; int8 29 MB in 8.8; 7168 x 2048 bf16 29 MB in 8.6), else the launch and one round trip (256 x 7168 bf16 4.3 us, 128 x 2048 3.5).
 template <int DT, int U>
 __global__ __launch_bounds__(512) void gemm_dense_few_kernel(const DenseArgs a, int lg) {
   typedef Operand<DT> Op;
@@ -360,7 +360,8 @@ __device__ __forceinline__ void dense_finish(const DenseArgs &a, const DenseTile
   } else {
     // A wave turns its tokens around in LDS, kRound fragments of them at a time, in fp32 (its own part; LDS operations of a wave execute in
     // order), and stores whole pieces of rows, activated and the residual added: 16 bytes a lane, or, where rows of either do not begin on 16
-    // bytes, a value a lane.
+    // bytes, a value a lane, which takes a round of 256 x 256 tiles 15 to 25 us more (8192 x 4095 x 7168 bf16 389 us, x 4096 354; 4779 x 3354 x 768 71, x 3360 40;
+    // int8 8005 x 3861 x 512 79, x 3864 38; gated 1531 x 767 x 2048 fp16 27.6, x 768 21.3; nothing in parts of K, 333 x 577 x 7168 16.0 and x 576 16.0).
     constexpr int kPitch = kCols * 4 + 16, kRound = dense_round(TM, TN, WM, WN, RING), kRows = kRound * 16;
     int8_t *const stg = smem + t.wave * kRows * kPitch;
     const bool whole = dense_whole(a);
@@ -630,7 +631,7 @@ template <int DT> __global__ __launch_bounds__(256) void gemm_dense_join_kernel(
 template <class K> static int launch_dense_kernel(const DenseArgs &a, K kernel, int lds, int threads, unsigned long long *done, hipStream_t stream) {
   const int rc = reserve_lds_once(reinterpret_cast<const void *>(kernel), lds, done);
   if (rc) return rc;
-  const int group_m = a.m_tiles < 4 ? a.m_tiles : 4;
+  const int group_m = a.m_tiles < 4 ? a.m_tiles : 4; // (2, 4, 8 and 16 are within 3 % of each other: 8192 x 4096 x 7168 bf16 360, 354, 352, 356 us, 2048 x 4096 x 4096 70, 69, 69, 69)
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((a.m_tiles * a.n_tiles + 7) / 8 * 8), a.splits), dim3(threads), lds, stream, a, group_m);
   return LO_OK;
 }

@@ -9,7 +9,9 @@ static int64_t k_blocks(int dtype, int64_t K) { return (K * (dtype == LO_I8 ? 1 
 // tn_us with as many as it holds (LDS); workgroups start and end in `start` us, those of each further round in `again`; the parts are joined by a launch
 // of kJoinUs, and kPartUs for each, that moves them twice at kJoinBytes a us.  The figures are fitted to bf16 and int8 products of 968 sizes (5 to 16384
 // tokens, N 20 to 160000, K 128 to 16384 bytes, plain and gated), each timed with every tile and 1 to 8 parts: the choice is 0.5 % off the fastest on average, 27 % at
-// the most (52 x 2652 x 6656 bf16, gated; three sizes are over 20 %); fits without 200 of the sizes are 0.8 to 1.2 % off for these.  us, by another tile / by the
+// the most (52 x 2652 x 6656 bf16, gated; three sizes are over 20 %); fits without 200 of the sizes are 0.8 to 1.2 % off for these.  Sizes whose rows of C begin
+// on 16 bytes and ones whose rows do not are fitted together, though a round of the two largest tiles ends faster with the former (beside its K blocks 8 to 10 us
+// against 24 to 36, where K has up to 20 of them): `again` lies between.  us, by another tile / by the
 // choice: 2003 x 1536 x 4096 int8, gated 37.2 (128 x 256) / 32.4 (128 x 192), 1531 x 768 x 2048 bf16, gated 23.4 (128 x 128) / 20.6 (96 x 96), 700 x 2048 x 2048 bf16 22.0
 // (128 x 128) / 17.2 (64 x 128), 24 x 7168 x 2048 int8 9.8 (64 x 64) / 7.3 (32 x 32).
 struct DenseTile {
@@ -42,7 +44,9 @@ static DensePlan plan_dense(int dtype, int64_t M, int64_t N, int64_t K, bool gat
     // Waves, and K blocks in flight of each (U): below 512 workgroups all steps at once on as many waves as that takes, from 36 steps on eight waves, one each; between,
     // as many as fit on the card at a time and share its bandwidth evenly, less than 4096 of both; beyond, all steps at once again.  More waves for the results of
     // many tokens.  U divides a wave's steps evenly.  Over 2900 sizes (1 to 16 tokens, 100 to 60000 rows, K 512 to 14336) that were timed with every C, waves and U:
-    // 3.1 % over the fastest on average.  us, by this / one K block in flight: bf16, 1 token 256 x 7168 4.3 / 5.0, 7168 x 2048 8.6 / 9.2, gated 2048 x 7168 14.4 / 14.8.
+    // 3.1 % over the fastest on average, tiles included; 20 sizes are over 20 %, 16 of them of over 10000 rows, 13 x 29696 x 640 bf16 the most (33 %, 14.3 us
+    // against 10.7 by a tile; 1 x 38987 x 768 16.7 against 13.5 by C = 4; these were timed again, as single figures of the 2900 are up to 80 % too high).  The
+    // borders are where the figures change; nothing in the mechanism says where they lie.  us, by this / one K block in flight: bf16, 1 token 256 x 7168 4.3 / 5.0, 7168 x 2048 8.6 / 9.2, gated 2048 x 7168 14.4 / 14.8.
     const int most = gated ? 3 : 4;
     const int64_t rows = gated ? 2 * N : N;
     int lg = 0, waves = 1;

@@ -659,7 +659,7 @@ int lo_fused_experts_fp8(const void *x, int dtype, int64_t M, int64_t H, int64_t
  *   z = residual_scale * residual + scale * act(gate) * h   (act: identity, or the sigmoid with gate_sigmoid)
  *   y = z * (mean(z^2) + eps)^-1/2 * weight                 (nothing of it without weight)
  *   x, residual [M, H] rows of `dtype` x_stride / residual_stride values apart (multiples of 16 bytes); H <= 65536, a
- *   multiple of 8 (q_form with groups: of 128)
+ *   multiple of 8 (q_form with groups: of 128); M < 2^31
  *   gate: NULL, or rows gate_stride values apart, one for gate_rows rows of x: row m takes gate row m / gate_rows, H values
  *   with gate_channels (16-byte aligned rows), else one value
  *   weight, post_weight [H], gate: of `dtype` or LO_F32

@@ -125,7 +125,7 @@ def rms_norm_block(x: torch.Tensor, residual: torch.Tensor, weight: Optional[tor
     ``z = residual_scale * residual + scale * act(gate) * h`` (``act``: none, or ``gate_activation="sigmoid"``),
     ``y = z / sqrt(mean(z^2) + eps) * weight``, from the fp32 z.
 
-    ``x`` and ``residual`` bf16, fp16 or fp32 of one shape (rows may be strided), the last dimension a multiple of 8; ``weight``,
+    ``x`` and ``residual`` bf16, fp16 or fp32 of one shape (rows may be strided, fewer than 2^31), the last dimension a multiple of 8 up to 65536; ``weight``,
     ``post_weight`` [H] and ``gate`` of their type or fp32.  ``gate`` is broadcast to x: [..., 1] a value for a token, [H] or
     [batch, 1, H] one for a channel, x's shape one for each.
 
